@@ -73,12 +73,17 @@ def draw(rng):
 
 # ---------------------------------------------------------------------------------------------- the 4-bit format
 
+def _pow2(e, like):
+    """Exact 2^e of whole numbers, in `like`'s type."""
+    return ((e.long() + 1023) << 52).view(torch.float64).to(like.dtype)
+
+
 def _blocks(v):
     """Values ``[rows, K]`` -> (e2m1 values, exponents): ``[rows, K / 32, 32]`` and ``[rows, K / 32, 1]``."""
     b = v.reshape(v.shape[0], -1, 32)
     mant, ex = torch.frexp(b.abs().amax(2, keepdim=True))
     e = torch.where(mant <= 0.875, ex - 3, ex - 2).clamp(min=-127)
-    y = torch.ldexp(b, -e)
+    y = b * _pow2(-e, b)
     a = y.abs()
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0)).to(v.dtype)
     q = ((a / step).round() * step).clamp(max=6.0)
@@ -88,7 +93,7 @@ def _blocks(v):
 def _rounded(v):
     """The values that 4 bits keep of ``[rows, K]``."""
     q, e = _blocks(v)
-    return torch.ldexp(q, e).reshape(v.shape)
+    return (q * _pow2(e, q)).reshape(v.shape)
 
 
 def _pack(v):
@@ -113,7 +118,7 @@ def _unpack(w4, sf):
     v = table[torch.stack((w4 & 15, w4 >> 4), dim=2).reshape(rows, k).int()]
     tiles, kb = sf.shape[0], sf.shape[1]
     byte = sf.view(tiles, kb, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(tiles * 128, kb * 4)[:rows, :k // 32]
-    return (v.view(rows, k // 32, 32) * torch.exp2(byte.float() - 127).unsqueeze(2)).view(rows, k)
+    return (v.view(rows, k // 32, 32) * _pow2(byte.int() - 127, v).unsqueeze(2)).view(rows, k)
 
 
 # ---------------------------------------------------------------------------------------------- inputs
@@ -279,22 +284,24 @@ def work(case):
     return {"bytes": b, "flops": 2.0 * m * n * k + (a and 2.0 * m * n * RANK)}
 
 
+_TABLE = torch.tensor([2.0 ** e for e in range(-127, 128)], dtype=torch.float64)  # by scale byte
+
+
 def _exact_values(v):
     """float64 ``[rows, K]`` -> what 4 bits keep, by counting the rounding borders that each value is above."""
     b = v.reshape(v.shape[0], v.shape[1] // 32, 32)
     top = b.abs().amax(2)
-    e = torch.floor(torch.log2(torch.where(top > 0, top, torch.ones_like(top)))) - 2
-    for d in (2, 1, 0, -1):  # the smallest e of the four with top <= 7 * 2^e
-        low = torch.floor(torch.log2(torch.where(top > 0, top, torch.ones_like(top)))) - 2 + d
-        e = torch.where(top <= 7 * torch.exp2(low), low, e)
-    e = torch.where(top > 0, e, torch.zeros_like(e)).clamp(min=-127)
-    y = b / torch.exp2(e).unsqueeze(2)
+    # the exponent field of a positive double; 7 = 1.75 * 2^2
+    field, frac = top.view(torch.int64) >> 52, top.view(torch.int64) & ((1 << 52) - 1)
+    e = torch.where(top > 0, field - 1023 - 2 + (frac > 3 << 50).long(), -127).clamp(min=-127)
+    power = _TABLE.to(v.device)[e + 127].unsqueeze(2)
+    y = b / power
     a, out = y.abs(), torch.zeros_like(b)
     # (border, step up, whether the border itself goes up: to the even code)
     for at, up, tie in ((0.25, 0.5, False), (0.75, 0.5, True), (1.25, 0.5, False), (1.75, 0.5, True), (2.5, 1.0, False),
                         (3.5, 1.0, True), (5.0, 2.0, False)):
         out += up * ((a >= at) if tie else (a > at)).double()
-    return (out * y.sign() * torch.exp2(e).unsqueeze(2)).reshape(v.shape)
+    return (out * y.sign() * power).reshape(v.shape)
 
 
 def _exact_weight(w4, sf):
@@ -307,7 +314,7 @@ def _exact_weight(w4, sf):
     r = torch.arange(n, device=w4.device)[:, None]
     blk = torch.arange(k // 32, device=w4.device)[None]
     byte = sf[r // 128, blk // 4, 16 * (r % 32) + 4 * (r % 128 // 32) + blk % 4]
-    return out * torch.exp2(byte.double() - 127).repeat_interleave(32, dim=1)
+    return out * _TABLE.to(w4.device)[byte.long()].repeat_interleave(32, dim=1)
 
 
 def _exact_delta(st, bounds):
