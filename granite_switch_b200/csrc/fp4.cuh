@@ -1,0 +1,99 @@
+// Microscaled 4-bit floating point (MXFP4): device helpers shared by the
+// quantisers (quant_fp4.cu) and the GEMM (gemm_fp4.cu).
+//
+// 32 neighbours along K share one power-of-two scale 2^e (a UE8M0 byte e + 127);
+// each value is e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign. The scale is the
+// smallest with max|x| <= 7 * 2^e: a value above 6 becomes 6, which is off by at
+// most 1, the same half step as between 4 and 6, and normal data lose 3% less
+// (2-norm) than with the smallest scale that keeps every value at or below 6, or
+// with the exponent of max|x| alone. e is at most 125, so that a finite block (its 6 * 2^e)
+// stays finite in bf16: what is above 7 * 2^125 saturates. A block that holds an infinity or a NaN gets
+// the scale byte 255 (NaN) and zero codes, so its products are NaN, as they would
+// be unquantised.
+//
+// Two codes a byte, the lower K in the low nibble. Scale bytes lie in 512-byte
+// atoms, [row tile of 128][K tile of 128][512]: row r's bytes of the tile's four
+// blocks are at 16 (r % 32) + 4 (r / 32). The number of K tiles is even (K padded to
+// 256, one GEMM stage), and the bytes past K are 0.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_fp4.h>
+
+namespace gsb {
+namespace f4 {
+
+constexpr int kBlock = 32;
+
+__host__ __device__ constexpr int64_t k_tiles(int64_t K) { return (K + 255) / 256 * 2; }
+
+// Scale byte of a block whose largest magnitude has the fp32 bits `amax` (sign clear).
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  const int f = (int)(amax >> 23);
+  if (f == 255) return 255u;
+  // 7 = 1.75 * 2^2: the exponent less two, one more when the mantissa is above 1.75
+  return (uint32_t)min(252, max(0, f - 2 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0)));
+}
+
+// 2^-e of a scale byte, exact for 0..252; 0 for 255 (the codes of such a block are 0).
+__device__ __forceinline__ float inv_scale(uint32_t byte) {
+  return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+}
+
+// 2^e of a scale byte: 2^-127 is a subnormal, 255 is NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x400000u : (byte == 255u ? 0x7fc00000u : byte << 23));
+}
+
+// Eight values times `inv` -> eight codes, v[0] in the lowest nibble (round to nearest
+// even, above 6 -> 6).
+__device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_E2M1,
+                                            cudaRoundNearest)
+         << (8 * j);
+  return r;
+}
+
+__device__ __forceinline__ uint32_t max_abs_bits(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);  // NaN bits are above infinity's
+  return m;
+}
+
+// Largest of four neighbouring lanes (one block of 32 values, eight per lane).
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+
+// Offset of the 4-byte word with the scales of row `row`, K tile `kt` (128 values).
+__device__ __forceinline__ int64_t sf_word(int64_t row, int64_t kt, int64_t ktiles) {
+  const int r = (int)(row & 127);
+  return ((row >> 7) * ktiles + kt) * 512 + 16 * (r & 31) + 4 * (r >> 5);
+}
+
+// Quantises eight values per lane of a whole warp (256 neighbours of a row from K index
+// 256 * k2): codes to `codes` (4 bytes a lane, where the lane's values lie before K) and
+// the scale words of both K tiles. Values past K are zero.
+__device__ __forceinline__ void store_warp256(const float (&v)[8], int lane, bool inside, uint8_t* codes, uint8_t* sf,
+                                              int64_t row, int64_t k2, int64_t ktiles) {
+  const uint32_t byte = scale_byte(quad_max(max_abs_bits(v)));
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = byte == 255u ? 0.f : v[j];
+  if (inside) *reinterpret_cast<uint32_t*>(codes) = pack8(w, inv_scale(byte));
+  // lanes 0, 4, 8, 12 hold the first tile's four bytes, 16.. the second's
+  const int base = lane & 16;
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, byte, base + 4 * j) << (8 * j);
+  if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(sf + sf_word(row, 2 * k2 + (lane >> 4), ktiles)) = word;
+}
+
+}  // namespace f4
+}  // namespace gsb

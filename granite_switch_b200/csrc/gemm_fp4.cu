@@ -1,0 +1,682 @@
+// MXFP4 GEMM with the switched-LoRA expand in the same accumulator (tcgen05, TMEM, TMA).
+//
+//   out[M, N] = epi( X4 . W4^T  (e2m1, one UE8M0 scale per 32 along K)  +  S . LB^T  (bf16) )
+//
+// Format of X4, W4 and their scale atoms: fp4.cuh. The MMA is tcgen05.mma
+// kind::mxf4.block_scale with two scales per K = 64 step, so dequantisation costs
+// nothing in the main loop; the LoRA expand appends kind::f16 MMAs to the same fp32
+// accumulator. Epilogues, each with one rounding:
+//   store    bf16(acc * scale)
+//   resadd   bf16(residual + acc * scale)
+//   swiglu   silu(gate) * up quantised to MXFP4 (and, on request, stored as bf16); the
+//            weight rows alternate in runs of 64: gate, up
+//
+// Operand-swapped kernel: the MMA's 128-row side is a tile of weight rows and its N
+// side the step's tokens (up to 256 per CTA), so a weight byte is read once per 256
+// tokens, whatever their number. The K range of a tile is split over the CTAs of a
+// cluster when the tiles alone do not fill the SMs; partial sums meet in distributed
+// shared memory in a fixed order, so results do not depend on timing.
+//
+// Warp roles (192 threads): warp 0 issues the TMA and bulk loads into a ring of
+// stages (256 K elements each), warp 1 owns the tensor memory and issues the scale
+// copies and MMAs, warps 2..5 drain the accumulator; all warps run the epilogue.
+// Every wait is bounded; a CTA that gives up still arrives at the cluster barriers.
+#include "common.cuh"
+#include "fp4.cuh"
+#include "gemm_common.cuh"
+#include "tma_util.h"
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <algorithm>
+#include <utility>
+#include <vector>
+
+namespace gsb {
+namespace f4 {
+
+constexpr int BW = 128;        // weight rows per tile (the MMA's M)
+constexpr int BT = 256;        // tokens per tile (the MMA's N), at most
+constexpr int BKB = 128;       // bytes of K per stage: 256 elements
+constexpr int THREADS = 192;
+constexpr int MAX_STAGES = 8;
+constexpr int MAX_KS = 8;      // portable cluster size
+constexpr int W_BYTES = BW * BKB;
+constexpr int SFW_BYTES = 1024;  // the stage's two scale atoms
+constexpr int P_STRIDE = BW;
+constexpr int SMEM_LIMIT = 227 * 1024;
+constexpr int BAR_BYTES = 256;
+
+struct LoraParams {
+  int blocks_per_adapter;  // rank / 32, times the two halves for swiglu
+  int rank_blocks, num_adapters, num_slices;
+  int slice_bounds[5];
+  const uint64_t* tile_mask;  // [ceil(M / 128)] adapters present per 128 rows, or null: all
+};
+
+struct SplitParams {
+  int M, N, kstages, stages, stage_bytes;
+  int mt_rows;        // tokens per tile
+  int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
+  int tmem_cols;
+  const uint8_t* sfx;
+  const uint8_t* sfw;
+  float scale;
+  void* out;          // bf16 [M, N]; swiglu: bf16 [M, N / 2] or null
+  int64_t ldo;
+  const __nv_bfloat16* residual;
+  int64_t ldr;
+  uint8_t* a4;        // swiglu: codes [M, N / 4] and their scale atoms
+  int64_t lda4;
+  uint8_t* sfa_out;
+  int lora;
+  LoraParams lp;
+};
+
+// Tokens per CTA of a cluster in the reduction: a multiple of 32, so that a 32-column
+// chunk of the accumulator belongs to one CTA.
+__host__ __device__ constexpr int rows_per_part(int rows, int ks) { return ((rows + ks - 1) / ks + 31) / 32 * 32; }
+
+// Instruction descriptor, kind::mxf4 with block scaling: e2m1 A and B, K-major, fp32
+// accumulator, UE8M0 scales; sf_id (0 or 2) picks the byte pair of the 32-bit scale words.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, int sf_id) {
+  return ((uint32_t)sf_id << 4)          // B scale-factor id
+         | (1u << 7) | (1u << 10)        // A, B format: E2M1
+         | ((uint32_t)(N >> 3) << 17)    // N / 8
+         | (1u << 23)                    // scale format: UE8M0
+         | ((uint32_t)(M >> 4) << 24)    // M / 16
+         | ((uint32_t)sf_id << 29);      // A scale-factor id
+}
+
+// Shared-memory descriptor of one scale atom as a tcgen05.cp source: 32 rows of 16
+// bytes, no swizzle, 8-row core matrices 128 bytes apart.
+__device__ __forceinline__ uint64_t sf_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
+}
+
+__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sf_desc(saddr)) : "memory");
+}
+
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t tsfa, uint32_t tsfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+          tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb)
+      : "memory");
+}
+
+// Untiled bulk copy global -> this CTA's shared memory (16-byte aligned, multiples of 16).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int OFF>
+__device__ __forceinline__ void st_dsmem_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0+%2], %1;" ::"r"(addr), "f"(v), "n"(OFF));
+}
+template <int... J>
+__device__ __forceinline__ void push_rows32(uint32_t addr, const uint32_t (&r)[32], std::integer_sequence<int, J...>) {
+  (st_dsmem_f32<J * P_STRIDE * 4>(addr, __uint_as_float(r[J])), ...);
+}
+
+// Adapters present among the rows of 128-row tile `t`.
+__device__ __forceinline__ uint64_t tile_adapters(const LoraParams& l, int t, int tiles) {
+  if (t >= tiles) return 0ull;
+  if (l.tile_mask == nullptr) return (l.num_adapters >= 64) ? ~0ull : ((1ull << l.num_adapters) - 1);
+  return l.tile_mask[t];
+}
+
+__device__ __forceinline__ int slice_base(const LoraParams& l, int row) {
+  int sl = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < l.num_slices && row >= l.slice_bounds[i]) sl = i;
+  return sl * l.num_adapters * l.rank_blocks * 32;
+}
+
+// Column of S (from the slice's first) and of LB of LoRA block j of the adapters in `mask`:
+// adapter by adapter, its rank blocks one after the other. For swiglu each adapter has the
+// gate's blocks, then the up's, whose columns start num_adapters * rank later.
+__device__ __forceinline__ int lora_column(const LoraParams& l, uint64_t mask, int j, int& bit) {
+  const int ai = j / l.blocks_per_adapter, b = j % l.blocks_per_adapter;
+  for (int t = 0; t < ai; ++t) mask &= mask - 1;
+  bit = __ffsll((long long)mask) - 1;
+  return bit * l.rank_blocks * 32 + (b / l.rank_blocks) * l.num_adapters * l.rank_blocks * 32 +
+         (b % l.rank_blocks) * 32;
+}
+
+__device__ __forceinline__ float swiglu_f(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+template <int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
+    mxfp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                       const __grid_constant__ CUtensorMap tm_lb, const __grid_constant__ CUtensorMap tm_s,
+                       const SplitParams p, uint32_t* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], tfull_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ks = p.ks, stages = p.stages;
+  const int part = ks > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = blockIdx.x / ks, n0 = tile * BW;
+  const int m0 = blockIdx.y * BT, rows = min(p.M - m0, p.mt_rows);  // several token tiles: mt_rows == BT
+  const int Mp = (rows + 15) / 16 * 16, xt = (Mp + 127) / 128;
+  const int x_bytes = p.mt_rows > 128 ? BT * BKB : (p.mt_rows + 15) / 16 * 16 * BKB;  // stage layout, same in every CTA
+  const int mtiles128 = (p.M + 127) / 128;
+  const int kb_lo = (int)((int64_t)part * p.kstages / ks), kb_hi = (int)((int64_t)(part + 1) * p.kstages / ks);
+  const int n_main = kb_hi - kb_lo;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&tfull_bar, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    if (p.lora) {
+      tma_prefetch_desc(&tm_lb);
+      tma_prefetch_desc(&tm_s);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, p.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  griddep_launch();
+  griddep_wait();
+
+  uint64_t amask = 0ull, tmask[2] = {0ull, 0ull};
+  if (p.lora) {
+    for (int t = 0; t < xt; ++t) amask |= tmask[t] = tile_adapters(p.lp, m0 / 128 + t, mtiles128);
+  }
+  const int n_lora_all = __popcll(amask) * p.lp.blocks_per_adapter;
+  const int n_lora = n_lora_all > part ? (n_lora_all - part + ks - 1) / ks : 0;
+  const int total = n_main + n_lora;
+  const int acc_cols = (p.mt_rows + 31) / 32 * 32;  // accumulator, then the ring of scales: 8 + 8 xt columns a stage
+
+  if (warp == 0) {
+    // ---------------- producer ----------------
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < total; ++i) {
+        const int s = i % stages;
+        const uint32_t ph = (i / stages) & 1;
+        if (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait)) {
+          abort_flag = 1;
+          break;
+        }
+        uint8_t* sw = smem + s * p.stage_bytes;
+        uint8_t* sx = sw + W_BYTES;
+        uint8_t* sf = sx + x_bytes;
+        if (i < n_main) {
+          const int kb = kb_lo + i;
+          mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
+          tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
+          tma_load_2d(sx, &tm_x, &full_bar[s], kb * BKB, m0);
+          bulk_load(sf, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
+          for (int t = 0; t < xt; ++t)
+            bulk_load(sf + 1024 * (1 + t), p.sfx + ((size_t)(m0 / 128 + t) * p.kstages + kb) * 1024, 1024,
+                      &full_bar[s]);
+        } else {
+          int bit;
+          const int col = lora_column(p.lp, amask, part + (i - n_main) * ks, bit);
+          const int s_rows = min((p.mt_rows + 15) / 16 * 16, 128);  // rows of the S box
+          mbar_arrive_expect_tx(&full_bar[s], BW * 64 + xt * s_rows * 64);
+          tma_load_2d(sw, &tm_lb, &full_bar[s], col, n0);
+          // columns of adapters absent from a 128-row tile were never written: such a tile
+          // reads rows past M, which TMA fills with zeros
+          for (int t = 0; t < xt; ++t)
+            tma_load_2d(sx + t * 128 * 64, &tm_s, &full_bar[s], slice_base(p.lp, n0) + col,
+                        ((tmask[t] >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
+        }
+        ++issued;
+      }
+      if (abort_flag) {
+        // no copy may still be landing in this CTA's shared memory at exit
+        for (int j = max(0, issued - stages); j < issued; ++j)
+          mbar_wait(&full_bar[j % stages], (j / stages) & 1, err, kErrGemmWait);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      const uint32_t idesc_bf = umma_idesc_bf16(BW, Mp);
+      bool ok = true;
+      for (int i = 0; i < total; ++i) {
+        const int s = i % stages;
+        if (abort_flag || !mbar_wait(&full_bar[s], (i / stages) & 1, err, kErrGemmWait)) {
+          abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + s * p.stage_bytes), sx = sw + W_BYTES;
+        if (i < n_main) {
+          // scales: the weights' atoms of both K tiles, then per K tile the tokens' atoms
+          const uint32_t sf = sx + x_bytes, tw = tmem_base + acc_cols + s * (8 + 8 * xt), tx = tw + 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tmem_cp_sf(tw + 4 * h, sf + 512 * h);
+            for (int t = 0; t < xt; ++t) tmem_cp_sf(tx + 4 * (h * xt + t), sf + 1024 * (1 + t) + 512 * h);
+          }
+          const uint64_t ad = umma_desc_sw128(sw), bd = umma_desc_sw128(sx);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_mxf4(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(BW, Mp, 2 * (kk & 1)), tw + 4 * (kk >> 1),
+                      tx + 4 * xt * (kk >> 1), (i | kk) != 0);
+        } else {
+          const uint64_t ad = umma_desc_sw64(sw), bd = umma_desc_sw64(sx);
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) umma_bf16(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_bf, 1);
+        }
+        umma_commit(&empty_bar[s]);
+      }
+      if (ok) umma_commit(&tfull_bar);
+    }
+  }
+
+  // Reduction over the cluster and epilogue. Token m of the tile belongs to CTA m / rows_per;
+  // the drain warps push their fp32 partial rows into the owner's buffer R[part][m - first][128].
+  bool ready = false;
+  if (warp >= 2) {
+    ready = !abort_flag && mbar_wait(&tfull_bar, 0, err, kErrGemmWait);
+    if (!ready) abort_flag = 1;
+    else tc_fence_after();
+  }
+  __syncthreads();
+  if (ks > 1) cluster_sync();  // every main loop is done: the rings are free
+  const int rows_per = p.rows_per;
+  float* R = reinterpret_cast<float*>(smem);
+  if (warp >= 2 && ready) {
+    const int q = warp & 3, n = q * 32 + lane;
+    for (int c = 0, owner = 0, oc = 0; c < rows; c += 32) {
+      if (c - oc >= rows_per) {
+        ++owner;
+        oc += rows_per;
+      }
+      uint32_t r[32];
+      tmem_ld32(tmem_base + c + ((uint32_t)(q * 32) << 16), r);
+      tmem_wait_ld();
+      const int row = part * rows_per + c - oc;
+      if (ks > 1) {
+        push_rows32(mapa_shared(smem_u32(R + row * P_STRIDE + n), (uint32_t)owner), r,
+                    std::make_integer_sequence<int, 32>{});
+      } else {
+        float* dst = R + row * P_STRIDE + n;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) dst[j * P_STRIDE] = __uint_as_float(r[j]);
+      }
+    }
+  }
+  __syncthreads();
+  if (ks > 1) cluster_sync();  // every partial row has landed
+  if (!abort_flag) {
+    const int r0 = part * rows_per, n_rows = max(0, min(rows, r0 + rows_per) - r0);
+    constexpr int GROUPS = (EPI == kEpiSwiGLU) ? 8 : 16;  // 8-column groups per token
+    const int items = n_rows * GROUPS;
+    for (int it = threadIdx.x; it < (items + 31) / 32 * 32; it += THREADS) {
+      const int lm = min(it, items - 1) / GROUPS, c = (it % GROUPS) * 8, m = m0 + r0 + lm;
+      float v[8], u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
+#pragma unroll 1
+      for (int q = 0; q < ks; ++q) {
+        const float* src = R + (q * rows_per + lm) * P_STRIDE + c;
+        const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
+        v[0] += a0.x; v[1] += a0.y; v[2] += a0.z; v[3] += a0.w;
+        v[4] += a1.x; v[5] += a1.y; v[6] += a1.z; v[7] += a1.w;
+        if (EPI == kEpiSwiGLU) {
+          const float4 b0 = *reinterpret_cast<const float4*>(src + 64), b1 = *reinterpret_cast<const float4*>(src + 68);
+          u[0] += b0.x; u[1] += b0.y; u[2] += b0.z; u[3] += b0.w;
+          u[4] += b1.x; u[5] += b1.y; u[6] += b1.z; u[7] += b1.w;
+        }
+      }
+      if (EPI == kEpiSwiGLU) {
+        // four neighbouring items are one block of 32 outputs
+        const int col = tile * 64 + c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = swiglu_f(v[j], u[j]);
+        const uint32_t byte = scale_byte(quad_max(max_abs_bits(v)));
+        if (it < items) {
+          if (p.out != nullptr)
+            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)m * p.ldo + col) = make_uint4(
+                pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+          const int64_t kt = k_tiles(p.N / 2);
+          uint8_t* word = p.sfa_out + sf_word(m, col >> 7, kt);
+          if ((c & 31) == 0) word[(col >> 5) & 3] = (uint8_t)byte;
+          // the last tile also clears the scales past the row's end
+          if (col + 8 == p.N / 2)
+            for (int b = p.N / 64; b < kt * 4; ++b) p.sfa_out[sf_word(m, b >> 2, kt) + (b & 3)] = 0;
+          if (byte == 255u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+          }
+          *reinterpret_cast<uint32_t*>(p.a4 + (int64_t)m * p.lda4 + col / 2) = pack8(v, inv_scale(byte));
+        }
+      } else {
+        const int col = n0 + c;
+        if (it >= items || col >= p.N) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= p.scale;
+        if (EPI == kEpiResAdd) {
+          const uint4 w = *reinterpret_cast<const uint4*>(p.residual + (int64_t)m * p.ldr + col);
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(ww[j]);
+            v[2 * j] += f.x;
+            v[2 * j + 1] += f.y;
+          }
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)m * p.ldo + col) = make_uint4(
+            pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      }
+    }
+  }
+  if (abort_flag) {
+    // error path: MMAs and copies this CTA issued may still be in flight; give them
+    // time to finish before the tensor memory is released (bounded, ~1 ms)
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, p.tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------- host
+constexpr int kMaxDevices = 64;
+
+static int current_device() {
+  int dev = 0;
+  GSB_CUDA_CHECK(cudaGetDevice(&dev));
+  GSB_CHECK(dev >= 0 && dev < kMaxDevices, "mxfp4_gemm: device index out of range");
+  return dev;
+}
+
+static int num_sms() {
+  static int cached[kMaxDevices] = {0};
+  const int dev = current_device();
+  if (!cached[dev])
+    GSB_CUDA_CHECK(cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev));
+  return cached[dev];
+}
+
+// Clusters of `ks` CTAs with `smem` bytes each that fit on the GPU at once (clusters lie
+// inside one GPC, so large ones leave SMs unused). Asked once per device and size.
+static int max_clusters(int ks) {
+  static int cached[kMaxDevices][MAX_KS + 1] = {{0}};
+  const int dev = current_device();
+  if (cached[dev][ks]) return cached[dev][ks];
+  auto kfn = mxfp4_split_kernel<kEpiStore>;
+  GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ks * num_sms()), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = SMEM_LIMIT - BAR_BYTES;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kfn, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = num_sms() / ks;
+  }
+  return cached[dev][ks] = n;
+}
+
+struct SplitPlan {
+  int mt_rows, token_tiles, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes;
+};
+
+// K parts per tile: the most whose clusters all fit at once, with two stages a part at
+// least. The ring takes what shared memory is left, the reduction buffer reuses it.
+static SplitPlan split_plan(int M, int N, int64_t K) {
+  SplitPlan s{};
+  s.mt_rows = std::min(M, BT);
+  s.token_tiles = (M + BT - 1) / BT;
+  s.weight_tiles = (N + BW - 1) / BW;
+  const int kstages = (int)((K + 255) / 256);
+  const int tiles = s.token_tiles * s.weight_tiles;
+  s.ks = 1;
+  for (int ks = 2; ks <= MAX_KS; ++ks)
+    if (kstages / ks >= 2 && tiles <= max_clusters(ks)) s.ks = ks;
+  const int mp = (s.mt_rows + 15) / 16 * 16, xt = (mp + 127) / 128;
+  s.stage_bytes = W_BYTES + (mp > 128 ? BT : mp) * BKB + SFW_BYTES * (1 + xt);
+  const int room = SMEM_LIMIT - BAR_BYTES - 1024;
+  const int reduce = s.ks * rows_per_part(s.mt_rows, s.ks) * P_STRIDE * 4;
+  const int acc = (s.mt_rows + 31) / 32 * 32;
+  s.stages = std::min({MAX_STAGES, room / s.stage_bytes, (512 - acc) / (8 + 8 * xt)});
+  const int cols = acc + s.stages * (8 + 8 * xt);
+  s.tmem_cols = 32;
+  while (s.tmem_cols < cols) s.tmem_cols *= 2;
+  s.smem_bytes = std::max(s.stages * s.stage_bytes, reduce) + 1024;
+  return s;
+}
+
+static bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+static void check_operand(const char* what, const at::Tensor& q, const at::Tensor& sf, int64_t K, const at::Device& dev) {
+  GSB_CHECK(q.is_cuda() && q.device() == dev && sf.device() == dev, "mxfp4_gemm: ", what, " must be on one CUDA device");
+  GSB_CHECK(q.scalar_type() == at::kByte && q.dim() == 2 && q.size(1) * 2 == K && q.stride(1) == 1 &&
+                q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1) && aligned16(q),
+            "mxfp4_gemm: ", what, " codes must be uint8 [rows, K / 2] with 16-byte aligned rows");
+  GSB_CHECK(sf.scalar_type() == at::kByte && sf.is_contiguous() && aligned16(sf) &&
+                sf.numel() == (q.size(0) + 127) / 128 * k_tiles(K) * 512,
+            "mxfp4_gemm: ", what, " scales must be uint8 atoms [ceil(rows / 128), 2 ceil(K / 256), 512]");
+}
+
+static void check_out(const char* what, const at::Tensor& t, int64_t M, int64_t N, const at::Device& dev) {
+  GSB_CHECK(t.device() == dev && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(0) == M &&
+                t.size(1) == N && (N == 1 || t.stride(1) == 1) && (M <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= N)) &&
+                aligned16(t),
+            "mxfp4_gemm: ", what, " must be bf16 [", M, ", ", N, "] with 16-byte aligned rows");
+}
+
+template <int EPI>
+static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tlb, const CUtensorMap& ts,
+                         const SplitParams& p, const SplitPlan& s, uint32_t* err, cudaStream_t st) {
+  auto kfn = mxfp4_split_kernel<EPI>;
+  static bool set[kMaxDevices] = {false};
+  const int dev = current_device();
+  if (!set[dev]) {
+    GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
+    set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(s.weight_tiles * s.ks), (unsigned)s.token_tiles, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = s.smem_bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (s.ks > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)s.ks;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  count_launch();
+  GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, tw, tx, tlb, ts, p, err));
+}
+
+struct LoraArgs {
+  const c10::optional<at::Tensor>& s;
+  const c10::optional<at::Tensor>& lb;
+  const c10::optional<at::Tensor>& tile_mask;
+  int64_t rank, num_adapters;
+  const std::vector<int64_t>& slice_bounds;
+};
+
+// One product on the current stream of x4's device. `a4` / `sfa_out` for swiglu only.
+static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                     const at::Tensor* out, int epi, double scale, const c10::optional<at::Tensor>& residual,
+                     const at::Tensor* a4, const at::Tensor* sfa_out, const LoraArgs& la, const at::Tensor& err) {
+  const at::Device dev = x4.device();
+  GSB_CHECK(x4.dim() == 2 && w4.dim() == 2 && x4.size(1) == w4.size(1), "mxfp4_gemm: operands [M, K / 2] and [N, K / 2] required");
+  const int64_t K = x4.size(1) * 2, M64 = x4.size(0), N64 = w4.size(0);
+  GSB_CHECK(K >= kBlock && K % kBlock == 0 && K < (int64_t(1) << 31), "mxfp4_gemm: K must be a positive multiple of 32");
+  GSB_CHECK(M64 < (int64_t(1) << 24) && N64 > 0 && N64 < (int64_t(1) << 24) && N64 % 8 == 0,
+            "mxfp4_gemm: N must be a positive multiple of 8");
+  check_operand("x", x4, sfx, K, dev);
+  check_operand("w", w4, sfw, K, dev);
+  GSB_CHECK(err.device() == dev, "mxfp4_gemm: error word on another device");
+  const int M = (int)M64, N = (int)N64;
+  SplitParams p{};
+  p.M = M;
+  p.N = N;
+  p.scale = (float)scale;
+  if (epi == kEpiSwiGLU) {
+    GSB_CHECK(N % 128 == 0, "mxfp4_gemm_swiglu: the weight must hold a multiple of 128 rows (64 gate, 64 up, ...)");
+    check_operand("output", *a4, *sfa_out, N / 2, dev);
+    GSB_CHECK(a4->size(0) == M, "mxfp4_gemm_swiglu: output codes must be [M, N / 4]");
+    p.a4 = a4->data_ptr<uint8_t>();
+    p.lda4 = a4->stride(0);
+    p.sfa_out = sfa_out->data_ptr<uint8_t>();
+    if (out != nullptr) check_out("act", *out, M, N / 2, dev);
+  } else {
+    check_out("out", *out, M, N, dev);
+  }
+  if (out != nullptr) {
+    p.out = out->data_ptr();
+    p.ldo = out->stride(0);
+  }
+  if (epi == kEpiResAdd) {
+    GSB_CHECK(residual.has_value(), "mxfp4_gemm: the residual epilogue needs a residual");
+    check_out("residual", *residual, M, N, dev);
+    p.residual = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
+    p.ldr = residual->stride(0);
+  }
+  const bool lora = la.s.has_value() || la.lb.has_value();
+  if (lora) {
+    GSB_CHECK(la.s.has_value() && la.lb.has_value(), "mxfp4_gemm: LoRA needs both s and lb");
+    GSB_CHECK(la.rank > 0 && la.rank % 32 == 0 && la.rank <= 4096 && la.num_adapters >= 1 && la.num_adapters <= 64,
+              "mxfp4_gemm: LoRA rank must be a multiple of 32, with 1 to 64 adapters");
+    const int64_t cols = la.rank * la.num_adapters;
+    const std::vector<int64_t>& b = la.slice_bounds;
+    const int64_t slices = epi == kEpiSwiGLU ? 2 : (int64_t)b.size() - 1;
+    if (epi != kEpiSwiGLU) {
+      GSB_CHECK(b.size() >= 2 && b.size() <= 5 && b.front() == 0 && b.back() == N,
+                "mxfp4_gemm: slice bounds must run from 0 to N (at most 4 slices)");
+      for (size_t i = 0; i + 1 < b.size(); ++i)
+        GSB_CHECK(b[i] % BW == 0 && b[i] < b[i + 1], "mxfp4_gemm: slice bounds must be rising multiples of 128");
+    }
+    const int64_t lb_cols = epi == kEpiSwiGLU ? 2 * cols : cols;
+    GSB_CHECK(la.s->device() == dev && la.lb->device() == dev && la.s->scalar_type() == at::kBFloat16 &&
+                  la.lb->scalar_type() == at::kBFloat16 && la.s->dim() == 2 && la.lb->dim() == 2 &&
+                  la.s->size(0) == M && la.s->size(1) >= slices * cols && la.lb->size(0) == N &&
+                  la.lb->size(1) >= lb_cols && la.s->stride(1) == 1 && la.lb->stride(1) == 1 &&
+                  la.s->stride(0) % 8 == 0 && la.lb->stride(0) % 8 == 0 && aligned16(*la.s) && aligned16(*la.lb),
+              "mxfp4_gemm: bf16 s [M, slices * adapters * rank] and lb [N, ", lb_cols,
+              "] with 16-byte aligned rows required");
+    p.lora = 1;
+    p.lp.rank_blocks = (int)la.rank / 32;
+    p.lp.blocks_per_adapter = p.lp.rank_blocks * (epi == kEpiSwiGLU ? 2 : 1);
+    p.lp.num_adapters = (int)la.num_adapters;
+    p.lp.num_slices = epi == kEpiSwiGLU ? 1 : (int)slices;
+    for (int i = 0; epi != kEpiSwiGLU && i <= slices; ++i) p.lp.slice_bounds[i] = (int)b[i];
+    if (la.tile_mask.has_value()) {
+      GSB_CHECK(la.tile_mask->device() == dev && la.tile_mask->scalar_type() == at::kLong &&
+                    la.tile_mask->is_contiguous() && la.tile_mask->numel() >= (M + 127) / 128,
+                "mxfp4_gemm: tile_mask must hold one int64 per 128-row tile");
+      p.lp.tile_mask = reinterpret_cast<const uint64_t*>(la.tile_mask->data_ptr());
+    }
+  }
+  if (M == 0) return;
+  c10::cuda::CUDAGuard g(dev);
+  auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());
+  p.sfx = sfx.data_ptr<uint8_t>();
+  p.sfw = sfw.data_ptr<uint8_t>();
+
+  const SplitPlan s = split_plan(M, N, K);
+  GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
+  p.kstages = (int)((K + 255) / 256);
+  p.stages = s.stages;
+  p.stage_bytes = s.stage_bytes;
+  p.mt_rows = s.mt_rows;
+  p.ks = s.ks;
+  p.rows_per = rows_per_part(s.mt_rows, s.ks);
+  p.tmem_cols = s.tmem_cols;
+  const uint32_t mp = (uint32_t)((s.mt_rows + 15) / 16 * 16);
+  const CUtensorMap tw = make_tmap_2d(w4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)N, (uint64_t)K / 2,
+                                      (uint64_t)w4.stride(0), BKB, BW, CU_TENSOR_MAP_SWIZZLE_128B);
+  const CUtensorMap tx = make_tmap_2d(x4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)M, (uint64_t)K / 2,
+                                      (uint64_t)x4.stride(0), BKB, mp, CU_TENSOR_MAP_SWIZZLE_128B);
+  CUtensorMap tlb = tw, ts = tx;
+  if (lora) {
+    tlb = make_tmap_bf16_2d(la.lb->data_ptr(), (uint64_t)N, (uint64_t)la.lb->size(1), (uint64_t)la.lb->stride(0), 32,
+                            BW, CU_TENSOR_MAP_SWIZZLE_64B);
+    ts = make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32,
+                           std::min(mp, 128u), CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  switch (epi) {
+    case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, ep, st); break;
+    case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, ep, st); break;
+    default: launch_split<kEpiSwiGLU>(tw, tx, tlb, ts, p, s, ep, st); break;
+  }
+}
+
+}  // namespace f4
+}  // namespace gsb
+
+using namespace gsb;
+
+// out [M, N] bf16 = epi(x4 . w4^T (+ s . lb^T)); epi 0 store (times scale), 1 residual + scale * acc.
+void gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                    const at::Tensor& out, int64_t epi, double scale, const c10::optional<at::Tensor>& residual,
+                    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
+                    const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
+                    std::vector<int64_t> slice_bounds, const at::Tensor& err) {
+  GSB_CHECK(epi == kEpiStore || epi == kEpiResAdd, "mxfp4_gemm: epilogue must be store (0) or residual add (1)");
+  f4::run_gemm(x4, sfx, w4, sfw, &out, (int)epi, scale, residual, nullptr, nullptr,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, slice_bounds}, err);
+}
+
+// a4 / sf <- quantised silu(gate) * up of the gate/up product; `act` also as bf16.
+void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                           const at::Tensor& a4, const at::Tensor& sf, const c10::optional<at::Tensor>& act,
+                           const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
+                           const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
+                           const at::Tensor& err) {
+  const std::vector<int64_t> none;
+  f4::run_gemm(x4, sfx, w4, sfw, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &a4, &sf,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, none}, err);
+}

@@ -91,3 +91,17 @@ int64_t gsb_attn_packed(int64_t v);
 int64_t gsb_gemm_splitk_max_tiles(int64_t v);
 int64_t gsb_attn_fp8t_stages(int64_t v);
 int64_t gsb_attn_decode_stages(int64_t v);
+void gsb_quantize_mxfp4(const at::Tensor& x, const at::Tensor& x4, const at::Tensor& sf);
+void gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps, const at::Tensor& x4,
+                       const at::Tensor& sf, const c10::optional<at::Tensor>& out);
+void gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, const at::Tensor& out);
+void gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                    const at::Tensor& out, int64_t epi, double scale, const c10::optional<at::Tensor>& residual,
+                    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
+                    const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
+                    std::vector<int64_t> slice_bounds, const at::Tensor& err);
+void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                           const at::Tensor& a4, const at::Tensor& sf, const c10::optional<at::Tensor>& act,
+                           const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
+                           const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
+                           const at::Tensor& err);

@@ -1,0 +1,378 @@
+"""MXFP4 quantisers and products against their fp64 statements (GPU).
+
+Tolerances. Quantisation is exact arithmetic up to the comparison with a border, so bytes are equal.
+A product sums K exact terms in fp32: each of the K / 64 accumulations and each sum inside one may lose a
+few units of 2^-24 of the terms' absolute sum, taken as (K / 32 + 16) 2^-23 of it; the output adds bf16's half
+step, 2^-8 of the value. SwiGLU's fp32 exponential and division add 2^-19 of the value.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA")
+    from granite_switch_b200 import _native
+
+    _native.native()  # fail loudly if the extension is missing
+    yield
+    _native.check_errors(torch.device("cuda", torch.cuda.current_device()))
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rows(m, k, seed, spread=6):
+    """bf16 values whose blocks of 32 span several decades, so that a misplaced scale shows."""
+    g = _gen(seed)
+    x = torch.randn(m, k, device="cuda", generator=g)
+    e = torch.randint(-spread, spread + 1, (m, k // 32, 1), device="cuda", generator=g).float()
+    return (x.view(m, k // 32, 32) * 2.0 ** e).view(m, k).to(torch.bfloat16)
+
+
+def _acc_tol(x4, sfx, w4, sfw, extra=0.0):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    k = 2 * x4.shape[1]
+    mass = F.dequantize_reference(x4, sfx).abs() @ F.dequantize_reference(w4, sfw).abs().t() + extra
+    return (k / 32 + 16) * 2.0 ** -23 * mass
+
+
+def _check(out, ref, tol):
+    out = out.double()
+    bad = ~((out - ref).abs() <= tol + ref.abs() * 2.0 ** -8 + 2.0 ** -133)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off; first {bad.nonzero()[0].tolist()}: " \
+                          f"{out[bad][0].item()} vs {ref[bad][0].item()}"
+
+
+def _check_codes(x4, sf, ref, tol):
+    """Codes stand for `ref` to within half a step of their own scale, and the scale is the smallest allowed
+    (or its neighbour where the block's largest value lies within `tol` of the border)."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, k = ref.shape
+    v = F.dequantize_reference(x4, sf).view(m, k // 32, 32)
+    byte = F.scale_bytes_from_atoms(sf, m, k)
+    b, t = ref.view(m, k // 32, 32), tol.view(m, k // 32, 32)
+    lo, hi = F._scale_bytes((b.abs() - t).clamp(min=0).amax(2)), F._scale_bytes((b.abs() + t).amax(2))
+    assert ((byte >= lo) & (byte <= hi)).all()
+    scale = F._pow2(byte.long().unsqueeze(2) - 127)
+    y = b.abs() / scale
+    half = torch.where(y < 2, 0.25, torch.where(y < 4, 0.5, 1.0))
+    # past a binade's border by the tolerance, the step above may already hold
+    half = torch.maximum(half, torch.where((y < 2) & (y + t / scale >= 2), 0.5, half))
+    half = torch.maximum(half, torch.where((y < 4) & (y + t / scale >= 4), 1.0, half))
+    bad = ~((v - b).abs() <= half * scale + t)
+    assert not bad.any(), f"{int(bad.sum())} values off by more than half a step"
+    pad = F.scale_bytes_from_atoms(sf, m, sf.shape[1] * 128)[:, k // 32:]
+    assert not pad.any(), "scales past K must be 0"
+
+
+# ------------------------------------------------------------------------------------------- quantisers
+@pytest.mark.parametrize("m", [1, 3, 128, 257])
+@pytest.mark.parametrize("k", [32, 96, 256, 2080, 4096])
+def test_quantize_matches_reference(m, k):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(m, k, seed=m * 7 + k)
+    x4, sf = F.quantize_rows_mxfp4(x)
+    r4, rsf = F.quantize_rows_reference(x)
+    assert torch.equal(x4, r4)
+    kt = sf.shape[1] * 128
+    assert torch.equal(F.scale_bytes_from_atoms(sf, m, kt), F.scale_bytes_from_atoms(rsf, m, kt))
+    assert torch.equal(F.dequantize_mxfp4(x4, sf).double(), F.dequantize_reference(r4, rsf))
+
+
+def test_quantize_edges_and_strides():
+    """Zeros, subnormals, the largest bf16, borders, infinities and NaN; rows wider than their K; a caller's buffers
+    with rows behind the last one left alone."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    wide = torch.zeros(9, 512, device="cuda", dtype=torch.bfloat16)
+    wide[:, 256:] = 77.0  # neighbours that are not part of the rows
+    x = wide[:, :160]
+    x[1, :32] = torch.tensor(2.0 ** -133)
+    x[2] = torch.finfo(torch.bfloat16).max
+    x[3, :8] = torch.tensor([7.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    x[4, 33] = float("inf")
+    x[5, 2] = float("nan")
+    x[6, 64:96] = -0.0
+    x[7] = torch.randn(160, device="cuda", generator=_gen(1)).to(torch.bfloat16) * 2.0 ** -126
+    x[8, 159] = -float("inf")
+    codes = torch.full((12, 96), 0xAB, dtype=torch.uint8, device="cuda")
+    x4, sf = F.quantize_rows_mxfp4(x, x4=codes[:9, :80])
+    r4, rsf = F.quantize_rows_reference(x)
+    assert torch.equal(x4, r4)
+    assert torch.equal(F.scale_bytes_from_atoms(sf, 9, 256), F.scale_bytes_from_atoms(rsf, 9, 256))
+    assert (codes[9:] == 0xAB).all() and (codes[:, 80:] == 0xAB).all()
+    back = F.dequantize_mxfp4(x4, sf)
+    assert back[4, 32:64].isnan().all() and back[5, :32].isnan().all() and back[8, 128:].isnan().all()
+    assert torch.equal(torch.nan_to_num(back.double()), torch.nan_to_num(F.dequantize_reference(r4, rsf)))
+    assert (back[2].double() == 6 * 2.0 ** 125).all()
+
+
+@pytest.mark.parametrize("m,h", [(1, 32), (5, 256), (33, 2080), (130, 4096), (3, 16384)])
+@pytest.mark.parametrize("with_out", [False, True])
+def test_rmsnorm_quantised(m, h, with_out):
+    from granite_switch_b200.ops import elementwise as E
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    g = _gen(h)
+    x = (torch.randn(m, h, device="cuda", generator=g) * 3).to(torch.bfloat16)
+    w = (1 + 0.2 * torch.randn(h, device="cuda", generator=g)).to(torch.bfloat16)
+    out = torch.empty(m, h, dtype=torch.bfloat16, device="cuda") if with_out else None
+    x4, sf = F.rmsnorm_mxfp4(x, w, 1e-5, out=out)
+    xd = x.double()
+    ref = xd * torch.rsqrt(xd.square().mean(1, keepdim=True) + 1e-5) * w.double()
+    # sum of H squares in fp32, the root and one product: (log2 H + 6) units of 2^-24
+    _check_codes(x4, sf, ref, ref.abs() * (h.bit_length() + 6) * 2.0 ** -23)
+    if with_out:
+        assert torch.equal(out, E.rmsnorm(x, w, 1e-5))
+
+
+def test_quantize_past_32_bits():
+    """Offsets of the last rows pass 2^31 elements."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, k = 66000, 32768
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    tail = _rows(3, k, seed=3)
+    x[-3:] = tail
+    x4, sf = F.quantize_rows_mxfp4(x)
+    r4, rsf = F.quantize_rows_reference(tail)
+    assert torch.equal(x4[-3:], r4)
+    assert torch.equal(F.dequantize_mxfp4(x4, sf)[-3:].double(), F.dequantize_reference(r4, rsf))
+    assert not x4[:-3].any()
+
+
+# ------------------------------------------------------------------------------------------- products
+@pytest.mark.parametrize("m", [1, 16, 77, 128, 200, 300, 600])
+@pytest.mark.parametrize("n,k", [(256, 256), (8, 32), (264, 1056), (1024, 4096), (4096, 288)])
+def test_gemm_store(m, n, k):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=1)), F.quantize_rows_mxfp4(_rows(n, k, seed=2, spread=3))
+    out = F.mxfp4_gemm(*a, *b, scale=0.5)
+    _check(out, 0.5 * F.mxfp4_product_reference(*a, *b), 0.5 * _acc_tol(*a, *b))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (222, 1024, 2080), (2048, 2304, 512), (1300, 4096, 1024)])
+def test_gemm_residual_in_place(m, n, k):
+    """The residual may be the output; rows of a wider, taller buffer are left as they were."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=3)), F.quantize_rows_mxfp4(_rows(n, k, seed=4, spread=2))
+    buf = torch.randn(m + 5, n + 64, device="cuda", generator=_gen(5)).to(torch.bfloat16)
+    keep = buf.clone()
+    h = buf[:m, :n]
+    ref = h.double() + 0.22 * F.mxfp4_product_reference(*a, *b)
+    F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.22, residual=h)
+    _check(h, ref, 0.22 * _acc_tol(*a, *b) + keep[:m, :n].abs().double() * 2.0 ** -23)
+    assert torch.equal(buf[m:], keep[m:]) and torch.equal(buf[:, n:], keep[:, n:])
+
+
+def _lora_inputs(m, n, slices, na, rank, seed, absent=2):
+    """Masked shrink output as the shrink leaves it: zero for other adapters of a 128-row tile, old values (NaN
+    here) in the columns of adapters that no row of the tile uses."""
+    g = _gen(seed)
+    ra = torch.randint(0, na + 1, (m,), device="cuda", generator=g)
+    ra[ra == absent] = 0
+    if m > 128:
+        ra[128:] = torch.where(ra[128:] == 1, 0, ra[128:])  # adapter 1 only in the first tile
+    cols = slices * na * rank
+    col = (torch.arange(cols, device="cuda") // rank) % na + 1
+    s = torch.randn(m, cols, device="cuda", generator=g) * (col == ra[:, None])
+    tiles = (m + 127) // 128
+    mask = torch.zeros(tiles, dtype=torch.int64)
+    dirty = s.clone()
+    for t in range(tiles):
+        here = set(ra[t * 128:(t + 1) * 128].tolist()) - {0}
+        mask[t] = sum(1 << (a - 1) for a in here)
+        gone = torch.tensor([int(c) not in here for c in col.tolist()], device="cuda")
+        dirty[t * 128:(t + 1) * 128, gone] = float("nan")
+    lb = (torch.randn(n, na * rank, device="cuda", generator=g) * 0.5).to(torch.bfloat16)
+    return s.to(torch.bfloat16), dirty.to(torch.bfloat16), lb, mask.cuda()
+
+
+@pytest.mark.parametrize("m", [1, 5, 130, 300, 1100])
+@pytest.mark.parametrize("bounds", [[0, 640], [0, 1024, 1280, 1536], [0, 384, 512, 2176]])
+def test_gemm_lora_slices(m, bounds):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    k, na, rank, n = 512, 5, 64, bounds[-1]
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=6)), F.quantize_rows_mxfp4(_rows(n, k, seed=7, spread=2))
+    s, dirty, lb, mask = _lora_inputs(m, n, len(bounds) - 1, na, rank, seed=8)
+    kw = dict(lb=lb, rank=rank, num_adapters=na, slice_bounds=bounds)
+    ref = F.mxfp4_product_reference(*a, *b, s=s, **kw)
+    tol = _acc_tol(*a, *b, extra=(s.double().abs().sum(1, keepdim=True) * lb.double().abs().max()))
+    _check(F.mxfp4_gemm(*a, *b, s=dirty, tile_mask=mask, **kw), ref, tol)
+    _check(F.mxfp4_gemm(*a, *b, s=s, **kw), ref, tol)  # without a mask every adapter is expanded
+
+
+@pytest.mark.parametrize("m,i,h", [(1, 64, 64), (17, 192, 512), (130, 1600, 256), (300, 512, 1056), (1300, 4096, 512)])
+@pytest.mark.parametrize("lora", [False, True])
+def test_gemm_swiglu(m, i, h, lora):
+    from granite_switch_b200.models.packing import interleave_gate_up
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    a = F.quantize_rows_mxfp4(_rows(m, h, seed=9, spread=1))
+    w = interleave_gate_up(_rows(2 * i, h, seed=10, spread=1) * h ** -0.5, F.SWIGLU_TILE)
+    b = F.quantize_rows_mxfp4(w)
+    kw, kd, extra = {}, {}, 0.0
+    if lora:
+        s, dirty, lb, mask = _lora_inputs(m, 2 * i, 2, 3, 32, seed=11)
+        lb2 = F.swiglu_lora_b(lb)
+        kw = dict(lb=lb2, rank=32, num_adapters=3)
+        kd = dict(s=dirty, tile_mask=mask)
+        extra = s.double().abs().sum(1, keepdim=True) * lb.double().abs().max()
+        acc = F.mxfp4_product_reference(*a, *b, s=s, **kw)
+    else:
+        acc = F.mxfp4_product_reference(*a, *b)
+    act = torch.full((m + 2, i), 5.0, dtype=torch.bfloat16, device="cuda")
+    a4, sf = F.mxfp4_gemm_swiglu(*a, *b, act=act[:m], **kw, **kd)
+    ref = F.swiglu_reference(acc)
+    t = _acc_tol(*a, *b, extra=extra).view(m, -1, 2, 64)
+    v = acc.view(m, -1, 2, 64)
+    # |silu'| <= 1.1
+    tol = (1.1 * v[:, :, 1].abs() * t[:, :, 0] + v[:, :, 0].abs() * t[:, :, 1] + t[:, :, 0] * t[:, :, 1]).reshape(m, i)
+    tol = tol + ref.abs() * 2.0 ** -19
+    _check(act[:m], ref, tol)
+    assert (act[m:] == 5.0).all()
+    _check_codes(a4, sf, ref, tol)
+    b4, bsf = F.mxfp4_gemm_swiglu(*a, *b, **kw, **kd)
+    assert torch.equal(a4, b4) and torch.equal(F.scale_bytes_from_atoms(sf, m, i), F.scale_bytes_from_atoms(bsf, m, i))
+
+
+@pytest.mark.parametrize("m", [2, 190, 1025])
+def test_mlp_block(m):
+    """Norm, gate/up, SwiGLU and down projection as a decoder runs them, each stage against fp64 on its own input."""
+    from granite_switch_b200.models.packing import interleave_gate_up
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    h, i = 512, 1088
+    g = _gen(12)
+    x = torch.randn(m, h, device="cuda", generator=g).to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(h, device="cuda", generator=g)).to(torch.bfloat16)
+    gu = torch.randn(2 * i, h, device="cuda", generator=g).to(torch.bfloat16) * h ** -0.5
+    down = torch.randn(h, i, device="cuda", generator=g).to(torch.bfloat16) * i ** -0.5
+    gu4, dn4 = F.quantize_rows_mxfp4(interleave_gate_up(gu, F.SWIGLU_TILE)), F.quantize_rows_mxfp4(down)
+    xq = F.rmsnorm_mxfp4(x, w, 1e-5)
+    aq = F.mxfp4_gemm_swiglu(*xq, *gu4)
+    out = F.mxfp4_gemm(*aq, *dn4, epi=F.EPI_RESADD, scale=0.22, residual=x)
+    ref = x.double() + 0.22 * F.mxfp4_product_reference(*aq, *dn4)
+    _check(out, ref, 0.22 * _acc_tol(*aq, *dn4) + x.double().abs() * 2.0 ** -23)
+    # against the whole block in fp64 from the same 4-bit weights: only rounding borders differ
+    full = F.swiglu_reference(F.mxfp4_product_reference(*xq, *gu4))
+    full = F.dequantize_reference(*F.quantize_rows_reference(full)) @ F.dequantize_reference(*dn4).t()
+    assert ((out.double() - x.double() - 0.22 * full).norm() / (0.22 * full).norm()).item() < 2.0 ** -6
+
+
+def test_nan_and_empty():
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(20, 512, seed=13)
+    x[3, 100] = float("inf")
+    b = F.quantize_rows_mxfp4(_rows(256, 512, seed=14, spread=1))
+    out = F.mxfp4_linear(x, *b)
+    assert out[3].isnan().all()
+    rest = torch.arange(20, device="cuda") != 3
+    assert out[rest].isfinite().all()
+    none = torch.empty(0, 512, dtype=torch.bfloat16, device="cuda")
+    assert F.mxfp4_linear(none, *b).shape == (0, 256)
+    a4, _ = F.mxfp4_gemm_swiglu(*F.rmsnorm_mxfp4(none, torch.ones(512, device="cuda").bfloat16(), 1e-5), *b)
+    assert a4.shape == (0, 64)
+
+
+def test_output_past_32_bits():
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, n, k = 264000, 8192, 64
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-2:] = _rows(2, k, seed=15, spread=1)
+    b = F.quantize_rows_mxfp4(_rows(n, k, seed=16, spread=1))
+    out = F.mxfp4_linear(x, *b)
+    a = F.quantize_rows_mxfp4(x[-2:])
+    _check(out[-2:], F.mxfp4_product_reference(*a, *b), _acc_tol(*a, *b))
+    assert not out[-300:-2].any()
+
+
+def test_streams_and_graphs():
+    """A call on another stream, and a captured pass replayed on new inputs, give the eager result bit for bit."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, n, k = 48, 1024, 2048
+    xs = [_rows(m, k, seed=s, spread=1) for s in (17, 18)]
+    b = F.quantize_rows_mxfp4(_rows(n, k, seed=19, spread=1))
+    want = [F.mxfp4_linear(x, *b) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = F.mxfp4_linear(xs[0], *b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want[0])
+    x = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.mxfp4_linear(x, *b)
+    for src, ref in zip(xs[::-1], want[::-1]):
+        x.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+
+
+def test_programmatic_launch_matches():
+    """Launched as programmatic dependents, with weights quantised just before, results are the same."""
+    from granite_switch_b200._native import native
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x, w = _rows(64, 2048, seed=20, spread=1), _rows(2048, 2048, seed=21, spread=1)
+    want = F.mxfp4_linear(x, *F.quantize_rows_mxfp4(w))
+    old = native().set_pdl(True)
+    try:
+        for _ in range(20):
+            assert torch.equal(F.mxfp4_linear(x, *F.quantize_rows_mxfp4(w)), want)
+    finally:
+        native().set_pdl(old)
+
+
+def test_refusals():
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(16, 256, seed=22)
+    a, b = F.quantize_rows_mxfp4(x), F.quantize_rows_mxfp4(_rows(256, 256, seed=23))
+    out = torch.empty(16, 256, dtype=torch.bfloat16, device="cuda")
+    bad = [
+        lambda: F.quantize_rows_mxfp4(x.float()),
+        lambda: F.quantize_rows_mxfp4(x[:, 1:33]),                                  # not 16-byte aligned
+        lambda: F.quantize_rows_mxfp4(x.t()),
+        lambda: F.quantize_rows_mxfp4(x, sf=a[1][:, :1]),
+        lambda: F.quantize_rows_mxfp4(x, x4=a[0][:8]),
+        lambda: F.rmsnorm_mxfp4(x, torch.ones(128, device="cuda").bfloat16(), 1e-5),
+        lambda: F.rmsnorm_mxfp4(x, torch.ones(256, device="cuda"), 1e-5),
+        lambda: F.dequantize_mxfp4(*a, out=torch.empty(16, 128, dtype=torch.bfloat16, device="cuda")),
+        lambda: F.mxfp4_gemm(a[0][:, :64], a[1], *b),                               # K differs
+        lambda: F.mxfp4_gemm(*a, b[0], a[1]),                                       # too few scales
+        lambda: F.mxfp4_gemm(*a, b[0][:252], b[1]),                                 # N not a multiple of 8
+        lambda: F.mxfp4_gemm(*a, *b, out=out.float()),
+        lambda: F.mxfp4_gemm(*a, *b, out=out[:8]),
+        lambda: F.mxfp4_gemm(*a, *b, epi=F.EPI_RESADD),
+        lambda: F.mxfp4_gemm(*a, *b, epi=2),
+        lambda: F.mxfp4_gemm(*a, *b, s=out),
+        lambda: F.mxfp4_gemm(*a, *b, s=out, lb=b[0].bfloat16(), rank=16, num_adapters=2),
+        lambda: F.mxfp4_gemm(*a, *b, s=out, lb=b[0].bfloat16(), rank=32, num_adapters=65),
+        lambda: F.mxfp4_gemm(*a, *b, s=out, lb=b[0].bfloat16(), rank=32, num_adapters=2, slice_bounds=[0, 100, 256]),
+        lambda: F.mxfp4_gemm(*a, *b, s=out, lb=b[0].bfloat16(), rank=32, num_adapters=16),  # s too narrow
+        lambda: F.mxfp4_gemm(*a, *b, s=out, lb=b[0].bfloat16(), rank=32, num_adapters=2,
+                             tile_mask=torch.zeros(1, dtype=torch.int32, device="cuda")),
+        lambda: F.mxfp4_gemm_swiglu(*a, b[0][:192], torch.empty(2, 2, 512, dtype=torch.uint8, device="cuda")),
+        lambda: F.mxfp4_gemm(a[0].cpu(), a[1], *b),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+            pytest.fail(f"call {i} was accepted")
