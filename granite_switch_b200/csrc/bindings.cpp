@@ -68,6 +68,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dequantize_mxfp4", &gsb_dequantize_mxfp4, "MXFP4 codes and scale atoms -> bf16 rows");
   m.def("mxfp4_gemm", &gsb_mxfp4_gemm, "MXFP4 tcgen05 GEMM with the bf16 switched-LoRA expand fused");
   m.def("mxfp4_gemm_swiglu", &gsb_mxfp4_gemm_swiglu, "MXFP4 gate/up GEMM, SwiGLU and MXFP4 quantisation in the epilogue");
+  m.def("mxfp4_pair_min_m", &gsb_mxfp4_pair_min_m,
+        "set the smallest M of the CTA-pair MXFP4 GEMM (negative: only reads; returns the old value)");
   m.def("rope_kv_fp8", &gsb_rope_kv_fp8, "RoPE on q / k then the quantised fp8 K / V write, one launch");
   m.def("kv_write_fp8", &gsb_kv_write_fp8, "quantised (e4m3, per-row scale) write of a step's K/V into the fp8 cache");
 }

@@ -409,6 +409,368 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
+// ---------------------------------------------------------------------------
+// CTA-pair kernel (cta_group::2) for many tokens: a cluster of two CTAs computes
+// 256 tokens x 256 weight rows. Each CTA stages its own 128 tokens and 128 weight rows
+// per 256-K stage (half the weight bytes that a single CTA's 128 x 256 tile takes in per
+// MMA; the 4-bit MMA eats 48 KB of operands in 512 cycles otherwise, which is the L2's
+// whole rate), and the scales of its tokens and of all 256 weight rows. The leader's MMA
+// thread issues the scale copies and MMAs for both CTAs. Persistent: one cluster per SM
+// pair walks the tiles.
+//
+// One 256-column accumulator and the ring of scales fill the tensor memory, so the
+// epilogue empties the accumulator into registers at once (eight warps, 128 columns each)
+// and gives it back before it converts and stores: the next tile's MMAs run meanwhile.
+// ---------------------------------------------------------------------------
+struct PairCfg {
+  static constexpr int THREADS = 320;  // warp 0 loads, warp 1 MMAs, warps 2..9 epilogue
+  static constexpr int BN = 256;
+  static constexpr int A_BYTES = 128 * BKB, B_BYTES = 128 * BKB;
+  static constexpr int SFA_OFF = A_BYTES + B_BYTES, SFB_OFF = SFA_OFF + 1024;
+  static constexpr int STAGE_BYTES = SFB_OFF + 2048;
+  static constexpr int STAGES = 5;
+  static constexpr int SF_COLS = 24;   // per stage: tokens 2 x 4 columns, weights 2 x 8
+  static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
+  static constexpr int STAGING = 4096;  // per epilogue warp: 32 rows x 128 bytes
+  static constexpr int SMEM_BYTES = STAGING_OFF + 8 * STAGING + 1024;
+};
+static_assert(PairCfg::STAGE_BYTES % 1024 == 0 && PairCfg::SMEM_BYTES <= SMEM_LIMIT - BAR_BYTES, "shared memory");
+static_assert(PairCfg::BN + PairCfg::STAGES * PairCfg::SF_COLS <= 512, "tensor memory");
+
+struct PairParams {
+  int M, N, kstages;
+  float scale;
+  void* out;
+  int64_t ldo;
+  const __nv_bfloat16* residual;
+  int64_t ldr;
+  uint8_t* a4;
+  int64_t lda4;
+  uint8_t* sfa_out;
+  int lora;
+  LoraParams lp;
+};
+
+// 3-D tiled load into this CTA's shared memory, completing on a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int32_t x,
+                                                 int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Scale atoms of both CTAs (the same offset in each one's shared memory) into both tensor memories.
+__device__ __forceinline__ void tmem_cp_sf_pair(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sf_desc(saddr)) : "memory");
+}
+
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t tsfa, uint32_t tsfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+          tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb)
+      : "memory");
+}
+
+// Tile order: columns of 8 token tiles walk the weight tiles, so that concurrent clusters share both in L2.
+__device__ __forceinline__ void pair_tile(int t, int m_tiles, int n_tiles, int& mt, int& nt) {
+  const int group = t / (8 * n_tiles), first = group * 8, size = min(8, m_tiles - first), in = t - group * 8 * n_tiles;
+  mt = first + in % size;
+  nt = in / size;
+}
+
+__device__ __forceinline__ uint32_t swz128(int row, int chunk) {
+  return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
+    mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_sfx, const __grid_constant__ CUtensorMap tm_sfw,
+                      const __grid_constant__ CUtensorMap tm_s, const __grid_constant__ CUtensorMap tm_lb,
+                      const __grid_constant__ CUtensorMap tm_out, const PairParams p, uint32_t* err) {
+  using C = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full_bar[C::STAGES], empty_bar[C::STAGES], tfull_bar, tempty_bar;  // full, tempty: the leader's
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int mtiles128 = (p.M + 127) / 128;
+  const int m_tiles = (p.M + 255) / 256, n_tiles = (p.N + C::BN - 1) / C::BN, num_tiles = m_tiles * n_tiles;
+  const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&tfull_bar, 1);
+    mbar_init(&tempty_bar, 16);  // one arrival per epilogue warp of both CTAs
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_sfx);
+    tma_prefetch_desc(&tm_sfw);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers are initialised before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  griddep_launch();
+  griddep_wait();
+
+  if (warp == 0) {
+    // ---------------- producer (both CTAs) ----------------
+    if (lane == 0) {
+      const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
+      uint32_t kb = 0;
+      bool stop = false;
+      for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters) {
+        int mt, nt;
+        pair_tile(t, m_tiles, n_tiles, mt, nt);
+        const int own = 2 * mt + (int)rank, m0 = own * 128, n0 = nt * C::BN;
+        uint64_t mask[2] = {0ull, 0ull};
+        if (p.lora) {
+          mask[0] = tile_adapters(p.lp, 2 * mt, mtiles128);
+          mask[1] = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
+        }
+        const uint64_t both = mask[0] | mask[1], mine = rank ? mask[1] : mask[0];
+        const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
+        for (int i = 0; i < total; ++i, ++kb) {
+          const int s = kb % C::STAGES;
+          if (abort_flag || !mbar_wait(&empty_bar[s], ((kb / C::STAGES) & 1) ^ 1, err, kErrGemmWait)) {
+            abort_flag = 1;
+            stop = true;
+            break;
+          }
+          uint8_t* sa = smem + s * C::STAGE_BYTES;
+          uint8_t* sb = sa + C::A_BYTES;
+          const uint32_t fb = full_leader + s * 8;
+          if (i < p.kstages) {
+            // tiles past the last row are zeros, scales too
+            if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+            tma_load_2d_pair(sa, &tm_x, fb, i * BKB, m0);
+            tma_load_2d_pair(sb, &tm_w, fb, i * BKB, n0 + (int)rank * 128);
+            tma_load_3d_pair(sa + C::SFA_OFF, &tm_sfx, fb, 0, i, own);
+            tma_load_3d_pair(sa + C::SFB_OFF, &tm_sfw, fb, 0, i, 2 * nt);
+          } else {
+            // two halves of 128 weight rows, each with its slice's S columns; either CTA
+            // stages 64 rows of each half of LB. A tile that lacks the adapter reads zeros.
+            int bit;
+            const int col = lora_column(p.lp, both, i - p.kstages, bit);
+            if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * (2 * 128 * 64 + 128 * 64));
+            const int y = ((mine >> bit) & 1ull) ? m0 : mtiles128 * 128;
+            tma_load_2d_pair(sa, &tm_s, fb, slice_base(p.lp, n0) + col, y);
+            tma_load_2d_pair(sa + 128 * 64, &tm_s, fb, slice_base(p.lp, n0 + 128) + col, y);
+            tma_load_2d_pair(sb, &tm_lb, fb, col, n0 + (int)rank * 64);
+            tma_load_2d_pair(sb + 64 * 64, &tm_lb, fb, col, n0 + 128 + (int)rank * 64);
+          }
+        }
+      }
+      // the pair MMA has released every stage this CTA filled before the CTA may exit
+      for (uint32_t j = kb > (uint32_t)C::STAGES ? kb - C::STAGES : 0; j < kb && !abort_flag; ++j)
+        if (!mbar_wait(&empty_bar[j % C::STAGES], (j / C::STAGES) & 1, err, kErrGemmWait)) abort_flag = 1;
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader only) ----------------
+    if (leader && lane == 0) {
+      uint32_t kb = 0;
+      int ltile = 0;
+      bool stop = false;
+      for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters, ++ltile) {
+        int mt, nt;
+        pair_tile(t, m_tiles, n_tiles, mt, nt);
+        int total = p.kstages;
+        if (p.lora)
+          total += __popcll(tile_adapters(p.lp, 2 * mt, mtiles128) | tile_adapters(p.lp, 2 * mt + 1, mtiles128)) *
+                   p.lp.blocks_per_adapter;
+        if (abort_flag || !mbar_wait(&tempty_bar, (ltile & 1) ^ 1, err, kErrGemmWait)) {
+          abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        for (int i = 0; i < total; ++i, ++kb) {
+          const int s = kb % C::STAGES;
+          if (abort_flag || !mbar_wait(&full_bar[s], (kb / C::STAGES) & 1, err, kErrGemmWait)) {
+            abort_flag = 1;
+            stop = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * C::STAGE_BYTES), sb = sa + C::A_BYTES;
+          if (i < p.kstages) {
+            const uint32_t ta = tmem_base + C::BN + s * C::SF_COLS, tb = ta + 8;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              tmem_cp_sf_pair(ta + 4 * h, sa + C::SFA_OFF + 512 * h);
+              tmem_cp_sf_pair(tb + 8 * h, sa + C::SFB_OFF + 512 * h);
+              tmem_cp_sf_pair(tb + 8 * h + 4, sa + C::SFB_OFF + 1024 + 512 * h);
+            }
+            const uint64_t ad = umma_desc_sw128(sa), bd = umma_desc_sw128(sb);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_mxf4_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(256, C::BN, 2 * (kk & 1)),
+                             ta + 4 * (kk >> 1), tb + 8 * (kk >> 1), (i | kk) != 0);
+          } else {
+            const uint32_t idesc = umma_idesc_bf16(256, 128);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint64_t ad = umma_desc_sw64(sa + u * 128 * 64), bd = umma_desc_sw64(sb + u * 64 * 64);
+#pragma unroll
+              for (int kk = 0; kk < 2; ++kk) umma_bf16_pair(tmem_base + u * 128, ad + 2 * kk, bd + 2 * kk, idesc, 1);
+            }
+          }
+          umma_commit_pair(&empty_bar[s], 0x3);
+        }
+        if (stop) break;
+        umma_commit_pair(&tfull_bar, 0x3);
+      }
+    }
+  } else {
+    // ---------------- epilogue: TMEM lane quarter warp % 4, columns 128 half .. ----------------
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* buf = smem + C::STAGING_OFF + (warp - 2) * C::STAGING;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty_bar), 0);
+    int ltile = 0;
+    for (int t = cluster_id; t < num_tiles; t += num_clusters, ++ltile) {
+      int mt, nt;
+      pair_tile(t, m_tiles, n_tiles, mt, nt);
+      if (abort_flag || !mbar_wait(&tfull_bar, ltile & 1, err, kErrGemmWait)) {
+        abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      uint32_t r[4][32];
+      const uint32_t tb = tmem_base + half * 128 + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(tb + 32 * c, r[c]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      const int row0 = mt * 256 + (int)rank * 128 + q * 32, row = row0 + lane, n0 = nt * C::BN + half * 128;
+      if (row0 >= p.M || n0 >= p.N) continue;
+      if constexpr (EPI == kEpiSwiGLU) {
+        // columns 0..63 gate, 64..127 up: two blocks of 32 outputs of one row
+        const int col = n0 / 2;
+        const int64_t kt = k_tiles(p.N / 2);
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          float v[4][8];
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v[j / 8][j % 8] = swiglu_f(__uint_as_float(r[b][j]), __uint_as_float(r[2 + b][j]));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) top = max(top, max_abs_bits(v[g]));
+          const uint32_t byte = scale_byte(top);
+          bytes |= byte << (8 * b);
+          if (row >= p.M) continue;
+          if (p.out != nullptr) {
+            uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ldo + col +
+                                                32 * b);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              o[g] = make_uint4(pack_bf16x2(v[g][0], v[g][1]), pack_bf16x2(v[g][2], v[g][3]),
+                                pack_bf16x2(v[g][4], v[g][5]), pack_bf16x2(v[g][6], v[g][7]));
+          }
+          if (byte == 255u) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j / 8][j % 8] = 0.f;
+          }
+          const float inv = inv_scale(byte);
+          *reinterpret_cast<uint4*>(p.a4 + (int64_t)row * p.lda4 + col / 2 + 16 * b) =
+              make_uint4(pack8(v[0], inv), pack8(v[1], inv), pack8(v[2], inv), pack8(v[3], inv));
+        }
+        if (row < p.M) {
+          *reinterpret_cast<uint16_t*>(p.sfa_out + sf_word(row, col >> 7, kt) + ((col >> 5) & 3)) = (uint16_t)bytes;
+          // the last columns' warp also clears the scales past the row's end
+          if (n0 + 128 == p.N)
+            for (int b = p.N / 64; b < kt * 4; ++b) p.sfa_out[sf_word(row, b >> 2, kt) + (b & 3)] = 0;
+        }
+      } else {
+        // 64 columns at a time through a swizzled buffer: coalesced residual reads, one TMA store
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = n0 + 64 * h;
+          if (col >= p.N) break;
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          if (EPI == kEpiResAdd) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int rr = 4 * j + (lane >> 3), ch = lane & 7;
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (row0 + rr < p.M && col + ch * 8 < p.N)
+                w = *reinterpret_cast<const uint4*>(p.residual + (int64_t)(row0 + rr) * p.ldr + col + ch * 8);
+              *reinterpret_cast<uint4*>(buf + swz128(rr, ch)) = w;
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            uint4* cell = reinterpret_cast<uint4*>(buf + swz128(lane, ch));
+            float2 f[4] = {};
+            if (EPI == kEpiResAdd) {
+              const uint4 w = *cell;
+              f[0] = unpack_bf16x2(w.x);
+              f[1] = unpack_bf16x2(w.y);
+              f[2] = unpack_bf16x2(w.z);
+              f[3] = unpack_bf16x2(w.w);
+            }
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int at = 8 * ch + 2 * j;
+              const float a = __uint_as_float(r[2 * h + at / 32][at % 32]) * p.scale;
+              const float b = __uint_as_float(r[2 * h + at / 32][at % 32 + 1]) * p.scale;
+              o[j] = EPI == kEpiResAdd ? pack_bf16x2(a + f[j].x, b + f[j].y) : pack_bf16x2(a, b);
+            }
+            *cell = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tm_out, buf, col, row0);
+            bulk_commit_group();
+          }
+        }
+      }
+    }
+    if (EPI != kEpiSwiGLU && lane == 0) bulk_wait_group_all();
+  }
+
+  if (abort_flag) {
+    // error path: copies and MMAs may still be in flight (bounded, ~1 ms)
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------- host
 constexpr int kMaxDevices = 64;
 
@@ -453,6 +815,9 @@ static int max_clusters(int ks) {
   }
   return cached[dev][ks] = n;
 }
+
+// Smallest M of the pair kernel (gsb_mxfp4_pair_min_m changes it for A/B runs).
+static int g_pair_min_m = 512;
 
 struct SplitPlan {
   int mt_rows, token_tiles, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes;
@@ -535,6 +900,54 @@ static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUt
   cfg.numAttrs = n;
   count_launch();
   GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, tw, tx, tlb, ts, p, err));
+}
+
+// Clusters of two of the pair kernel that fit at once (asked once per device and epilogue).
+template <int EPI>
+static int pair_clusters() {
+  static int cached[kMaxDevices] = {0};
+  const int dev = current_device();
+  if (cached[dev]) return cached[dev];
+  auto kfn = mxfp4_pair_kernel<EPI>;
+  GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::SMEM_BYTES));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(num_sms() / 2 * 2), 1, 1);
+  cfg.blockDim = dim3(PairCfg::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  GSB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kfn, &cfg));
+  return cached[dev] = std::max(1, n);
+}
+
+template <int EPI>
+static void launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& tsfx, const CUtensorMap& tsfw,
+                        const CUtensorMap& ts, const CUtensorMap& tlb, const CUtensorMap& to, const PairParams& p,
+                        uint32_t* err, cudaStream_t st) {
+  const int tiles = ((p.M + 255) / 256) * ((p.N + PairCfg::BN - 1) / PairCfg::BN);
+  const int clusters = std::min(tiles, pair_clusters<EPI>());  // also sets the shared-memory attribute
+  launch_dependent(mxfp4_pair_kernel<EPI>, dim3(2 * clusters), dim3(PairCfg::THREADS), PairCfg::SMEM_BYTES, st, tx, tw,
+                   tsfx, tsfw, ts, tlb, to, p, err);
+}
+
+// Scale atoms [tiles, K stages, 1024 bytes]; the box takes `tiles_per_box` row tiles of one stage.
+static CUtensorMap make_tmap_sf(const at::Tensor& sf, int64_t rows, int64_t kstages, uint32_t tiles_per_box) {
+  CUtensorMap m;
+  cuuint64_t dims[3] = {256, (cuuint64_t)kstages, (cuuint64_t)((rows + 127) / 128)};
+  cuuint64_t strides[2] = {1024, (cuuint64_t)kstages * 1024};
+  cuuint32_t box[3] = {256, 1, tiles_per_box};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, sf.data_ptr(), dims, strides, box, estr,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  GSB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (scales) failed with code ", (int)r);
+  return m;
 }
 
 struct LoraArgs {
@@ -626,9 +1039,47 @@ static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tens
   p.sfx = sfx.data_ptr<uint8_t>();
   p.sfw = sfw.data_ptr<uint8_t>();
 
+  p.kstages = (int)((K + 255) / 256);
+  if (M >= g_pair_min_m) {
+    PairParams pp{};
+    pp.M = M;
+    pp.N = N;
+    pp.kstages = p.kstages;
+    pp.scale = p.scale;
+    pp.out = p.out;
+    pp.ldo = p.ldo;
+    pp.residual = p.residual;
+    pp.ldr = p.ldr;
+    pp.a4 = p.a4;
+    pp.lda4 = p.lda4;
+    pp.sfa_out = p.sfa_out;
+    pp.lora = p.lora;
+    pp.lp = p.lp;
+    const CUtensorMap tx = make_tmap_2d(x4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)M, (uint64_t)K / 2,
+                                        (uint64_t)x4.stride(0), BKB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    const CUtensorMap tw = make_tmap_2d(w4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)N, (uint64_t)K / 2,
+                                        (uint64_t)w4.stride(0), BKB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    const CUtensorMap tsfx = make_tmap_sf(sfx, M, p.kstages, 1), tsfw = make_tmap_sf(sfw, N, p.kstages, 2);
+    CUtensorMap ts = tx, tlb = tw, to = tx;
+    if (lora) {
+      ts = make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32, 128,
+                             CU_TENSOR_MAP_SWIZZLE_64B);
+      tlb = make_tmap_bf16_2d(la.lb->data_ptr(), (uint64_t)N, (uint64_t)la.lb->size(1), (uint64_t)la.lb->stride(0), 32,
+                              64, CU_TENSOR_MAP_SWIZZLE_64B);
+    }
+    if (epi != kEpiSwiGLU)
+      to = make_tmap_bf16_2d(out->data_ptr(), (uint64_t)M, (uint64_t)N, (uint64_t)out->stride(0), 64, 32,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+    switch (epi) {
+      case kEpiStore: launch_pair<kEpiStore>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+      case kEpiResAdd: launch_pair<kEpiResAdd>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+      default: launch_pair<kEpiSwiGLU>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+    }
+    return;
+  }
+
   const SplitPlan s = split_plan(M, N, K);
   GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
-  p.kstages = (int)((K + 255) / 256);
   p.stages = s.stages;
   p.stage_bytes = s.stage_bytes;
   p.mt_rows = s.mt_rows;
@@ -679,4 +1130,11 @@ void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at
   const std::vector<int64_t> none;
   f4::run_gemm(x4, sfx, w4, sfw, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &a4, &sf,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, none}, err);
+}
+
+// Sets the smallest M that takes the pair kernel; returns the previous value (negative: only reads).
+int64_t gsb_mxfp4_pair_min_m(int64_t m) {
+  const int64_t old = f4::g_pair_min_m;
+  if (m >= 0) f4::g_pair_min_m = (int)std::min<int64_t>(m, 1 << 30);
+  return old;
 }

@@ -105,3 +105,4 @@ void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at
                            const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
                            const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
                            const at::Tensor& err);
+int64_t gsb_mxfp4_pair_min_m(int64_t m);
