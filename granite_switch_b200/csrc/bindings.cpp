@@ -67,6 +67,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_mxfp4", &gsb_rmsnorm_mxfp4, "RMSNorm and its MXFP4 quantisation (optionally the bf16 rows too)");
   m.def("dequantize_mxfp4", &gsb_dequantize_mxfp4, "MXFP4 codes and scale atoms -> bf16 rows");
   m.def("mxfp4_gemm", &gsb_mxfp4_gemm, "MXFP4 tcgen05 GEMM with the bf16 switched-LoRA expand fused");
+  m.def("mxfp4_linear", &gsb_mxfp4_linear, "MXFP4 GEMM of bf16 rows, quantised on the way");
   m.def("mxfp4_gemm_swiglu", &gsb_mxfp4_gemm_swiglu, "MXFP4 gate/up GEMM, SwiGLU and MXFP4 quantisation in the epilogue");
   m.def("mxfp4_pair_min_m", &gsb_mxfp4_pair_min_m,
         "set the smallest M of the CTA-pair MXFP4 GEMM (negative: only reads; returns the old value)");

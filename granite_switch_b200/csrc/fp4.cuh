@@ -77,21 +77,13 @@ __device__ __forceinline__ int64_t sf_word(int64_t row, int64_t kt, int64_t ktil
   return ((row >> 7) * ktiles + kt) * 512 + 16 * (r & 31) + 4 * (r >> 5);
 }
 
-// Quantises eight values per lane of a whole warp (256 neighbours of a row from K index
-// 256 * k2): codes to `codes` (4 bytes a lane, where the lane's values lie before K) and
-// the scale words of both K tiles. Values past K are zero.
-__device__ __forceinline__ void store_warp256(const float (&v)[8], int lane, bool inside, uint8_t* codes, uint8_t* sf,
-                                              int64_t row, int64_t k2, int64_t ktiles) {
-  const uint32_t byte = scale_byte(quad_max(max_abs_bits(v)));
-  float w[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = byte == 255u ? 0.f : v[j];
-  if (inside) *reinterpret_cast<uint32_t*>(codes) = pack8(w, inv_scale(byte));
-  // lanes 0, 4, 8, 12 hold the first tile's four bytes, 16.. the second's
-  const int base = lane & 16;
-  uint32_t word = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, byte, base + 4 * j) << (8 * j);
+// Scale bytes of a whole warp's 256 neighbours (row `row` from K index 256 * k2; `byte` of
+// each lane's block of four lanes) -> the words of both K tiles.
+__device__ __forceinline__ void store_scales256(uint32_t byte, int lane, uint8_t* sf, int64_t row, int64_t k2,
+                                                int64_t ktiles) {
+  uint32_t word = byte << (8 * ((lane >> 2) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  word |= __shfl_xor_sync(0xffffffffu, word, 8);
   if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(sf + sf_word(row, 2 * k2 + (lane >> 4), ktiles)) = word;
 }
 

@@ -23,6 +23,7 @@
 // Every wait is bounded; a CTA that gives up still arrives at the cluster barriers.
 #include "common.cuh"
 #include "fp4.cuh"
+#include "fp4_host.h"
 #include "gemm_common.cuh"
 #include "tma_util.h"
 
@@ -31,6 +32,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -61,6 +63,7 @@ struct SplitParams {
   int mt_rows;        // tokens per tile
   int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
   int tmem_cols;
+  int early;          // load weights before the wait for the kernel before this one
   const uint8_t* sfx;
   const uint8_t* sfw;
   float scale;
@@ -204,12 +207,27 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   griddep_launch();
+
+  // Launched as a dependent of the quantiser of its own call, the kernel loads the first
+  // stages' weights while that one still runs; nothing else is read before the wait.
+  auto load_w = [&](int i, int s) {
+    const int kb = kb_lo + i;
+    uint8_t* sw = smem + s * p.stage_bytes;
+    mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
+    tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
+    bulk_load(sw + W_BYTES + x_bytes, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
+  };
+  const int early = p.early ? min(stages, n_main) : 0;
+  if (warp == 0 && lane == 0)
+    for (int i = 0; i < early; ++i) load_w(i, i);  // a fresh ring: no wait for empty stages
   griddep_wait();
 
-  uint64_t amask = 0ull, tmask[2] = {0ull, 0ull};
+  uint64_t mask0 = 0ull, mask1 = 0ull;  // adapters of the token tile's two 128-row halves
   if (p.lora) {
-    for (int t = 0; t < xt; ++t) amask |= tmask[t] = tile_adapters(p.lp, m0 / 128 + t, mtiles128);
+    mask0 = tile_adapters(p.lp, m0 / 128, mtiles128);
+    if (xt > 1) mask1 = tile_adapters(p.lp, m0 / 128 + 1, mtiles128);
   }
+  const uint64_t amask = mask0 | mask1;
   const int n_lora_all = __popcll(amask) * p.lp.blocks_per_adapter;
   const int n_lora = n_lora_all > part ? (n_lora_all - part + ks - 1) / ks : 0;
   const int total = n_main + n_lora;
@@ -222,7 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < total; ++i) {
         const int s = i % stages;
         const uint32_t ph = (i / stages) & 1;
-        if (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait)) {
+        if (i >= early && (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait))) {
           abort_flag = 1;
           break;
         }
@@ -231,10 +249,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint8_t* sf = sx + x_bytes;
         if (i < n_main) {
           const int kb = kb_lo + i;
-          mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
-          tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
+          if (i >= early) load_w(i, s);
           tma_load_2d(sx, &tm_x, &full_bar[s], kb * BKB, m0);
-          bulk_load(sf, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
           for (int t = 0; t < xt; ++t)
             bulk_load(sf + 1024 * (1 + t), p.sfx + ((size_t)(m0 / 128 + t) * p.kstages + kb) * 1024, 1024,
                       &full_bar[s]);
@@ -248,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // reads rows past M, which TMA fills with zeros
           for (int t = 0; t < xt; ++t)
             tma_load_2d(sx + t * 128 * 64, &tm_s, &full_bar[s], slice_base(p.lp, n0) + col,
-                        ((tmask[t] >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
+                        (((t ? mask1 : mask0) >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
         }
         ++issued;
       }
@@ -545,12 +561,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         int mt, nt;
         pair_tile(t, m_tiles, n_tiles, mt, nt);
         const int own = 2 * mt + (int)rank, m0 = own * 128, n0 = nt * C::BN;
-        uint64_t mask[2] = {0ull, 0ull};
+        uint64_t mask0 = 0ull, mask1 = 0ull;
         if (p.lora) {
-          mask[0] = tile_adapters(p.lp, 2 * mt, mtiles128);
-          mask[1] = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
+          mask0 = tile_adapters(p.lp, 2 * mt, mtiles128);
+          mask1 = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
         }
-        const uint64_t both = mask[0] | mask[1], mine = rank ? mask[1] : mask[0];
+        const uint64_t both = mask0 | mask1, mine = rank ? mask1 : mask0;
         const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
         for (int i = 0; i < total; ++i, ++kb) {
           const int s = kb % C::STAGES;
@@ -848,9 +864,16 @@ static SplitPlan split_plan(int M, int N, int64_t K) {
   return s;
 }
 
-static bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// Codes and scale atoms of an operand.
+struct Codes {
+  uint8_t* q;
+  int64_t ld;
+  uint8_t* sf;
+  int64_t rows;
+};
 
-static void check_operand(const char* what, const at::Tensor& q, const at::Tensor& sf, int64_t K, const at::Device& dev) {
+static Codes check_operand(const char* what, const at::Tensor& q, const at::Tensor& sf, int64_t K,
+                           const at::Device& dev) {
   GSB_CHECK(q.is_cuda() && q.device() == dev && sf.device() == dev, "mxfp4_gemm: ", what, " must be on one CUDA device");
   GSB_CHECK(q.scalar_type() == at::kByte && q.dim() == 2 && q.size(1) * 2 == K && q.stride(1) == 1 &&
                 q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1) && aligned16(q),
@@ -858,6 +881,7 @@ static void check_operand(const char* what, const at::Tensor& q, const at::Tenso
   GSB_CHECK(sf.scalar_type() == at::kByte && sf.is_contiguous() && aligned16(sf) &&
                 sf.numel() == (q.size(0) + 127) / 128 * k_tiles(K) * 512,
             "mxfp4_gemm: ", what, " scales must be uint8 atoms [ceil(rows / 128), 2 ceil(K / 256), 512]");
+  return {q.data_ptr<uint8_t>(), q.stride(0), sf.data_ptr<uint8_t>(), q.size(0)};
 }
 
 static void check_out(const char* what, const at::Tensor& t, int64_t M, int64_t N, const at::Device& dev) {
@@ -867,31 +891,26 @@ static void check_out(const char* what, const at::Tensor& t, int64_t M, int64_t 
             "mxfp4_gemm: ", what, " must be bf16 [", M, ", ", N, "] with 16-byte aligned rows");
 }
 
-template <int EPI>
-static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tlb, const CUtensorMap& ts,
-                         const SplitParams& p, const SplitPlan& s, uint32_t* err, cudaStream_t st) {
-  auto kfn = mxfp4_split_kernel<EPI>;
-  static bool set[kMaxDevices] = {false};
-  const int dev = current_device();
-  if (!set[dev]) {
-    GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
-    set[dev] = true;
-  }
+// Launches with `cluster` CTAs a cluster (1: none; the pair kernel has its size compiled in),
+// as a programmatic dependent of the kernel before when `dependent`.
+template <typename... KArgs, typename... Args>
+static void launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, int cluster, bool dependent,
+                   cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(s.weight_tiles * s.ks), (unsigned)s.token_tiles, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = s.smem_bytes;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   unsigned n = 0;
-  if (s.ks > 1) {
+  if (cluster > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = (unsigned)s.ks;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
     attr[n].val.clusterDim.y = 1;
     attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl_enabled()) {
+  if (dependent) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -899,7 +918,21 @@ static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUt
   cfg.attrs = attr;
   cfg.numAttrs = n;
   count_launch();
-  GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, tw, tx, tlb, ts, p, err));
+  GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+template <int EPI>
+static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tlb, const CUtensorMap& ts,
+                         const SplitParams& p, const SplitPlan& s, bool dependent, uint32_t* err, cudaStream_t st) {
+  auto kfn = mxfp4_split_kernel<EPI>;
+  static bool set[kMaxDevices] = {false};
+  const int dev = current_device();
+  if (!set[dev]) {
+    GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
+    set[dev] = true;
+  }
+  launch(kfn, dim3((unsigned)(s.weight_tiles * s.ks), (unsigned)s.token_tiles), THREADS, s.smem_bytes, s.ks, dependent,
+         st, tw, tx, tlb, ts, p, err);
 }
 
 // Clusters of two of the pair kernel that fit at once (asked once per device and epilogue).
@@ -929,25 +962,30 @@ static int pair_clusters() {
 template <int EPI>
 static void launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& tsfx, const CUtensorMap& tsfw,
                         const CUtensorMap& ts, const CUtensorMap& tlb, const CUtensorMap& to, const PairParams& p,
-                        uint32_t* err, cudaStream_t st) {
+                        bool dependent, uint32_t* err, cudaStream_t st) {
   const int tiles = ((p.M + 255) / 256) * ((p.N + PairCfg::BN - 1) / PairCfg::BN);
   const int clusters = std::min(tiles, pair_clusters<EPI>());  // also sets the shared-memory attribute
-  launch_dependent(mxfp4_pair_kernel<EPI>, dim3(2 * clusters), dim3(PairCfg::THREADS), PairCfg::SMEM_BYTES, st, tx, tw,
-                   tsfx, tsfw, ts, tlb, to, p, err);
+  launch(mxfp4_pair_kernel<EPI>, dim3(2 * clusters), PairCfg::THREADS, PairCfg::SMEM_BYTES, 1, dependent, st, tx, tw,
+         tsfx, tsfw, ts, tlb, to, p, err);
 }
 
 // Scale atoms [tiles, K stages, 1024 bytes]; the box takes `tiles_per_box` row tiles of one stage.
-static CUtensorMap make_tmap_sf(const at::Tensor& sf, int64_t rows, int64_t kstages, uint32_t tiles_per_box) {
+static CUtensorMap make_tmap_sf(const Codes& c, int64_t kstages, uint32_t tiles_per_box) {
   CUtensorMap m;
-  cuuint64_t dims[3] = {256, (cuuint64_t)kstages, (cuuint64_t)((rows + 127) / 128)};
+  cuuint64_t dims[3] = {256, (cuuint64_t)kstages, (cuuint64_t)((c.rows + 127) / 128)};
   cuuint64_t strides[2] = {1024, (cuuint64_t)kstages * 1024};
   cuuint32_t box[3] = {256, 1, tiles_per_box};
   cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, sf.data_ptr(), dims, strides, box, estr,
+  const CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, c.sf, dims, strides, box, estr,
                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   GSB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (scales) failed with code ", (int)r);
   return m;
+}
+
+static CUtensorMap make_tmap_codes(const Codes& c, int64_t K, uint32_t box_rows) {
+  return make_tmap_2d(c.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)c.rows, (uint64_t)K / 2, (uint64_t)c.ld, BKB,
+                      box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 struct LoraArgs {
@@ -955,39 +993,33 @@ struct LoraArgs {
   const c10::optional<at::Tensor>& lb;
   const c10::optional<at::Tensor>& tile_mask;
   int64_t rank, num_adapters;
-  const std::vector<int64_t>& slice_bounds;
+  std::vector<int64_t> slice_bounds;
 };
 
-// One product on the current stream of x4's device. `a4` / `sfa_out` for swiglu only.
-static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
-                     const at::Tensor* out, int epi, double scale, const c10::optional<at::Tensor>& residual,
-                     const at::Tensor* a4, const at::Tensor* sfa_out, const LoraArgs& la, const at::Tensor& err) {
-  const at::Device dev = x4.device();
-  GSB_CHECK(x4.dim() == 2 && w4.dim() == 2 && x4.size(1) == w4.size(1), "mxfp4_gemm: operands [M, K / 2] and [N, K / 2] required");
-  const int64_t K = x4.size(1) * 2, M64 = x4.size(0), N64 = w4.size(0);
+// One product on stream `st` of `dev`, the current device. `a4` (codes and scales of the
+// output) for swiglu, `out` otherwise (for swiglu: the bf16 copy, or null). `own_quantiser`:
+// the kernel before in the stream is this call's quantiser of x, which neither writes
+// weights nor lets a dependent start before all that came earlier is done.
+static void run_gemm(const Codes& x, const Codes& w, int64_t K, const at::Tensor* out, int epi, double scale,
+                     const c10::optional<at::Tensor>& residual, const Codes* a4, const LoraArgs& la,
+                     const at::Tensor& err, const at::Device& dev, bool own_quantiser, cudaStream_t st) {
   GSB_CHECK(K >= kBlock && K % kBlock == 0 && K < (int64_t(1) << 31), "mxfp4_gemm: K must be a positive multiple of 32");
-  GSB_CHECK(M64 < (int64_t(1) << 24) && N64 > 0 && N64 < (int64_t(1) << 24) && N64 % 8 == 0,
+  GSB_CHECK(x.rows < (int64_t(1) << 24) && w.rows > 0 && w.rows < (int64_t(1) << 24) && w.rows % 8 == 0,
             "mxfp4_gemm: N must be a positive multiple of 8");
-  check_operand("x", x4, sfx, K, dev);
-  check_operand("w", w4, sfw, K, dev);
   GSB_CHECK(err.device() == dev, "mxfp4_gemm: error word on another device");
-  const int M = (int)M64, N = (int)N64;
+  const int M = (int)x.rows, N = (int)w.rows;
   SplitParams p{};
   p.M = M;
   p.N = N;
   p.scale = (float)scale;
-  if (epi == kEpiSwiGLU) {
-    GSB_CHECK(N % 128 == 0, "mxfp4_gemm_swiglu: the weight must hold a multiple of 128 rows (64 gate, 64 up, ...)");
-    check_operand("output", *a4, *sfa_out, N / 2, dev);
-    GSB_CHECK(a4->size(0) == M, "mxfp4_gemm_swiglu: output codes must be [M, N / 4]");
-    p.a4 = a4->data_ptr<uint8_t>();
-    p.lda4 = a4->stride(0);
-    p.sfa_out = sfa_out->data_ptr<uint8_t>();
-    if (out != nullptr) check_out("act", *out, M, N / 2, dev);
-  } else {
-    check_out("out", *out, M, N, dev);
+  p.kstages = (int)((K + 255) / 256);
+  if (a4 != nullptr) {
+    p.a4 = a4->q;
+    p.lda4 = a4->ld;
+    p.sfa_out = a4->sf;
   }
   if (out != nullptr) {
+    check_out(epi == kEpiSwiGLU ? "act" : "out", *out, M, epi == kEpiSwiGLU ? N / 2 : N, dev);
     p.out = out->data_ptr();
     p.ldo = out->stride(0);
   }
@@ -1033,13 +1065,17 @@ static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tens
     }
   }
   if (M == 0) return;
-  c10::cuda::CUDAGuard g(dev);
-  auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());
-  p.sfx = sfx.data_ptr<uint8_t>();
-  p.sfw = sfw.data_ptr<uint8_t>();
+  const bool dependent = own_quantiser || pdl_enabled();
+  auto tmap_s = [&](uint32_t rows) {
+    return make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32,
+                             rows, CU_TENSOR_MAP_SWIZZLE_64B);
+  };
+  auto tmap_lb = [&](uint32_t rows) {
+    return make_tmap_bf16_2d(la.lb->data_ptr(), (uint64_t)N, (uint64_t)la.lb->size(1), (uint64_t)la.lb->stride(0), 32,
+                             rows, CU_TENSOR_MAP_SWIZZLE_64B);
+  };
 
-  p.kstages = (int)((K + 255) / 256);
   if (M >= g_pair_min_m) {
     PairParams pp{};
     pp.M = M;
@@ -1055,54 +1091,48 @@ static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tens
     pp.sfa_out = p.sfa_out;
     pp.lora = p.lora;
     pp.lp = p.lp;
-    const CUtensorMap tx = make_tmap_2d(x4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)M, (uint64_t)K / 2,
-                                        (uint64_t)x4.stride(0), BKB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    const CUtensorMap tw = make_tmap_2d(w4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)N, (uint64_t)K / 2,
-                                        (uint64_t)w4.stride(0), BKB, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    const CUtensorMap tsfx = make_tmap_sf(sfx, M, p.kstages, 1), tsfw = make_tmap_sf(sfw, N, p.kstages, 2);
-    CUtensorMap ts = tx, tlb = tw, to = tx;
-    if (lora) {
-      ts = make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32, 128,
-                             CU_TENSOR_MAP_SWIZZLE_64B);
-      tlb = make_tmap_bf16_2d(la.lb->data_ptr(), (uint64_t)N, (uint64_t)la.lb->size(1), (uint64_t)la.lb->stride(0), 32,
-                              64, CU_TENSOR_MAP_SWIZZLE_64B);
-    }
-    if (epi != kEpiSwiGLU)
-      to = make_tmap_bf16_2d(out->data_ptr(), (uint64_t)M, (uint64_t)N, (uint64_t)out->stride(0), 64, 32,
-                             CU_TENSOR_MAP_SWIZZLE_128B);
+    const CUtensorMap tx = make_tmap_codes(x, K, 128), tw = make_tmap_codes(w, K, 128);
+    const CUtensorMap tsfx = make_tmap_sf(x, p.kstages, 1), tsfw = make_tmap_sf(w, p.kstages, 2);
+    const CUtensorMap ts = lora ? tmap_s(128) : tx, tlb = lora ? tmap_lb(64) : tw;
+    const CUtensorMap to = epi == kEpiSwiGLU
+                               ? tx
+                               : make_tmap_bf16_2d(p.out, (uint64_t)M, (uint64_t)N, (uint64_t)p.ldo, 64, 32,
+                                                   CU_TENSOR_MAP_SWIZZLE_128B);
     switch (epi) {
-      case kEpiStore: launch_pair<kEpiStore>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
-      case kEpiResAdd: launch_pair<kEpiResAdd>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
-      default: launch_pair<kEpiSwiGLU>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+      case kEpiStore: launch_pair<kEpiStore>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
+      case kEpiResAdd: launch_pair<kEpiResAdd>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
+      default: launch_pair<kEpiSwiGLU>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
     }
     return;
   }
 
   const SplitPlan s = split_plan(M, N, K);
   GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
+  p.sfx = x.sf;
+  p.sfw = w.sf;
   p.stages = s.stages;
   p.stage_bytes = s.stage_bytes;
   p.mt_rows = s.mt_rows;
   p.ks = s.ks;
   p.rows_per = rows_per_part(s.mt_rows, s.ks);
   p.tmem_cols = s.tmem_cols;
+  p.early = own_quantiser ? 1 : 0;
   const uint32_t mp = (uint32_t)((s.mt_rows + 15) / 16 * 16);
-  const CUtensorMap tw = make_tmap_2d(w4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)N, (uint64_t)K / 2,
-                                      (uint64_t)w4.stride(0), BKB, BW, CU_TENSOR_MAP_SWIZZLE_128B);
-  const CUtensorMap tx = make_tmap_2d(x4.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)M, (uint64_t)K / 2,
-                                      (uint64_t)x4.stride(0), BKB, mp, CU_TENSOR_MAP_SWIZZLE_128B);
-  CUtensorMap tlb = tw, ts = tx;
-  if (lora) {
-    tlb = make_tmap_bf16_2d(la.lb->data_ptr(), (uint64_t)N, (uint64_t)la.lb->size(1), (uint64_t)la.lb->stride(0), 32,
-                            BW, CU_TENSOR_MAP_SWIZZLE_64B);
-    ts = make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32,
-                           std::min(mp, 128u), CU_TENSOR_MAP_SWIZZLE_64B);
-  }
+  const CUtensorMap tw = make_tmap_codes(w, K, BW), tx = make_tmap_codes(x, K, mp);
+  const CUtensorMap tlb = lora ? tmap_lb(BW) : tw, ts = lora ? tmap_s(std::min(mp, 128u)) : tx;
   switch (epi) {
-    case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, ep, st); break;
-    case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, ep, st); break;
-    default: launch_split<kEpiSwiGLU>(tw, tx, tlb, ts, p, s, ep, st); break;
+    case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
+    case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
+    default: launch_split<kEpiSwiGLU>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
   }
+}
+
+static at::Tensor new_out(int64_t M, int64_t N, const at::Device& dev) {
+  return at::empty({M, N}, at::TensorOptions().dtype(at::kBFloat16).device(dev));
+}
+
+static void check_epi(int64_t epi) {
+  GSB_CHECK(epi == kEpiStore || epi == kEpiResAdd, "mxfp4_gemm: epilogue must be store (0) or residual add (1)");
 }
 
 }  // namespace f4
@@ -1110,26 +1140,76 @@ static void run_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tens
 
 using namespace gsb;
 
-// out [M, N] bf16 = epi(x4 . w4^T (+ s . lb^T)); epi 0 store (times scale), 1 residual + scale * acc.
-void gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
-                    const at::Tensor& out, int64_t epi, double scale, const c10::optional<at::Tensor>& residual,
-                    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
-                    const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
-                    std::vector<int64_t> slice_bounds, const at::Tensor& err) {
-  GSB_CHECK(epi == kEpiStore || epi == kEpiResAdd, "mxfp4_gemm: epilogue must be store (0) or residual add (1)");
-  f4::run_gemm(x4, sfx, w4, sfw, &out, (int)epi, scale, residual, nullptr, nullptr,
-               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, slice_bounds}, err);
+// out [M, N] bf16 = epi(x4 . w4^T (+ s . lb^T)); epi 0: times scale, 1: residual + scale * that.
+at::Tensor gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                          const c10::optional<at::Tensor>& out_, int64_t epi, double scale,
+                          const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& s,
+                          const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask, int64_t rank,
+                          int64_t num_adapters, const c10::optional<std::vector<int64_t>>& slice_bounds,
+                          const at::Tensor& err) {
+  f4::check_epi(epi);
+  GSB_CHECK(x4.dim() == 2 && w4.dim() == 2, "mxfp4_gemm: operands [M, K / 2] and [N, K / 2] required");
+  const int64_t K = x4.size(1) * 2;
+  const at::Device dev = x4.device();
+  const f4::Codes x = f4::check_operand("x", x4, sfx, K, dev), w = f4::check_operand("w", w4, sfw, K, dev);
+  c10::cuda::CUDAGuard g(dev);
+  const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(x.rows, w.rows, dev);
+  f4::run_gemm(x, w, K, &out, (int)epi, scale, residual, nullptr,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
+                            slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
+               err, dev, false, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  return out;
 }
 
-// a4 / sf <- quantised silu(gate) * up of the gate/up product; `act` also as bf16.
-void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
-                           const at::Tensor& a4, const at::Tensor& sf, const c10::optional<at::Tensor>& act,
-                           const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
-                           const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
-                           const at::Tensor& err) {
-  const std::vector<int64_t> none;
-  f4::run_gemm(x4, sfx, w4, sfw, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &a4, &sf,
-               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, none}, err);
+// The same from bf16 rows x [M, K], quantised into a workspace of the call.
+at::Tensor gsb_mxfp4_linear(const at::Tensor& x, const at::Tensor& w4, const at::Tensor& sfw,
+                            const c10::optional<at::Tensor>& out_, int64_t epi, double scale,
+                            const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& s,
+                            const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask,
+                            int64_t rank, int64_t num_adapters, const c10::optional<std::vector<int64_t>>& slice_bounds,
+                            const at::Tensor& err) {
+  f4::check_epi(epi);
+  f4::check_rows("mxfp4_linear", "x", x, x.device());
+  const int64_t M = x.size(0), K = x.size(1);
+  const at::Device dev = x.device();
+  const f4::Codes w = f4::check_operand("w", w4, sfw, K, dev);
+  c10::cuda::CUDAGuard g(dev);
+  const int64_t code_bytes = (M * (K / 2) + 1023) / 1024 * 1024;
+  const at::Tensor work = at::empty({code_bytes + (M + 127) / 128 * f4::k_tiles(K) * 512},
+                                    at::TensorOptions().dtype(at::kByte).device(dev));
+  uint8_t* q = work.data_ptr<uint8_t>();
+  const f4::Codes c{q, K / 2, q + code_bytes, M};
+  const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(M, w.rows, dev);
+  auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  if (M > 0) f4::quantize_launch(x.data_ptr(), x.stride(0), M, K, c.q, c.ld, c.sf, st);
+  f4::run_gemm(c, w, K, &out, (int)epi, scale, residual, nullptr,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
+                            slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
+               err, dev, M > 0, st);
+  return out;
+}
+
+// (a4, sf) <- quantised silu(gate) * up of the gate/up product; `act` also as bf16.
+std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
+    const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+    const c10::optional<at::Tensor>& a4_, const c10::optional<at::Tensor>& sf_, const c10::optional<at::Tensor>& act,
+    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask,
+    int64_t rank, int64_t num_adapters, const at::Tensor& err) {
+  GSB_CHECK(x4.dim() == 2 && w4.dim() == 2, "mxfp4_gemm_swiglu: operands [M, K / 2] and [2 I, K / 2] required");
+  const int64_t K = x4.size(1) * 2, I = w4.size(0) / 2;
+  const at::Device dev = x4.device();
+  const f4::Codes x = f4::check_operand("x", x4, sfx, K, dev), w = f4::check_operand("w", w4, sfw, K, dev);
+  GSB_CHECK(w.rows > 0 && w.rows % 128 == 0,
+            "mxfp4_gemm_swiglu: the weight must hold a multiple of 128 rows (64 gate, 64 up, ...)");
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor a4 = a4_.value_or(at::Tensor()), sf = sf_.value_or(at::Tensor());
+  f4::make_codes(x.rows, I, dev, a4, sf);
+  const f4::Codes o = f4::check_operand("output", a4, sf, I, dev);
+  GSB_CHECK(o.rows == x.rows, "mxfp4_gemm_swiglu: output codes must be [M, I / 2]");
+  f4::run_gemm(x, w, K, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &o,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, {}}, err, dev, false,
+               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  return {a4, sf};
 }
 
 // Sets the smallest M that takes the pair kernel; returns the previous value (negative: only reads).

@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
 
+#include <tuple>
 #include <vector>
 
 void gsb_switched_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& out,
@@ -91,18 +92,28 @@ int64_t gsb_attn_packed(int64_t v);
 int64_t gsb_gemm_splitk_max_tiles(int64_t v);
 int64_t gsb_attn_fp8t_stages(int64_t v);
 int64_t gsb_attn_decode_stages(int64_t v);
-void gsb_quantize_mxfp4(const at::Tensor& x, const at::Tensor& x4, const at::Tensor& sf);
-void gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps, const at::Tensor& x4,
-                       const at::Tensor& sf, const c10::optional<at::Tensor>& out);
-void gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, const at::Tensor& out);
-void gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
-                    const at::Tensor& out, int64_t epi, double scale, const c10::optional<at::Tensor>& residual,
-                    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
-                    const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
-                    std::vector<int64_t> slice_bounds, const at::Tensor& err);
-void gsb_mxfp4_gemm_swiglu(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
-                           const at::Tensor& a4, const at::Tensor& sf, const c10::optional<at::Tensor>& act,
-                           const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb,
-                           const c10::optional<at::Tensor>& tile_mask, int64_t rank, int64_t num_adapters,
-                           const at::Tensor& err);
+std::tuple<at::Tensor, at::Tensor> gsb_quantize_mxfp4(const at::Tensor& x, const c10::optional<at::Tensor>& x4,
+                                                      const c10::optional<at::Tensor>& sf);
+std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps,
+                                                     const c10::optional<at::Tensor>& x4,
+                                                     const c10::optional<at::Tensor>& sf,
+                                                     const c10::optional<at::Tensor>& out);
+at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, const c10::optional<at::Tensor>& out);
+at::Tensor gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+                          const c10::optional<at::Tensor>& out, int64_t epi, double scale,
+                          const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& s,
+                          const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask, int64_t rank,
+                          int64_t num_adapters, const c10::optional<std::vector<int64_t>>& slice_bounds,
+                          const at::Tensor& err);
+at::Tensor gsb_mxfp4_linear(const at::Tensor& x, const at::Tensor& w4, const at::Tensor& sfw,
+                            const c10::optional<at::Tensor>& out, int64_t epi, double scale,
+                            const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& s,
+                            const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask,
+                            int64_t rank, int64_t num_adapters, const c10::optional<std::vector<int64_t>>& slice_bounds,
+                            const at::Tensor& err);
+std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
+    const at::Tensor& x4, const at::Tensor& sfx, const at::Tensor& w4, const at::Tensor& sfw,
+    const c10::optional<at::Tensor>& a4, const c10::optional<at::Tensor>& sf, const c10::optional<at::Tensor>& act,
+    const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask,
+    int64_t rank, int64_t num_adapters, const at::Tensor& err);
 int64_t gsb_mxfp4_pair_min_m(int64_t m);

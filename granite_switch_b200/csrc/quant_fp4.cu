@@ -11,6 +11,7 @@
 //   dequantize_mxfp4: codes times scale, exact in bf16.
 #include "common.cuh"
 #include "fp4.cuh"
+#include "fp4_host.h"
 #include "tma_util.h"
 
 #include <ATen/ATen.h>
@@ -18,12 +19,14 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <tuple>
 
 namespace gsb {
 namespace f4 {
 
 constexpr int kQuantThreads = 256;
-constexpr int kUnits = 4;  // 256-value units in flight per warp
+constexpr int kWarpNormRows = 1184;
+constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 
 __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
   const uint32_t p[4] = {q.x, q.y, q.z, q.w};
@@ -35,58 +38,108 @@ __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
   }
 }
 
+// fp32 bits of the largest magnitude of eight packed bf16 values (as 16-bit integers, so a
+// NaN is above infinity).
+__device__ __forceinline__ uint32_t max_abs_bits_bf16(const uint4& q) {
+  const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu),
+                              __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+  return max(m << 16, m & 0xffff0000u);
+}
+
+// Warp `blockIdx.x * 8 + ..` takes `kUnits` units of one row; `per_row` warps make a row.
 __global__ void __launch_bounds__(kQuantThreads)
-    quantize_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int64_t K, int64_t k2s, int64_t units,
-                          uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf) {
-  griddep_launch();
+    quantize_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int K, int k2s, uint32_t per_row,
+                          uint32_t warps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf) {
   griddep_wait();
+  griddep_launch();  // after the wait: a dependent may count on all that came before this kernel
   const int lane = threadIdx.x & 31;
-  const int64_t warp = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
-  const int64_t first = warp * kUnits;
+  const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+  if (warp >= warps) return;
+  const uint32_t row = warp / per_row;
+  const int first = (int)(warp - row * per_row) * kUnits;
+  const __nv_bfloat16* xr = x + row * ldx + lane * 8;
   uint4 q[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const int64_t unit = first + u;
+    const int k = (first + u) * 256;
     q[u] = make_uint4(0u, 0u, 0u, 0u);
-    const int64_t row = unit / k2s, k = (unit % k2s) * 256 + lane * 8;
-    if (unit < units && k < K) q[u] = *reinterpret_cast<const uint4*>(x + row * ldx + k);
+    if (k + lane * 8 < K) q[u] = *reinterpret_cast<const uint4*>(xr + k);
   }
+  uint8_t* xo = x4 + row * ld4 + lane * 4;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const int64_t unit = first + u;
-    if (unit >= units) break;  // the whole warp
-    const int64_t row = unit / k2s, k2 = unit % k2s, k = k2 * 256 + lane * 8;
+    const int k2 = first + u, k = k2 * 256 + lane * 8;
+    if (k2 >= k2s) break;  // the whole warp
+    const uint32_t byte = scale_byte(quad_max(max_abs_bits_bf16(q[u])));
     float v[8];
-    unpack8(q[u], v);
-    store_warp256(v, lane, k < K, x4 + row * ld4 + k / 2, sf, row, k2, 2 * k2s);
+    unpack8(byte == 255u ? make_uint4(0u, 0u, 0u, 0u) : q[u], v);
+    if (k < K) *reinterpret_cast<uint32_t*>(xo + k2 * 128) = pack8(v, inv_scale(byte));
+    store_scales256(byte, lane, sf, row, k2, 2 * k2s);
   }
 }
 
+// Normalised values of eight inputs -> codes, scales and (optionally) the bf16 row.
+__device__ __forceinline__ void norm_store8(const uint4& xq, const uint4& wq, float inv, bool inside, int lane,
+                                            int64_t row, int v, int64_t ktiles, uint8_t* x4_row, uint8_t* sf,
+                                            __nv_bfloat16* out_row) {
+  float f[8], g[8], y[8];
+  unpack8(xq, f);
+  unpack8(wq, g);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = inside ? (f[j] * g[j]) * inv : 0.f;  // inv is NaN in a row that is not finite
+  const uint32_t byte = scale_byte(quad_max(max_abs_bits(y)));
+  if (inside) {
+    if (out_row != nullptr) {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
+                           __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
+      reinterpret_cast<uint4*>(out_row)[v] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    if (byte == 255u) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    }
+    *reinterpret_cast<uint32_t*>(x4_row + v * 4) = pack8(y, inv_scale(byte));
+  }
+  store_scales256(byte, lane, sf, row, v / 32, ktiles);
+}
+
+__device__ __forceinline__ float sum_squares8(const uint4& q, float ss) {
+  float f[8];
+  unpack8(q, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ss += f[2 * j] * f[2 * j] + f[2 * j + 1] * f[2 * j + 1];
+  return ss;
+}
+
+// One CTA per row (few rows, or wide ones): the sum of squares in the RMSNorm kernel's order.
 template <int VPT>
 __global__ void __launch_bounds__(256)
     rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w, int H,
                          float eps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf,
                          __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  griddep_launch();
   griddep_wait();
-  const int r = blockIdx.x;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + (int64_t)r * ldx);
+  griddep_launch();
+  const int64_t r = blockIdx.x;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
   const uint4* wv = reinterpret_cast<const uint4*>(w);
   const int nvec = H / 8, nvec_pad = (int)k_tiles(H) * 16;
-  uint4 buf[VPT];
+  uint4 buf[VPT], wbuf[VPT];
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * 256;
-    buf[i] = make_uint4(0u, 0u, 0u, 0u);
+    buf[i] = wbuf[i] = make_uint4(0u, 0u, 0u, 0u);
     if (v < nvec) {
       buf[i] = xv[v];
-      float f[8];
-      unpack8(buf[i], f);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ss += f[2 * j] * f[2 * j] + f[2 * j + 1] * f[2 * j + 1];
+      wbuf[i] = wv[v];
     }
   }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+    if (threadIdx.x + i * 256 < nvec) ss = sum_squares8(buf[i], ss);
   __shared__ float red[32];
   ss = warp_sum(ss);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
@@ -98,51 +151,85 @@ __global__ void __launch_bounds__(256)
   }
   __syncthreads();
   const float inv = rsqrtf(red[0] / (float)H + eps);
+  __nv_bfloat16* orow = out ? out + r * ldo : nullptr;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * 256;
     if (v >= nvec_pad) break;  // the whole warp: nvec_pad is a multiple of 32
+    norm_store8(buf[i], wbuf[i], inv, v < nvec, threadIdx.x & 31, r, v, k_tiles(H), x4 + r * ld4, sf, orow);
+  }
+}
+
+// One warp per row (many rows of up to 4096 columns): no barrier, and the whole row's loads
+// in flight. Lane l holds what the threads l, l + 32, ... of the CTA kernel hold and adds in
+// the same order, so both give the same bits.
+template <int NI>  // ceil(H / 2048)
+__global__ void __launch_bounds__(256)
+    rmsnorm_mxfp4_warp_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w,
+                              int M, int H, float eps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf,
+                              __nv_bfloat16* __restrict__ out, int64_t ldo) {
+  griddep_wait();
+  griddep_launch();
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= M) return;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
+  const uint4* wv = reinterpret_cast<const uint4*>(w);
+  const int nvec = H / 8, units = (int)k_tiles(H) / 2;
+  uint4 buf[8 * NI];
+#pragma unroll
+  for (int j = 0; j < 8 * NI; ++j) {
+    const int v = lane + 32 * j;
+    buf[j] = v < nvec ? xv[v] : make_uint4(0u, 0u, 0u, 0u);
+  }
+  float a[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (lane + 32 * (t + 8 * i) < nvec) ss = sum_squares8(buf[t + 8 * i], ss);
+    a[t] = warp_sum(ss);
+  }
+  const float total = ((a[0] + a[4]) + (a[2] + a[6])) + ((a[1] + a[5]) + (a[3] + a[7]));
+  const float inv = rsqrtf(total / (float)H + eps);
+  __nv_bfloat16* orow = out ? out + r * ldo : nullptr;
+#pragma unroll
+  for (int j = 0; j < 8 * NI; ++j) {
+    if (j >= units) break;
+    const int v = lane + 32 * j;
     const bool inside = v < nvec;
-    float f[8], g[8], y[8];
-    unpack8(buf[i], f);
-    unpack8(inside ? wv[v] : make_uint4(0u, 0u, 0u, 0u), g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (f[j] * g[j]) * inv;
-    if (!inside) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.f;  // a row that is not finite has inv = NaN
-    }
-    store_warp256(y, threadIdx.x & 31, inside, x4 + (int64_t)r * ld4 + v * 4, sf, r, v / 32, k_tiles(H));
-    if (out != nullptr && inside) {
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
-                           __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
-      reinterpret_cast<uint4*>(out + (int64_t)r * ldo)[v] = make_uint4(o[0], o[1], o[2], o[3]);
-    }
+    norm_store8(buf[j], inside ? wv[v] : make_uint4(0u, 0u, 0u, 0u), inv, inside, lane, r, v, 2 * units, x4 + r * ld4,
+                sf, orow);
   }
 }
 
 __global__ void __launch_bounds__(kQuantThreads)
-    dequantize_mxfp4_kernel(const uint8_t* __restrict__ x4, int64_t ld4, const uint8_t* __restrict__ sf, int64_t K,
-                            int64_t k2s, int64_t units, __nv_bfloat16* __restrict__ out, int64_t ldo) {
+    dequantize_mxfp4_kernel(const uint8_t* __restrict__ x4, int64_t ld4, const uint8_t* __restrict__ sf, int K,
+                            int k2s, uint32_t per_row, uint32_t warps, __nv_bfloat16* __restrict__ out, int64_t ldo) {
+  griddep_wait();
+  griddep_launch();
   const int lane = threadIdx.x & 31;
-  const int64_t warp = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+  if (warp >= warps) return;
+  const uint32_t row = warp / per_row;
+  const int first = (int)(warp - row * per_row) * kUnits;
+  const uint8_t* xi = x4 + row * ld4 + lane * 4;
   uint32_t c[kUnits], b[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const int64_t unit = warp * kUnits + u, row = unit / k2s, k2 = unit % k2s, k = k2 * 256 + lane * 8;
+    const int k2 = first + u;
     c[u] = b[u] = 0u;
-    if (unit < units && k < K) {
-      c[u] = *reinterpret_cast<const uint32_t*>(x4 + row * ld4 + k / 2);
+    if (k2 * 256 + lane * 8 < K) {
+      c[u] = *reinterpret_cast<const uint32_t*>(xi + k2 * 128);
       b[u] = sf[sf_word(row, 2 * k2 + (lane >> 4), 2 * k2s) + ((lane >> 2) & 3)];
     }
   }
+  __nv_bfloat16* oo = out + row * ldo + lane * 8;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const int64_t unit = warp * kUnits + u, row = unit / k2s, k = (unit % k2s) * 256 + lane * 8;
-    if (unit >= units || k >= K) continue;
+    const int k = (first + u) * 256;
+    if (k + lane * 8 >= K) continue;
     const float s = scale_value(b[u]);
     uint32_t o[4];
 #pragma unroll
@@ -151,11 +238,9 @@ __global__ void __launch_bounds__(kQuantThreads)
       const float2 f = __half22float2(__half2(h));
       o[j] = pack_bf16x2(f.x * s, f.y * s);
     }
-    *reinterpret_cast<uint4*>(out + row * ldo + k) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(oo + k) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
-
-static bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
 // Codes [M, K / 2] and scale atoms of an [M, K] matrix.
 static void check_codes(const char* op, const at::Tensor& x4, const at::Tensor& sf, int64_t M, int64_t K,
@@ -169,7 +254,7 @@ static void check_codes(const char* op, const at::Tensor& x4, const at::Tensor& 
             op, ": scales must be uint8 atoms [ceil(M / 128), 2 ceil(K / 256), 512]");
 }
 
-static void check_rows(const char* op, const char* what, const at::Tensor& x, const at::Device& dev) {
+void check_rows(const char* op, const char* what, const at::Tensor& x, const at::Device& dev) {
   GSB_CHECK(x.is_cuda() && x.device() == dev && x.scalar_type() == at::kBFloat16 && x.dim() == 2 &&
                 (x.size(1) == 1 || x.stride(1) == 1) && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && aligned16(x),
             op, ": ", what, " must be bf16 [M, K] on one CUDA device with 16-byte aligned rows");
@@ -178,10 +263,29 @@ static void check_rows(const char* op, const char* what, const at::Tensor& x, co
             op, ": K must be a positive multiple of 32");
 }
 
-static unsigned unit_grid(const char* op, int64_t units) {
-  const int64_t per = (int64_t)(kQuantThreads / 32) * kUnits, n = (units + per - 1) / per;
-  GSB_CHECK(n < (int64_t(1) << 31), op, ": too many rows");
-  return (unsigned)n;
+// Warps per row and in all, and the grid, of the streaming kernels.
+struct StreamGrid {
+  uint32_t per_row, warps;
+  dim3 grid;
+};
+static StreamGrid stream_grid(const char* op, int64_t M, int64_t K) {
+  const int64_t per_row = (k_tiles(K) / 2 + kUnits - 1) / kUnits, warps = M * per_row;
+  GSB_CHECK(warps < (int64_t(1) << 32) - 64, op, ": too many rows");
+  return {(uint32_t)per_row, (uint32_t)warps, dim3((unsigned)((warps + kQuantThreads / 32 - 1) / (kQuantThreads / 32)))};
+}
+
+void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf) {
+  const auto opt = at::TensorOptions().dtype(at::kByte).device(dev);
+  if (!x4.defined()) x4 = at::empty({M, K / 2}, opt);
+  if (!sf.defined()) sf = at::empty({(M + 127) / 128, k_tiles(K), 512}, opt);
+}
+
+void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
+                     cudaStream_t st) {
+  const StreamGrid g = stream_grid("quantize_mxfp4", M, K);
+  launch_dependent(quantize_mxfp4_kernel, g.grid, dim3(kQuantThreads), 0, st,
+                   reinterpret_cast<const __nv_bfloat16*>(x), ldx, (int)K, (int)(k_tiles(K) / 2), g.per_row, g.warps, x4,
+                   ld4, sf);
 }
 
 }  // namespace f4
@@ -189,28 +293,35 @@ static unsigned unit_grid(const char* op, int64_t units) {
 
 using namespace gsb;
 
-// x [M, K] bf16 -> x4 [M, K / 2] codes, sf [ceil(M / 128), 2 ceil(K / 256), 512] scale atoms.
-void gsb_quantize_mxfp4(const at::Tensor& x, const at::Tensor& x4, const at::Tensor& sf) {
+// x [M, K] bf16 -> (x4 [M, K / 2] codes, sf [ceil(M / 128), 2 ceil(K / 256), 512] scale atoms).
+std::tuple<at::Tensor, at::Tensor> gsb_quantize_mxfp4(const at::Tensor& x, const c10::optional<at::Tensor>& x4_,
+                                                      const c10::optional<at::Tensor>& sf_) {
   f4::check_rows("quantize_mxfp4", "x", x, x.device());
-  const int64_t M = x.size(0), K = x.size(1), k2s = f4::k_tiles(K) / 2;
-  f4::check_codes("quantize_mxfp4", x4, sf, M, K, x.device());
-  if (M == 0) return;
+  const int64_t M = x.size(0), K = x.size(1);
   c10::cuda::CUDAGuard g(x.device());
-  auto st = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
-  launch_dependent(f4::quantize_mxfp4_kernel, dim3(f4::unit_grid("quantize_mxfp4", M * k2s)), dim3(f4::kQuantThreads),
-                   0, st, reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()), x.stride(0), K, k2s, M * k2s,
-                   x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>());
+  at::Tensor x4 = x4_.value_or(at::Tensor()), sf = sf_.value_or(at::Tensor());
+  f4::make_codes(M, K, x.device(), x4, sf);
+  f4::check_codes("quantize_mxfp4", x4, sf, M, K, x.device());
+  if (M > 0)
+    f4::quantize_launch(x.data_ptr(), x.stride(0), M, K, x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(),
+                        c10::cuda::getCurrentCUDAStream(x.device().index()).stream());
+  return {x4, sf};
 }
 
 // RMSNorm of x [M, H] and its quantisation; `out` (optional) also receives the bf16 rows.
-void gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps, const at::Tensor& x4,
-                       const at::Tensor& sf, const c10::optional<at::Tensor>& out) {
+std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps,
+                                                     const c10::optional<at::Tensor>& x4_,
+                                                     const c10::optional<at::Tensor>& sf_,
+                                                     const c10::optional<at::Tensor>& out) {
   f4::check_rows("rmsnorm_mxfp4", "x", x, x.device());
   const int64_t M = x.size(0), H = x.size(1);
   GSB_CHECK(H <= 16384, "rmsnorm_mxfp4: at most 16384 columns");
   GSB_CHECK(w.device() == x.device() && w.scalar_type() == at::kBFloat16 && w.is_contiguous() && w.numel() == H &&
                 f4::aligned16(w),
             "rmsnorm_mxfp4: the weight must be bf16 [H], contiguous and 16-byte aligned");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor x4 = x4_.value_or(at::Tensor()), sf = sf_.value_or(at::Tensor());
+  f4::make_codes(M, H, x.device(), x4, sf);
   f4::check_codes("rmsnorm_mxfp4", x4, sf, M, H, x.device());
   __nv_bfloat16* op = nullptr;
   int64_t ldo = 0;
@@ -220,8 +331,7 @@ void gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps, con
     op = reinterpret_cast<__nv_bfloat16*>(out->data_ptr());
     ldo = out->stride(0);
   }
-  if (M == 0) return;
-  c10::cuda::CUDAGuard g(x.device());
+  if (M == 0) return {x4, sf};
   auto st = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   auto* xp = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
@@ -230,22 +340,34 @@ void gsb_rmsnorm_mxfp4(const at::Tensor& x, const at::Tensor& w, double eps, con
     launch_dependent(kernel, dim3((unsigned)M), dim3(256), 0, st, xp, x.stride(0), wp, (int)H, (float)eps,
                      x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
   };
+  if (M >= f4::kWarpNormRows && H <= 4096) {
+    launch_dependent(H <= 2048 ? f4::rmsnorm_mxfp4_warp_kernel<1> : f4::rmsnorm_mxfp4_warp_kernel<2>,
+                     dim3((unsigned)((M + 7) / 8)), dim3(256), 0, st, xp, x.stride(0), wp, (int)M, (int)H, (float)eps,
+                     x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
+    return {x4, sf};
+  }
   if (vpt <= 1) go(f4::rmsnorm_mxfp4_kernel<1>);
   else if (vpt <= 2) go(f4::rmsnorm_mxfp4_kernel<2>);
   else if (vpt <= 4) go(f4::rmsnorm_mxfp4_kernel<4>);
   else go(f4::rmsnorm_mxfp4_kernel<8>);
+  return {x4, sf};
 }
 
 // out [M, K] bf16 <- codes x4 and scale atoms sf.
-void gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, const at::Tensor& out) {
-  f4::check_rows("dequantize_mxfp4", "out", out, out.device());
-  const int64_t M = out.size(0), K = out.size(1), k2s = f4::k_tiles(K) / 2;
-  f4::check_codes("dequantize_mxfp4", x4, sf, M, K, out.device());
-  if (M == 0) return;
-  c10::cuda::CUDAGuard g(out.device());
-  auto st = c10::cuda::getCurrentCUDAStream(out.device().index()).stream();
-  f4::dequantize_mxfp4_kernel<<<(::gsb::count_launch(), f4::unit_grid("dequantize_mxfp4", M * k2s)), f4::kQuantThreads,
-                                0, st>>>(x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), K, k2s,
-                                         M * k2s, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), out.stride(0));
-  GSB_CUDA_CHECK(cudaGetLastError());
+at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, const c10::optional<at::Tensor>& out_) {
+  GSB_CHECK(x4.is_cuda() && x4.dim() == 2, "dequantize_mxfp4: codes must be a CUDA matrix");
+  const int64_t M = x4.size(0), K = x4.size(1) * 2;
+  c10::cuda::CUDAGuard g(x4.device());
+  at::Tensor out = out_.has_value() ? *out_
+                                    : at::empty({M, K}, at::TensorOptions().dtype(at::kBFloat16).device(x4.device()));
+  f4::check_rows("dequantize_mxfp4", "out", out, x4.device());
+  GSB_CHECK(out.size(0) == M && out.size(1) == K, "dequantize_mxfp4: out must be [M, K]");
+  f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
+  if (M == 0) return out;
+  const f4::StreamGrid s = f4::stream_grid("dequantize_mxfp4", M, K);
+  launch_dependent(f4::dequantize_mxfp4_kernel, s.grid, dim3(f4::kQuantThreads), 0,
+                   c10::cuda::getCurrentCUDAStream(x4.device().index()).stream(), x4.data_ptr<uint8_t>(),
+                   x4.stride(0), sf.data_ptr<uint8_t>(), (int)K, (int)(f4::k_tiles(K) / 2), s.per_row, s.warps,
+                   reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), out.stride(0));
+  return out;
 }

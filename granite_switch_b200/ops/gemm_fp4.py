@@ -29,40 +29,22 @@ SWIGLU_TILE = 128  # gate/up rows of a packed weight alternate in runs of 64
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
-def _empty_codes(m: int, k: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    if k % BLOCK or k <= 0:
-        raise ValueError(f"K must be a positive multiple of {BLOCK}, got {k}")
-    return (torch.empty(m, k // 2, dtype=torch.uint8, device=device),
-            torch.empty((m + 127) // 128, (k + 255) // 256 * 2, 512, dtype=torch.uint8, device=device))
-
-
 def quantize_rows_mxfp4(x: torch.Tensor, x4: torch.Tensor | None = None, sf: torch.Tensor | None = None):
     """``x [M, K]`` bf16 -> (codes ``[M, K / 2]``, scale atoms), on the GPU."""
-    if x4 is None or sf is None:
-        c, s = _empty_codes(x.shape[0], x.shape[1], x.device)
-        x4, sf = c if x4 is None else x4, s if sf is None else sf
-    native().quantize_mxfp4(x, x4, sf)
-    return x4, sf
+    return native().quantize_mxfp4(x, x4, sf)
 
 
 def dequantize_mxfp4(x4: torch.Tensor, sf: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """The bf16 values ``[M, K]`` that codes and scale atoms stand for (exact), on the GPU."""
-    if out is None:
-        out = torch.empty(x4.shape[0], x4.shape[1] * 2, dtype=torch.bfloat16, device=x4.device)
-    native().dequantize_mxfp4(x4, sf, out)
-    return out
+    return native().dequantize_mxfp4(x4, sf, out)
 
 
 def rmsnorm_mxfp4(x: torch.Tensor, w: torch.Tensor, eps: float, x4: torch.Tensor | None = None,
                   sf: torch.Tensor | None = None, out: torch.Tensor | None = None):
     """RMSNorm of ``x [M, H]`` bf16 and its quantisation in one pass: ``x w / sqrt(mean(x^2) + eps)``
     in fp32, rounded once, to 4 bits. ``out [M, H]`` also receives the bf16 rows that
-    :func:`ops.elementwise.rmsnorm` writes (the LoRA shrink reads them)."""
-    if x4 is None or sf is None:
-        c, s = _empty_codes(x.shape[0], x.shape[1], x.device)
-        x4, sf = c if x4 is None else x4, s if sf is None else sf
-    native().rmsnorm_mxfp4(x, w, float(eps), x4, sf, out)
-    return x4, sf
+    :func:`ops.elementwise.rmsnorm` writes (the LoRA shrink reads them). H is at most 16384."""
+    return native().rmsnorm_mxfp4(x, w, eps, x4, sf, out)
 
 
 def mxfp4_gemm(x4, sfx, w4, sfw, out=None, *, epi: int = EPI_STORE, scale: float = 1.0, residual=None, s=None,
@@ -74,18 +56,15 @@ def mxfp4_gemm(x4, sfx, w4, sfw, out=None, *, epi: int = EPI_STORE, scale: float
     ``s`` the masked shrink output, ``tile_mask`` the adapters present per 128 rows); slice
     bounds are multiples of 128.
     """
-    n = w4.shape[0]
-    if out is None:
-        out = torch.empty(x4.shape[0], n, dtype=torch.bfloat16, device=x4.device)
-    native().mxfp4_gemm(x4, sfx, w4, sfw, out, int(epi), float(scale), residual, s, lb, tile_mask, int(rank),
-                        int(num_adapters), list(slice_bounds) if slice_bounds is not None else [0, n],
-                        err_buffer(x4.device))
-    return out
+    return native().mxfp4_gemm(x4, sfx, w4, sfw, out, epi, scale, residual, s, lb, tile_mask, rank, num_adapters,
+                               slice_bounds, err_buffer(x4.device))
 
 
-def mxfp4_linear(x, w4, sfw, out=None, **kw):
-    """:func:`mxfp4_gemm` of bf16 rows ``x [M, K]``, quantised on the way."""
-    return mxfp4_gemm(*quantize_rows_mxfp4(x), w4, sfw, out, **kw)
+def mxfp4_linear(x, w4, sfw, out=None, *, epi: int = EPI_STORE, scale: float = 1.0, residual=None, s=None, lb=None,
+                 tile_mask=None, rank: int = 0, num_adapters: int = 0, slice_bounds=None):
+    """:func:`mxfp4_gemm` of bf16 rows ``x [M, K]``, quantised into a workspace of the call."""
+    return native().mxfp4_linear(x, w4, sfw, out, epi, scale, residual, s, lb, tile_mask, rank, num_adapters,
+                                 slice_bounds, err_buffer(x.device))
 
 
 def mxfp4_gemm_swiglu(x4, sfx, w4, sfw, a4=None, sf=None, act=None, *, s=None, lb=None, tile_mask=None,
@@ -95,12 +74,8 @@ def mxfp4_gemm_swiglu(x4, sfx, w4, sfw, a4=None, sf=None, act=None, *, s=None, l
     ``w4`` alternate in runs of 64 (``models.packing.interleave_gate_up(w, SWIGLU_TILE)``), I is
     a multiple of 64. With LoRA ``s`` holds the gate's columns, then the up's, and ``lb`` is
     :func:`swiglu_lora_b` of the interleaved expand weights."""
-    if a4 is None or sf is None:
-        c, q = _empty_codes(x4.shape[0], w4.shape[0] // 2, x4.device)
-        a4, sf = c if a4 is None else a4, q if sf is None else sf
-    native().mxfp4_gemm_swiglu(x4, sfx, w4, sfw, a4, sf, act, s, lb, tile_mask, int(rank), int(num_adapters),
-                               err_buffer(x4.device))
-    return a4, sf
+    return native().mxfp4_gemm_swiglu(x4, sfx, w4, sfw, a4, sf, act, s, lb, tile_mask, rank, num_adapters,
+                                      err_buffer(x4.device))
 
 
 def swiglu_lora_b(lb: torch.Tensor) -> torch.Tensor:

@@ -115,7 +115,8 @@ def test_quantize_edges_and_strides():
     assert (back[2].double() == 6 * 2.0 ** 125).all()
 
 
-@pytest.mark.parametrize("m,h", [(1, 32), (5, 256), (33, 2080), (130, 4096), (3, 16384)])
+@pytest.mark.parametrize("m,h", [(1, 32), (5, 256), (33, 2080), (130, 4096), (3, 16384), (1300, 2048), (1301, 4096),
+                                 (1200, 2080), (1190, 96)])
 @pytest.mark.parametrize("with_out", [False, True])
 def test_rmsnorm_quantised(m, h, with_out):
     from granite_switch_b200.ops import elementwise as E
@@ -350,6 +351,8 @@ def test_refusals():
         lambda: F.quantize_rows_mxfp4(x.float()),
         lambda: F.quantize_rows_mxfp4(x[:, 1:33]),                                  # not 16-byte aligned
         lambda: F.quantize_rows_mxfp4(x.t()),
+        lambda: F.quantize_rows_mxfp4(x[:, :48]),
+        lambda: F.mxfp4_linear(x[:, :128], *b),
         lambda: F.quantize_rows_mxfp4(x, sf=a[1][:, :1]),
         lambda: F.quantize_rows_mxfp4(x, x4=a[0][:8]),
         lambda: F.rmsnorm_mxfp4(x, torch.ones(128, device="cuda").bfloat16(), 1e-5),
