@@ -77,14 +77,13 @@ __device__ __forceinline__ int64_t sf_word(int64_t row, int64_t kt, int64_t ktil
   return ((row >> 7) * ktiles + kt) * 512 + 16 * (r & 31) + 4 * (r >> 5);
 }
 
-// Scale bytes of a whole warp's 256 neighbours (row `row` from K index 256 * k2; `byte` of
-// each lane's block of four lanes) -> the words of both K tiles.
-__device__ __forceinline__ void store_scales256(uint32_t byte, int lane, uint8_t* sf, int64_t row, int64_t k2,
-                                                int64_t ktiles) {
+// Scale bytes of a whole warp's 256 neighbours (`byte` of each lane's block of four lanes)
+// -> the words of both K tiles; `sf` is the first tile's word.
+__device__ __forceinline__ void store_scales256(uint32_t byte, int lane, uint8_t* sf) {
   uint32_t word = byte << (8 * ((lane >> 2) & 3));
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
   word |= __shfl_xor_sync(0xffffffffu, word, 8);
-  if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(sf + sf_word(row, 2 * k2 + (lane >> 4), ktiles)) = word;
+  if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(sf + (lane >> 4) * 512) = word;
 }
 
 }  // namespace f4

@@ -25,7 +25,6 @@ namespace gsb {
 namespace f4 {
 
 constexpr int kQuantThreads = 256;
-constexpr int kWarpNormRows = 1184;
 constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 
 __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
@@ -66,55 +65,64 @@ __global__ void __launch_bounds__(kQuantThreads)
     if (k + lane * 8 < K) q[u] = *reinterpret_cast<const uint4*>(xr + k);
   }
   uint8_t* xo = x4 + row * ld4 + lane * 4;
+  uint8_t* so = sf + sf_word(row, 2 * first, 2 * k2s);
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     const int k2 = first + u, k = k2 * 256 + lane * 8;
     if (k2 >= k2s) break;  // the whole warp
     const uint32_t byte = scale_byte(quad_max(max_abs_bits_bf16(q[u])));
     float v[8];
-    unpack8(byte == 255u ? make_uint4(0u, 0u, 0u, 0u) : q[u], v);
-    if (k < K) *reinterpret_cast<uint32_t*>(xo + k2 * 128) = pack8(v, inv_scale(byte));
-    store_scales256(byte, lane, sf, row, k2, 2 * k2s);
+    unpack8(q[u], v);
+    const uint32_t codes = pack8(v, inv_scale(byte));
+    if (k < K) *reinterpret_cast<uint32_t*>(xo + k2 * 128) = byte == 255u ? 0u : codes;
+    store_scales256(byte, lane, so + u * 1024);
   }
 }
 
-// Normalised values of eight inputs -> codes, scales and (optionally) the bf16 row.
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Eight normalised values -> codes, scales and (optionally) their part of the bf16 row. The
+// products x w are exact, and one multiplication by inv (times the block's power of two,
+// exact too) rounds each value; the maximum may be taken before it, since rounding keeps order.
 __device__ __forceinline__ void norm_store8(const uint4& xq, const uint4& wq, float inv, bool inside, int lane,
-                                            int64_t row, int v, int64_t ktiles, uint8_t* x4_row, uint8_t* sf,
-                                            __nv_bfloat16* out_row) {
+                                            uint8_t* codes_out, uint8_t* sf, uint4* out) {
   float f[8], g[8], y[8];
   unpack8(xq, f);
   unpack8(wq, g);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = inside ? (f[j] * g[j]) * inv : 0.f;  // inv is NaN in a row that is not finite
-  const uint32_t byte = scale_byte(quad_max(max_abs_bits(y)));
+  for (int j = 0; j < 8; ++j) y[j] = f[j] * g[j];
+  float top = fabsf(y[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = max_nan(top, fabsf(y[j]));
+  uint32_t byte = scale_byte(quad_max(__float_as_uint(fabsf(top * inv))));
+  byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
+  float s = inv_scale(byte);
+  if (byte < 32u) {  // inv * 2^-e may overflow
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] *= inv;
+  } else {
+    s *= inv;
+  }
+  const uint32_t codes = pack8(y, s);
   if (inside) {
-    if (out_row != nullptr) {
+    *reinterpret_cast<uint32_t*>(codes_out) = byte == 255u ? 0u : codes;
+    if (out != nullptr) {
       uint32_t o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
                            __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
-      reinterpret_cast<uint4*>(out_row)[v] = make_uint4(o[0], o[1], o[2], o[3]);
+      *out = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    if (byte == 255u) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.f;
-    }
-    *reinterpret_cast<uint32_t*>(x4_row + v * 4) = pack8(y, inv_scale(byte));
   }
-  store_scales256(byte, lane, sf, row, v / 32, ktiles);
+  store_scales256(byte, lane, sf);
 }
 
-__device__ __forceinline__ float sum_squares8(const uint4& q, float ss) {
-  float f[8];
-  unpack8(q, f);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) ss += f[2 * j] * f[2 * j] + f[2 * j + 1] * f[2 * j + 1];
-  return ss;
-}
-
-// One CTA per row (few rows, or wide ones): the sum of squares in the RMSNorm kernel's order.
+// One CTA per row; the sum of squares in the RMSNorm kernel's order.
 template <int VPT>
 __global__ void __launch_bounds__(256)
     rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w, int H,
@@ -126,81 +134,44 @@ __global__ void __launch_bounds__(256)
   const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
   const uint4* wv = reinterpret_cast<const uint4*>(w);
   const int nvec = H / 8, nvec_pad = (int)k_tiles(H) * 16;
-  uint4 buf[VPT], wbuf[VPT];
+  uint4 buf[VPT];
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * 256;
-    buf[i] = wbuf[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (v < nvec) {
-      buf[i] = xv[v];
-      wbuf[i] = wv[v];
-    }
+    buf[i] = v < nvec ? xv[v] : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (threadIdx.x + i * 256 < nvec) ss = sum_squares8(buf[i], ss);
-  __shared__ float red[32];
+  for (int i = 0; i < VPT; ++i) {
+    const uint32_t p[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(p[j]);
+      ss += f.x * f.x + f.y * f.y;
+    }
+  }
+  __shared__ float red[8], s_inv;
   ss = warp_sum(ss);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
   __syncthreads();
   if (threadIdx.x < 32) {
     float t = threadIdx.x < 8 ? red[threadIdx.x] : 0.f;
     t = warp_sum(t);
-    if (threadIdx.x == 0) red[0] = t;
+    if (threadIdx.x == 0) s_inv = rsqrtf(t / (float)H + eps);
   }
   __syncthreads();
-  const float inv = rsqrtf(red[0] / (float)H + eps);
-  __nv_bfloat16* orow = out ? out + r * ldo : nullptr;
+  const float inv = s_inv;
+  const int lane = threadIdx.x & 31;
+  uint8_t* codes = x4 + r * ld4 + threadIdx.x * 4;
+  uint8_t* scales = sf + sf_word(r, 2 * (threadIdx.x >> 5), k_tiles(H));
+  uint4* ov = out ? reinterpret_cast<uint4*>(out + r * ldo) + threadIdx.x : nullptr;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * 256;
     if (v >= nvec_pad) break;  // the whole warp: nvec_pad is a multiple of 32
-    norm_store8(buf[i], wbuf[i], inv, v < nvec, threadIdx.x & 31, r, v, k_tiles(H), x4 + r * ld4, sf, orow);
-  }
-}
-
-// One warp per row (many rows of up to 4096 columns): no barrier, and the whole row's loads
-// in flight. Lane l holds what the threads l, l + 32, ... of the CTA kernel hold and adds in
-// the same order, so both give the same bits.
-template <int NI>  // ceil(H / 2048)
-__global__ void __launch_bounds__(256)
-    rmsnorm_mxfp4_warp_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w,
-                              int M, int H, float eps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf,
-                              __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  griddep_wait();
-  griddep_launch();
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= M) return;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
-  const uint4* wv = reinterpret_cast<const uint4*>(w);
-  const int nvec = H / 8, units = (int)k_tiles(H) / 2;
-  uint4 buf[8 * NI];
-#pragma unroll
-  for (int j = 0; j < 8 * NI; ++j) {
-    const int v = lane + 32 * j;
-    buf[j] = v < nvec ? xv[v] : make_uint4(0u, 0u, 0u, 0u);
-  }
-  float a[8];
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (lane + 32 * (t + 8 * i) < nvec) ss = sum_squares8(buf[t + 8 * i], ss);
-    a[t] = warp_sum(ss);
-  }
-  const float total = ((a[0] + a[4]) + (a[2] + a[6])) + ((a[1] + a[5]) + (a[3] + a[7]));
-  const float inv = rsqrtf(total / (float)H + eps);
-  __nv_bfloat16* orow = out ? out + r * ldo : nullptr;
-#pragma unroll
-  for (int j = 0; j < 8 * NI; ++j) {
-    if (j >= units) break;
-    const int v = lane + 32 * j;
     const bool inside = v < nvec;
-    norm_store8(buf[j], inside ? wv[v] : make_uint4(0u, 0u, 0u, 0u), inv, inside, lane, r, v, 2 * units, x4 + r * ld4,
-                sf, orow);
+    norm_store8(buf[i], inside ? wv[v] : make_uint4(0u, 0u, 0u, 0u), inv, inside, lane, codes + i * 1024,
+                scales + i * 8 * 1024, ov ? ov + i * 256 : nullptr);
   }
 }
 
@@ -340,12 +311,6 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
     launch_dependent(kernel, dim3((unsigned)M), dim3(256), 0, st, xp, x.stride(0), wp, (int)H, (float)eps,
                      x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
   };
-  if (M >= f4::kWarpNormRows && H <= 4096) {
-    launch_dependent(H <= 2048 ? f4::rmsnorm_mxfp4_warp_kernel<1> : f4::rmsnorm_mxfp4_warp_kernel<2>,
-                     dim3((unsigned)((M + 7) / 8)), dim3(256), 0, st, xp, x.stride(0), wp, (int)M, (int)H, (float)eps,
-                     x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
-    return {x4, sf};
-  }
   if (vpt <= 1) go(f4::rmsnorm_mxfp4_kernel<1>);
   else if (vpt <= 2) go(f4::rmsnorm_mxfp4_kernel<2>);
   else if (vpt <= 4) go(f4::rmsnorm_mxfp4_kernel<4>);
