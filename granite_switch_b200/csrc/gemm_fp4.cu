@@ -63,7 +63,6 @@ struct SplitParams {
   int mt_rows;        // tokens per tile
   int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
   int tmem_cols;
-  int early;          // load weights before the wait for the kernel before this one
   const uint8_t* sfx;
   const uint8_t* sfw;
   float scale;
@@ -122,6 +121,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
 template <int OFF>
 __device__ __forceinline__ void st_dsmem_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0+%2], %1;" ::"r"(addr), "f"(v), "n"(OFF));
@@ -158,6 +164,14 @@ __device__ __forceinline__ int lora_column(const LoraParams& l, uint64_t mask, i
 }
 
 __device__ __forceinline__ float swiglu_f(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+}  // namespace f4
+}  // namespace gsb
+
+#include "gemv_fp4.cuh"
+
+namespace gsb {
+namespace f4 {
 
 template <int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -208,18 +222,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem_base = tmem_slot;
   griddep_launch();
 
-  // Launched as a dependent of the quantiser of its own call, the kernel loads the first
-  // stages' weights while that one still runs; nothing else is read before the wait.
-  auto load_w = [&](int i, int s) {
-    const int kb = kb_lo + i;
-    uint8_t* sw = smem + s * p.stage_bytes;
-    mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
-    tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
-    bulk_load(sw + W_BYTES + x_bytes, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
-  };
-  const int early = p.early ? min(stages, n_main) : 0;
+  // The first stages' weights start towards L2 before the wait for the kernel before this
+  // one (a prefetch into L2 reads nothing that could be stale).
   if (warp == 0 && lane == 0)
-    for (int i = 0; i < early; ++i) load_w(i, i);  // a fresh ring: no wait for empty stages
+    for (int i = 0; i < min(stages, n_main); ++i) tma_prefetch_2d(&tm_w, (kb_lo + i) * BKB, n0);
   griddep_wait();
 
   uint64_t mask0 = 0ull, mask1 = 0ull;  // adapters of the token tile's two 128-row halves
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < total; ++i) {
         const int s = i % stages;
         const uint32_t ph = (i / stages) & 1;
-        if (i >= early && (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait))) {
+        if (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait)) {
           abort_flag = 1;
           break;
         }
@@ -249,7 +255,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint8_t* sf = sx + x_bytes;
         if (i < n_main) {
           const int kb = kb_lo + i;
-          if (i >= early) load_w(i, s);
+          mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
+          tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
+          bulk_load(sf, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
           tma_load_2d(sx, &tm_x, &full_bar[s], kb * BKB, m0);
           for (int t = 0; t < xt; ++t)
             bulk_load(sf + 1024 * (1 + t), p.sfx + ((size_t)(m0 / 128 + t) * p.kstages + kb) * 1024, 1024,
@@ -789,6 +797,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 
 // ---------------------------------------------------------------------------- host
 constexpr int kMaxDevices = 64;
+constexpr int GV_MAX_SMEM = 200 * 1024;
 
 static int current_device() {
   int dev = 0;
@@ -983,6 +992,45 @@ static CUtensorMap make_tmap_sf(const Codes& c, int64_t kstages, uint32_t tiles_
   return m;
 }
 
+// Two CTAs per SM where a step of both fits beside their tokens, else one; as many steps in
+// flight as fit and the CTA has. 0 stages: the kernel does not take the call.
+struct GemvPlan {
+  int per_sm, stages, smem;
+};
+static GemvPlan gemv_plan(int MT, int kblocks, int units, int steps) {
+  const int stage = gemv_stage(kblocks), tokens = gemv_tokens(MT, kblocks);
+  for (int per_sm = 2; per_sm >= 1; --per_sm) {
+    const int room = (per_sm == 2 ? 110 * 1024 : GV_MAX_SMEM) - tokens;
+    if (room < stage) continue;
+    const int ctas = per_sm * num_sms(), have = (units + ctas - 1) / ctas * steps;
+    const int stages = std::min({GV_MAX_STAGES, room / stage, have});
+    return {per_sm, stages, stages * stage + tokens};
+  }
+  return {0, 0, 0};
+}
+
+template <int MT, int EPI>
+static void launch_gemv(GemvParams p, const LoraParams& lp, bool dependent, uint32_t* err, cudaStream_t st) {
+  auto kfn = mxfp4_gemv_kernel<MT, EPI>;
+  static bool set[kMaxDevices] = {false};
+  const int dev = current_device();
+  if (!set[dev]) {
+    GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, GV_MAX_SMEM));
+    set[dev] = true;
+  }
+  const int units = EPI == kEpiSwiGLU ? p.N / 64 : (p.N + GV_STEP - 1) / GV_STEP;
+  const GemvPlan g = gemv_plan(MT, p.kblocks, units, EPI == kEpiSwiGLU ? 64 / GV_STEP : 1);
+  p.stages = g.stages;
+  launch(kfn, dim3((unsigned)std::min(units, g.per_sm * num_sms())), GV_THREADS, g.smem, 1, dependent, st, p, lp, err);
+}
+
+template <int EPI>
+static void gemv_by_rows(const GemvParams& p, const LoraParams& lp, bool dependent, uint32_t* err, cudaStream_t st) {
+  if (p.M == 1) launch_gemv<1, EPI>(p, lp, dependent, err, st);
+  else if (p.M == 2) launch_gemv<2, EPI>(p, lp, dependent, err, st);
+  else launch_gemv<4, EPI>(p, lp, dependent, err, st);
+}
+
 static CUtensorMap make_tmap_codes(const Codes& c, int64_t K, uint32_t box_rows) {
   return make_tmap_2d(c.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)c.rows, (uint64_t)K / 2, (uint64_t)c.ld, BKB,
                       box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -996,13 +1044,19 @@ struct LoraArgs {
   std::vector<int64_t> slice_bounds;
 };
 
-// One product on stream `st` of `dev`, the current device. `a4` (codes and scales of the
-// output) for swiglu, `out` otherwise (for swiglu: the bf16 copy, or null). `own_quantiser`:
-// the kernel before in the stream is this call's quantiser of x, which neither writes
-// weights nor lets a dependent start before all that came earlier is done.
-static void run_gemm(const Codes& x, const Codes& w, int64_t K, const at::Tensor* out, int epi, double scale,
+// Tokens of a product: codes, or bf16 rows (`bf` not null, codes filled in when quantised).
+struct Tokens {
+  Codes c;
+  const void* bf;
+  int64_t ldbf;
+};
+
+// One product on the current stream of `dev`, the current device. `a4` (codes and scales of
+// the output) for swiglu, `out` otherwise (for swiglu: the bf16 copy, or null).
+static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out, int epi, double scale,
                      const c10::optional<at::Tensor>& residual, const Codes* a4, const LoraArgs& la,
-                     const at::Tensor& err, const at::Device& dev, bool own_quantiser, cudaStream_t st) {
+                     const at::Tensor& err, const at::Device& dev) {
+  Codes& x = t.c;
   GSB_CHECK(K >= kBlock && K % kBlock == 0 && K < (int64_t(1) << 31), "mxfp4_gemm: K must be a positive multiple of 32");
   GSB_CHECK(x.rows < (int64_t(1) << 24) && w.rows > 0 && w.rows < (int64_t(1) << 24) && w.rows % 8 == 0,
             "mxfp4_gemm: N must be a positive multiple of 8");
@@ -1065,8 +1119,53 @@ static void run_gemm(const Codes& x, const Codes& w, int64_t K, const at::Tensor
     }
   }
   if (M == 0) return;
+  auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());
-  const bool dependent = own_quantiser || pdl_enabled();
+  bool dependent = pdl_enabled();
+
+  if (M <= GV_MAX_M && gemv_stage((int)(K / 32)) + gemv_tokens(GV_MAX_M, (int)(K / 32)) <= GV_MAX_SMEM) {
+    GemvParams g{};
+    g.M = M;
+    g.N = N;
+    g.kblocks = (int)(K / 32);
+    g.x = reinterpret_cast<const __nv_bfloat16*>(t.bf);
+    g.ldx = t.ldbf;
+    g.x4 = x.q;
+    g.ld4 = x.ld;
+    g.sfx = x.sf;
+    g.w4 = w.q;
+    g.ldw = w.ld;
+    g.sfw = w.sf;
+    g.scale = p.scale;
+    g.out = reinterpret_cast<__nv_bfloat16*>(p.out);
+    g.ldo = p.ldo;
+    g.residual = p.residual;
+    g.ldr = p.ldr;
+    g.a4 = p.a4;
+    g.lda4 = p.lda4;
+    g.sfa_out = p.sfa_out;
+    g.lora = p.lora;
+    if (lora) {
+      g.s = reinterpret_cast<const __nv_bfloat16*>(la.s->data_ptr());
+      g.lds = la.s->stride(0);
+      g.lb = reinterpret_cast<const __nv_bfloat16*>(la.lb->data_ptr());
+      g.ldlb = la.lb->stride(0);
+    }
+    switch (epi) {
+      case kEpiStore: gemv_by_rows<kEpiStore>(g, p.lp, dependent, ep, st); break;
+      case kEpiResAdd: gemv_by_rows<kEpiResAdd>(g, p.lp, dependent, ep, st); break;
+      default: gemv_by_rows<kEpiSwiGLU>(g, p.lp, dependent, ep, st); break;
+    }
+    return;
+  }
+  at::Tensor work;  // codes and scales of bf16 rows; the stream orders its reuse
+  if (t.bf != nullptr) {
+    const int64_t code_bytes = (M * (K / 2) + 1023) / 1024 * 1024;
+    work = at::empty({code_bytes + (M + 127) / 128 * k_tiles(K) * 512}, at::TensorOptions().dtype(at::kByte).device(dev));
+    x = Codes{work.data_ptr<uint8_t>(), K / 2, work.data_ptr<uint8_t>() + code_bytes, M};
+    quantize_launch(t.bf, t.ldbf, M, K, x.q, x.ld, x.sf, st);
+    dependent = true;  // of the quantiser, which lets it start when all before is done
+  }
   auto tmap_s = [&](uint32_t rows) {
     return make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32,
                              rows, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -1116,7 +1215,6 @@ static void run_gemm(const Codes& x, const Codes& w, int64_t K, const at::Tensor
   p.ks = s.ks;
   p.rows_per = rows_per_part(s.mt_rows, s.ks);
   p.tmem_cols = s.tmem_cols;
-  p.early = own_quantiser ? 1 : 0;
   const uint32_t mp = (uint32_t)((s.mt_rows + 15) / 16 * 16);
   const CUtensorMap tw = make_tmap_codes(w, K, BW), tx = make_tmap_codes(x, K, mp);
   const CUtensorMap tlb = lora ? tmap_lb(BW) : tw, ts = lora ? tmap_s(std::min(mp, 128u)) : tx;
@@ -1154,10 +1252,10 @@ at::Tensor gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at:
   const f4::Codes x = f4::check_operand("x", x4, sfx, K, dev), w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
   const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(x.rows, w.rows, dev);
-  f4::run_gemm(x, w, K, &out, (int)epi, scale, residual, nullptr,
+  f4::run_gemm(f4::Tokens{x, nullptr, 0}, w, K, &out, (int)epi, scale, residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
                             slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
-               err, dev, false, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+               err, dev);
   return out;
 }
 
@@ -1174,18 +1272,12 @@ at::Tensor gsb_mxfp4_linear(const at::Tensor& x, const at::Tensor& w4, const at:
   const at::Device dev = x.device();
   const f4::Codes w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
-  const int64_t code_bytes = (M * (K / 2) + 1023) / 1024 * 1024;
-  const at::Tensor work = at::empty({code_bytes + (M + 127) / 128 * f4::k_tiles(K) * 512},
-                                    at::TensorOptions().dtype(at::kByte).device(dev));
-  uint8_t* q = work.data_ptr<uint8_t>();
-  const f4::Codes c{q, K / 2, q + code_bytes, M};
   const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(M, w.rows, dev);
-  auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-  if (M > 0) f4::quantize_launch(x.data_ptr(), x.stride(0), M, K, c.q, c.ld, c.sf, st);
-  f4::run_gemm(c, w, K, &out, (int)epi, scale, residual, nullptr,
+  f4::run_gemm(f4::Tokens{f4::Codes{nullptr, 0, nullptr, M}, x.data_ptr(), x.stride(0)}, w, K, &out, (int)epi, scale,
+               residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
                             slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
-               err, dev, M > 0, st);
+               err, dev);
   return out;
 }
 
@@ -1206,9 +1298,8 @@ std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
   f4::make_codes(x.rows, I, dev, a4, sf);
   const f4::Codes o = f4::check_operand("output", a4, sf, I, dev);
   GSB_CHECK(o.rows == x.rows, "mxfp4_gemm_swiglu: output codes must be [M, I / 2]");
-  f4::run_gemm(x, w, K, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &o,
-               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, {}}, err, dev, false,
-               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  f4::run_gemm(f4::Tokens{x, nullptr, 0}, w, K, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &o,
+               f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, {}}, err, dev);
   return {a4, sf};
 }
 

@@ -151,7 +151,7 @@ def test_quantize_past_32_bits():
 
 
 # ------------------------------------------------------------------------------------------- products
-@pytest.mark.parametrize("m", [1, 16, 77, 128, 200, 300, 600])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 16, 77, 128, 200, 300, 600])
 @pytest.mark.parametrize("n,k", [(256, 256), (8, 32), (264, 1056), (1024, 4096), (4096, 288)])
 def test_gemm_store(m, n, k):
     from granite_switch_b200.ops import gemm_fp4 as F
@@ -199,7 +199,7 @@ def _lora_inputs(m, n, slices, na, rank, seed, absent=2):
     return s.to(torch.bfloat16), dirty.to(torch.bfloat16), lb, mask.cuda()
 
 
-@pytest.mark.parametrize("m", [1, 5, 130, 300, 1100])
+@pytest.mark.parametrize("m", [1, 3, 5, 130, 300, 1100])
 @pytest.mark.parametrize("bounds", [[0, 640], [0, 1024, 1280, 1536], [0, 384, 512, 2176]])
 def test_gemm_lora_slices(m, bounds):
     from granite_switch_b200.ops import gemm_fp4 as F
@@ -214,7 +214,7 @@ def test_gemm_lora_slices(m, bounds):
     _check(F.mxfp4_gemm(*a, *b, s=s, **kw), ref, tol)  # without a mask every adapter is expanded
 
 
-@pytest.mark.parametrize("m,i,h", [(1, 64, 64), (17, 192, 512), (130, 1600, 256), (300, 512, 1056), (1300, 4096, 512)])
+@pytest.mark.parametrize("m,i,h", [(1, 64, 64), (2, 1600, 288), (4, 320, 512), (17, 192, 512), (130, 1600, 256), (300, 512, 1056), (1300, 4096, 512)])
 @pytest.mark.parametrize("lora", [False, True])
 def test_gemm_swiglu(m, i, h, lora):
     from granite_switch_b200.models.packing import interleave_gate_up
@@ -282,6 +282,8 @@ def test_nan_and_empty():
     assert out[3].isnan().all()
     rest = torch.arange(20, device="cuda") != 3
     assert out[rest].isfinite().all()
+    few = F.mxfp4_linear(x[2:5], *b)
+    assert few[1].isnan().all() and few[::2].isfinite().all()
     none = torch.empty(0, 512, dtype=torch.bfloat16, device="cuda")
     assert F.mxfp4_linear(none, *b).shape == (0, 256)
     a4, _ = F.mxfp4_gemm_swiglu(*F.rmsnorm_mxfp4(none, torch.ones(512, device="cuda").bfloat16(), 1e-5), *b)
