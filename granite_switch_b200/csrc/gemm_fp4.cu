@@ -48,6 +48,7 @@ constexpr int MAX_KS = 8;      // portable cluster size
 constexpr int W_BYTES = BW * BKB;
 constexpr int SFW_BYTES = 1024;  // the stage's two scale atoms
 constexpr int P_STRIDE = BW;
+constexpr int FRAME_PAD = 12 * 1024;  // around the ring of 32-row tiles: the rest of a 128-row frame
 constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int BAR_BYTES = 256;
 
@@ -61,6 +62,7 @@ struct LoraParams {
 struct SplitParams {
   int M, N, kstages, stages, stage_bytes;
   int mt_rows;        // tokens per tile
+  int tr;             // weight rows per tile: 128, or 32
   int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
   int tmem_cols;
   const uint8_t* sfx;
@@ -128,6 +130,32 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t 
                : "memory");
 }
 
+// One lane of the (converged) warp, always the same one. The issuing warps run their loops whole,
+// so that addresses and descriptors stay in uniform registers, and only the issue is one lane's.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// mbar_wait of a whole warp that also ends when another warp of the CTA gave up.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!__all_sync(0xffffffffu, ok)) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!(ok = mbar_try_wait(bar, parity))) {
+      if (*abort_flag) break;
+      if (globaltimer_ns() - t0 > kWaitBudgetNs) {
+        raise_error(err, kErrGemmWait);
+        *abort_flag = 1;
+        break;
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  }
+  return ok;
+}
+
 template <int OFF>
 __device__ __forceinline__ void st_dsmem_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0+%2], %1;" ::"r"(addr), "f"(v), "n"(OFF));
@@ -179,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                        const __grid_constant__ CUtensorMap tm_lb, const __grid_constant__ CUtensorMap tm_s,
                        const SplitParams p, uint32_t* err) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023) + (p.tr < BW ? FRAME_PAD : 0);
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], tfull_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
@@ -187,7 +215,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = p.ks, stages = p.stages;
   const int part = ks > 1 ? (int)cluster_ctarank() : 0;
-  const int tile = blockIdx.x / ks, n0 = tile * BW;
+  // A tile of 32 rows is one quarter of a 128-row tile: the MMA runs over the whole frame, whose
+  // other rows are whatever lies around the quarter in shared memory, and only its own quarter
+  // of the accumulator's lanes is read. Frame and scales keep their 128-row places.
+  const int tr = p.tr, n0 = (int)(blockIdx.x / ks) * tr, tile = n0 / BW, quarter = (n0 % BW) / 32;
+  const int w_bytes = tr * BKB;
   const int m0 = blockIdx.y * BT, rows = min(p.M - m0, p.mt_rows);  // several token tiles: mt_rows == BT
   const int Mp = (rows + 15) / 16 * 16, xt = (Mp + 127) / 128;
   const int x_bytes = p.mt_rows > 128 ? BT * BKB : (p.mt_rows + 15) / 16 * 16 * BKB;  // stage layout, same in every CTA
@@ -241,83 +273,104 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     // ---------------- producer ----------------
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < total; ++i) {
-        const int s = i % stages;
-        const uint32_t ph = (i / stages) & 1;
-        if (abort_flag || !mbar_wait(&empty_bar[s], ph ^ 1, err, kErrGemmWait)) {
-          abort_flag = 1;
-          break;
+    const bool one = elect_one();
+    const uint32_t stage_tx = w_bytes + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt);
+    const uint8_t* sfw = p.sfw + ((size_t)tile * p.kstages + kb_lo) * 1024;
+    const uint8_t* sfx = p.sfx + ((size_t)(m0 / 128) * p.kstages + kb_lo) * 1024;
+    int issued = 0, slot = 0;
+    uint32_t ph = 1;
+    uint8_t* sw = smem;
+    for (int i = 0; i < total; ++i) {
+      if (!ring_wait(&empty_bar[slot], ph, &abort_flag, err)) break;
+      uint64_t* bar = &full_bar[slot];
+      uint8_t* sx = sw + w_bytes;
+      if (i < n_main) {
+        if (one) {
+          uint8_t* sf = sx + x_bytes;
+          mbar_arrive_expect_tx(bar, stage_tx);
+          tma_load_2d(sw, &tm_w, bar, (kb_lo + i) * BKB, n0);
+          tma_load_2d(sx, &tm_x, bar, (kb_lo + i) * BKB, m0);
+          bulk_load(sf, sfw, 1024, bar);
+          bulk_load(sf + 1024, sfx, 1024, bar);
+          if (xt > 1) bulk_load(sf + 2048, sfx + (size_t)p.kstages * 1024, 1024, bar);
         }
-        uint8_t* sw = smem + s * p.stage_bytes;
-        uint8_t* sx = sw + W_BYTES;
-        uint8_t* sf = sx + x_bytes;
-        if (i < n_main) {
-          const int kb = kb_lo + i;
-          mbar_arrive_expect_tx(&full_bar[s], W_BYTES + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt));
-          tma_load_2d(sw, &tm_w, &full_bar[s], kb * BKB, n0);
-          bulk_load(sf, p.sfw + ((size_t)tile * p.kstages + kb) * 1024, 1024, &full_bar[s]);
-          tma_load_2d(sx, &tm_x, &full_bar[s], kb * BKB, m0);
-          for (int t = 0; t < xt; ++t)
-            bulk_load(sf + 1024 * (1 + t), p.sfx + ((size_t)(m0 / 128 + t) * p.kstages + kb) * 1024, 1024,
-                      &full_bar[s]);
-        } else {
-          int bit;
-          const int col = lora_column(p.lp, amask, part + (i - n_main) * ks, bit);
-          const int s_rows = min((p.mt_rows + 15) / 16 * 16, 128);  // rows of the S box
-          mbar_arrive_expect_tx(&full_bar[s], BW * 64 + xt * s_rows * 64);
-          tma_load_2d(sw, &tm_lb, &full_bar[s], col, n0);
-          // columns of adapters absent from a 128-row tile were never written: such a tile
-          // reads rows past M, which TMA fills with zeros
-          for (int t = 0; t < xt; ++t)
-            tma_load_2d(sx + t * 128 * 64, &tm_s, &full_bar[s], slice_base(p.lp, n0) + col,
-                        (((t ? mask1 : mask0) >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
-        }
-        ++issued;
+        sfw += 1024;
+        sfx += 1024;
+      } else if (one) {
+        int bit;
+        const int col = lora_column(p.lp, amask, part + (i - n_main) * ks, bit);
+        const int s_rows = min((p.mt_rows + 15) / 16 * 16, 128);  // rows of the S box
+        mbar_arrive_expect_tx(bar, tr * 64 + xt * s_rows * 64);
+        tma_load_2d(sw, &tm_lb, bar, col, n0);
+        // columns of adapters absent from a 128-row tile were never written: such a tile
+        // reads rows past M, which TMA fills with zeros
+        for (int t = 0; t < xt; ++t)
+          tma_load_2d(sx + t * 128 * 64, &tm_s, bar, slice_base(p.lp, n0) + col,
+                      (((t ? mask1 : mask0) >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
       }
-      if (abort_flag) {
-        // no copy may still be landing in this CTA's shared memory at exit
-        for (int j = max(0, issued - stages); j < issued; ++j)
-          mbar_wait(&full_bar[j % stages], (j / stages) & 1, err, kErrGemmWait);
+      ++issued;
+      sw += p.stage_bytes;
+      if (++slot == stages) {
+        slot = 0;
+        ph ^= 1;
+        sw = smem;
       }
+    }
+    if (abort_flag) {
+      // no copy may still be landing in this CTA's shared memory at exit
+      for (int j = max(0, issued - stages); j < issued; ++j)
+        mbar_wait(&full_bar[j % stages], (j / stages) & 1, err, kErrGemmWait);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      const uint32_t idesc_bf = umma_idesc_bf16(BW, Mp);
-      bool ok = true;
-      for (int i = 0; i < total; ++i) {
-        const int s = i % stages;
-        if (abort_flag || !mbar_wait(&full_bar[s], (i / stages) & 1, err, kErrGemmWait)) {
-          abort_flag = 1;
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t sw = smem_u32(smem + s * p.stage_bytes), sx = sw + W_BYTES;
+    const bool one = elect_one();
+    const uint32_t idesc_bf = umma_idesc_bf16(BW, Mp), idesc0 = idesc_mxf4(BW, Mp, 0), idesc2 = idesc_mxf4(BW, Mp, 2);
+    const int sf_cols = 8 + 8 * xt;
+    const uint32_t base = smem_u32(smem);
+    int slot = 0;
+    uint32_t ph = 0, sw = base, tw = tmem_base + acc_cols;
+    bool ok = true;
+    for (int i = 0; i < total; ++i) {
+      if (!ring_wait(&full_bar[slot], ph, &abort_flag, err)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sx = sw + w_bytes;
+      if (one) {
         if (i < n_main) {
           // scales: the weights' atoms of both K tiles, then per K tile the tokens' atoms
-          const uint32_t sf = sx + x_bytes, tw = tmem_base + acc_cols + s * (8 + 8 * xt), tx = tw + 8;
+          const uint32_t sf = sx + x_bytes, tx = tw + 8;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             tmem_cp_sf(tw + 4 * h, sf + 512 * h);
-            for (int t = 0; t < xt; ++t) tmem_cp_sf(tx + 4 * (h * xt + t), sf + 1024 * (1 + t) + 512 * h);
+            tmem_cp_sf(tx + 4 * h * xt, sf + 1024 + 512 * h);
+            if (xt > 1) tmem_cp_sf(tx + 4 * h * xt + 4, sf + 2048 + 512 * h);
           }
-          const uint64_t ad = umma_desc_sw128(sw), bd = umma_desc_sw128(sx);
+          const uint64_t ad = umma_desc_sw128(sw - quarter * 32 * 128), bd = umma_desc_sw128(sx);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_mxf4(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(BW, Mp, 2 * (kk & 1)), tw + 4 * (kk >> 1),
+            umma_mxf4(tmem_base, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? idesc2 : idesc0, tw + 4 * (kk >> 1),
                       tx + 4 * xt * (kk >> 1), (i | kk) != 0);
         } else {
-          const uint64_t ad = umma_desc_sw64(sw), bd = umma_desc_sw64(sx);
+          const uint64_t ad = umma_desc_sw64(sw - quarter * 32 * 64), bd = umma_desc_sw64(sx);
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) umma_bf16(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_bf, 1);
         }
-        umma_commit(&empty_bar[s]);
+        umma_commit(&empty_bar[slot]);
       }
-      if (ok) umma_commit(&tfull_bar);
+      __syncwarp();
+      sw += p.stage_bytes;
+      tw += sf_cols;
+      if (++slot == stages) {
+        slot = 0;
+        ph ^= 1;
+        sw = base;
+        tw = tmem_base + acc_cols;
+      }
     }
+    if (ok && one) umma_commit(&tfull_bar);
+    __syncwarp();
   }
 
   // Reduction over the cluster and epilogue. Token m of the tile belongs to CTA m / rows_per;
@@ -332,8 +385,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (ks > 1) cluster_sync();  // every main loop is done: the rings are free
   const int rows_per = p.rows_per;
   float* R = reinterpret_cast<float*>(smem);
-  if (warp >= 2 && ready) {
-    const int q = warp & 3, n = q * 32 + lane;
+  if (warp >= 2 && ready && (tr == BW || (warp & 3) == quarter)) {
+    const int q = warp & 3, n = (tr == BW ? q * 32 : 0) + lane;
     for (int c = 0, owner = 0, oc = 0; c < rows; c += 32) {
       if (c - oc >= rows_per) {
         ++owner;
@@ -357,10 +410,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (ks > 1) cluster_sync();  // every partial row has landed
   if (!abort_flag) {
     const int r0 = part * rows_per, n_rows = max(0, min(rows, r0 + rows_per) - r0);
-    constexpr int GROUPS = (EPI == kEpiSwiGLU) ? 8 : 16;  // 8-column groups per token
-    const int items = n_rows * GROUPS;
+    const int groups_log = EPI == kEpiSwiGLU ? 3 : (tr == BW ? 4 : 2);  // 8-column groups per token
+    const int items = n_rows << groups_log;
     for (int it = threadIdx.x; it < (items + 31) / 32 * 32; it += THREADS) {
-      const int lm = min(it, items - 1) / GROUPS, c = (it % GROUPS) * 8, m = m0 + r0 + lm;
+      const int lm = min(it, items - 1) >> groups_log, c = (it & ((1 << groups_log) - 1)) * 8, m = m0 + r0 + lm;
       float v[8], u[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
@@ -561,34 +614,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 
   if (warp == 0) {
     // ---------------- producer (both CTAs) ----------------
-    if (lane == 0) {
-      const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
-      uint32_t kb = 0;
-      bool stop = false;
-      for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters) {
-        int mt, nt;
-        pair_tile(t, m_tiles, n_tiles, mt, nt);
-        const int own = 2 * mt + (int)rank, m0 = own * 128, n0 = nt * C::BN;
-        uint64_t mask0 = 0ull, mask1 = 0ull;
-        if (p.lora) {
-          mask0 = tile_adapters(p.lp, 2 * mt, mtiles128);
-          mask1 = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
+    const bool one = elect_one();
+    const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
+    uint32_t ph = 1, issued = 0;
+    int slot = 0;
+    bool stop = false;
+    for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters) {
+      int mt, nt;
+      pair_tile(t, m_tiles, n_tiles, mt, nt);
+      const int own = 2 * mt + (int)rank, m0 = own * 128, n0 = nt * C::BN;
+      uint64_t mask0 = 0ull, mask1 = 0ull;
+      if (p.lora) {
+        mask0 = tile_adapters(p.lp, 2 * mt, mtiles128);
+        mask1 = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
+      }
+      const uint64_t both = mask0 | mask1, mine = rank ? mask1 : mask0;
+      const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
+      for (int i = 0; i < total; ++i) {
+        if (!ring_wait(&empty_bar[slot], ph, &abort_flag, err)) {
+          stop = true;
+          break;
         }
-        const uint64_t both = mask0 | mask1, mine = rank ? mask1 : mask0;
-        const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
-        for (int i = 0; i < total; ++i, ++kb) {
-          const int s = kb % C::STAGES;
-          if (abort_flag || !mbar_wait(&empty_bar[s], ((kb / C::STAGES) & 1) ^ 1, err, kErrGemmWait)) {
-            abort_flag = 1;
-            stop = true;
-            break;
-          }
-          uint8_t* sa = smem + s * C::STAGE_BYTES;
-          uint8_t* sb = sa + C::A_BYTES;
-          const uint32_t fb = full_leader + s * 8;
+        uint8_t* sa = smem + slot * C::STAGE_BYTES;
+        uint8_t* sb = sa + C::A_BYTES;
+        const uint32_t fb = full_leader + slot * 8;
+        if (one) {
           if (i < p.kstages) {
             // tiles past the last row are zeros, scales too
-            if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+            if (leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * C::STAGE_BYTES);
             tma_load_2d_pair(sa, &tm_x, fb, i * BKB, m0);
             tma_load_2d_pair(sb, &tm_w, fb, i * BKB, n0 + (int)rank * 128);
             tma_load_3d_pair(sa + C::SFA_OFF, &tm_sfx, fb, 0, i, own);
@@ -598,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             // stages 64 rows of each half of LB. A tile that lacks the adapter reads zeros.
             int bit;
             const int col = lora_column(p.lp, both, i - p.kstages, bit);
-            if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * (2 * 128 * 64 + 128 * 64));
+            if (leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * (2 * 128 * 64 + 128 * 64));
             const int y = ((mine >> bit) & 1ull) ? m0 : mtiles128 * 128;
             tma_load_2d_pair(sa, &tm_s, fb, slice_base(p.lp, n0) + col, y);
             tma_load_2d_pair(sa + 128 * 64, &tm_s, fb, slice_base(p.lp, n0 + 128) + col, y);
@@ -606,16 +659,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             tma_load_2d_pair(sb + 64 * 64, &tm_lb, fb, col, n0 + 128 + (int)rank * 64);
           }
         }
+        __syncwarp();
+        ++issued;
+        if (++slot == C::STAGES) {
+          slot = 0;
+          ph ^= 1;
+        }
       }
-      // the pair MMA has released every stage this CTA filled before the CTA may exit
-      for (uint32_t j = kb > (uint32_t)C::STAGES ? kb - C::STAGES : 0; j < kb && !abort_flag; ++j)
-        if (!mbar_wait(&empty_bar[j % C::STAGES], (j / C::STAGES) & 1, err, kErrGemmWait)) abort_flag = 1;
     }
+    // the pair MMA has released every stage this CTA filled before the CTA may exit
+    for (uint32_t j = issued > (uint32_t)C::STAGES ? issued - C::STAGES : 0; j < issued && !abort_flag; ++j)
+      if (!mbar_wait(&empty_bar[j % C::STAGES], (j / C::STAGES) & 1, err, kErrGemmWait)) abort_flag = 1;
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader only) ----------------
-    if (leader && lane == 0) {
-      uint32_t kb = 0;
-      int ltile = 0;
+    if (leader) {
+      const bool one = elect_one();
+      const uint32_t base = smem_u32(smem);
+      uint32_t ph = 0;
+      int slot = 0, ltile = 0;
       bool stop = false;
       for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters, ++ltile) {
         int mt, nt;
@@ -624,46 +685,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         if (p.lora)
           total += __popcll(tile_adapters(p.lp, 2 * mt, mtiles128) | tile_adapters(p.lp, 2 * mt + 1, mtiles128)) *
                    p.lp.blocks_per_adapter;
-        if (abort_flag || !mbar_wait(&tempty_bar, (ltile & 1) ^ 1, err, kErrGemmWait)) {
-          abort_flag = 1;
-          break;
-        }
+        if (!ring_wait(&tempty_bar, (ltile & 1) ^ 1, &abort_flag, err)) break;
         tc_fence_after();
-        for (int i = 0; i < total; ++i, ++kb) {
-          const int s = kb % C::STAGES;
-          if (abort_flag || !mbar_wait(&full_bar[s], (kb / C::STAGES) & 1, err, kErrGemmWait)) {
-            abort_flag = 1;
+        for (int i = 0; i < total; ++i) {
+          if (!ring_wait(&full_bar[slot], ph, &abort_flag, err)) {
             stop = true;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * C::STAGE_BYTES), sb = sa + C::A_BYTES;
-          if (i < p.kstages) {
-            const uint32_t ta = tmem_base + C::BN + s * C::SF_COLS, tb = ta + 8;
+          const uint32_t sa = base + slot * C::STAGE_BYTES, sb = sa + C::A_BYTES;
+          if (one) {
+            if (i < p.kstages) {
+              const uint32_t ta = tmem_base + C::BN + slot * C::SF_COLS, tb = ta + 8;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tmem_cp_sf_pair(ta + 4 * h, sa + C::SFA_OFF + 512 * h);
-              tmem_cp_sf_pair(tb + 8 * h, sa + C::SFB_OFF + 512 * h);
-              tmem_cp_sf_pair(tb + 8 * h + 4, sa + C::SFB_OFF + 1024 + 512 * h);
+              for (int h = 0; h < 2; ++h) {
+                tmem_cp_sf_pair(ta + 4 * h, sa + C::SFA_OFF + 512 * h);
+                tmem_cp_sf_pair(tb + 8 * h, sa + C::SFB_OFF + 512 * h);
+                tmem_cp_sf_pair(tb + 8 * h + 4, sa + C::SFB_OFF + 1024 + 512 * h);
+              }
+              const uint64_t ad = umma_desc_sw128(sa), bd = umma_desc_sw128(sb);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_mxf4_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(256, C::BN, 2 * (kk & 1)),
+                               ta + 4 * (kk >> 1), tb + 8 * (kk >> 1), (i | kk) != 0);
+            } else {
+              const uint32_t idesc = umma_idesc_bf16(256, 128);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint64_t ad = umma_desc_sw64(sa + u * 128 * 64), bd = umma_desc_sw64(sb + u * 64 * 64);
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) umma_bf16_pair(tmem_base + u * 128, ad + 2 * kk, bd + 2 * kk, idesc, 1);
+              }
             }
-            const uint64_t ad = umma_desc_sw128(sa), bd = umma_desc_sw128(sb);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_mxf4_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(256, C::BN, 2 * (kk & 1)),
-                             ta + 4 * (kk >> 1), tb + 8 * (kk >> 1), (i | kk) != 0);
-          } else {
-            const uint32_t idesc = umma_idesc_bf16(256, 128);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint64_t ad = umma_desc_sw64(sa + u * 128 * 64), bd = umma_desc_sw64(sb + u * 64 * 64);
-#pragma unroll
-              for (int kk = 0; kk < 2; ++kk) umma_bf16_pair(tmem_base + u * 128, ad + 2 * kk, bd + 2 * kk, idesc, 1);
-            }
+            umma_commit_pair(&empty_bar[slot], 0x3);
           }
-          umma_commit_pair(&empty_bar[s], 0x3);
+          __syncwarp();
+          if (++slot == C::STAGES) {
+            slot = 0;
+            ph ^= 1;
+          }
         }
         if (stop) break;
-        umma_commit_pair(&tfull_bar, 0x3);
+        if (one) umma_commit_pair(&tfull_bar, 0x3);
+        __syncwarp();
       }
     }
   } else {
@@ -814,18 +878,21 @@ static int num_sms() {
   return cached[dev];
 }
 
-// Clusters of `ks` CTAs with `smem` bytes each that fit on the GPU at once (clusters lie
+// Clusters of `ks` CTAs that fit on the GPU at once with one or two CTAs per SM (clusters lie
 // inside one GPC, so large ones leave SMs unused). Asked once per device and size.
-static int max_clusters(int ks) {
-  static int cached[kMaxDevices][MAX_KS + 1] = {{0}};
+constexpr int HALF_SMEM = 112 * 1024;
+static int max_clusters(int ks, int per_sm) {
+  static int cached[kMaxDevices][MAX_KS + 1][3] = {{{0}}};
   const int dev = current_device();
-  if (cached[dev][ks]) return cached[dev][ks];
+  if (cached[dev][ks][per_sm]) return cached[dev][ks][per_sm];
+  if (ks == 1) return cached[dev][ks][per_sm] = per_sm * num_sms();
   auto kfn = mxfp4_split_kernel<kEpiStore>;
+  const int smem = per_sm == 2 ? HALF_SMEM - BAR_BYTES : SMEM_LIMIT - BAR_BYTES;
   GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ks * num_sms()), 1, 1);
+  cfg.gridDim = dim3((unsigned)(2 * ks * num_sms()), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = SMEM_LIMIT - BAR_BYTES;
+  cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ks;
@@ -836,40 +903,48 @@ static int max_clusters(int ks) {
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, kfn, &cfg) != cudaSuccess || n <= 0) {
     (void)cudaGetLastError();
-    n = num_sms() / ks;
+    n = per_sm * num_sms() / ks;
   }
-  return cached[dev][ks] = n;
+  return cached[dev][ks][per_sm] = n;
 }
 
 // Smallest M of the pair kernel (gsb_mxfp4_pair_min_m changes it for A/B runs).
 static int g_pair_min_m = 512;
 
 struct SplitPlan {
-  int mt_rows, token_tiles, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes;
+  int mt_rows, token_tiles, tr, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes;
 };
 
-// K parts per tile: the most whose clusters all fit at once, with two stages a part at
-// least. The ring takes what shared memory is left, the reduction buffer reuses it.
-static SplitPlan split_plan(int M, int N, int64_t K) {
+static int env_int(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+
+static SplitPlan split_plan(int M, int N, int64_t K, int epi) {
   SplitPlan s{};
   s.mt_rows = std::min(M, BT);
   s.token_tiles = (M + BT - 1) / BT;
-  s.weight_tiles = (N + BW - 1) / BW;
   const int kstages = (int)((K + 255) / 256);
-  const int tiles = s.token_tiles * s.weight_tiles;
-  s.ks = 1;
-  for (int ks = 2; ks <= MAX_KS; ++ks)
-    if (kstages / ks >= 2 && tiles <= max_clusters(ks)) s.ks = ks;
   const int mp = (s.mt_rows + 15) / 16 * 16, xt = (mp + 127) / 128;
-  s.stage_bytes = W_BYTES + (mp > 128 ? BT : mp) * BKB + SFW_BYTES * (1 + xt);
-  const int room = SMEM_LIMIT - BAR_BYTES - 1024;
+  const int acc = (s.mt_rows + 31) / 32 * 32, sf_cols = 8 + 8 * xt;
+  s.tr = (epi != kEpiSwiGLU && M <= env_int("F4_TR32_M", 64) && (N + 31) / 32 <= env_int("F4_TR32_T", 2 * num_sms())) ? 32 : BW;
+  s.weight_tiles = (N + s.tr - 1) / s.tr;
+  const int tiles = s.token_tiles * s.weight_tiles;
+  s.stage_bytes = s.tr * BKB + (mp > 128 ? BT : mp) * BKB + SFW_BYTES * (1 + xt);
+  const int pad = s.tr < BW ? 2 * FRAME_PAD : 0;
+  for (int per_sm = M <= env_int("F4_TWO_M", 128) ? 2 : 1; per_sm >= 1; --per_sm) {
+    const int room = (per_sm == 2 ? HALF_SMEM : SMEM_LIMIT) - BAR_BYTES - 1024 - pad;
+    s.stages = std::min({MAX_STAGES, room / s.stage_bytes, (512 / per_sm - acc) / sf_cols});
+    if (per_sm == 2 && s.stages < 3) continue;
+    s.ks = 1;
+    for (int ks = 2; ks <= MAX_KS; ++ks)
+      if (kstages / ks >= env_int("F4_MINST", 2) && tiles <= max_clusters(ks, per_sm) &&
+          ks * rows_per_part(s.mt_rows, ks) * P_STRIDE * 4 <= room && ks <= env_int("F4_MAXKS", 8))
+        s.ks = ks;
+    break;
+  }
   const int reduce = s.ks * rows_per_part(s.mt_rows, s.ks) * P_STRIDE * 4;
-  const int acc = (s.mt_rows + 31) / 32 * 32;
-  s.stages = std::min({MAX_STAGES, room / s.stage_bytes, (512 - acc) / (8 + 8 * xt)});
-  const int cols = acc + s.stages * (8 + 8 * xt);
+  const int cols = acc + s.stages * sf_cols;
   s.tmem_cols = 32;
   while (s.tmem_cols < cols) s.tmem_cols *= 2;
-  s.smem_bytes = std::max(s.stages * s.stage_bytes, reduce) + 1024;
+  s.smem_bytes = std::max(s.stages * s.stage_bytes, reduce) + pad + 1024;
   return s;
 }
 
@@ -1205,19 +1280,20 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
     return;
   }
 
-  const SplitPlan s = split_plan(M, N, K);
+  const SplitPlan s = split_plan(M, N, K, epi);
   GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
   p.sfx = x.sf;
   p.sfw = w.sf;
   p.stages = s.stages;
   p.stage_bytes = s.stage_bytes;
   p.mt_rows = s.mt_rows;
+  p.tr = s.tr;
   p.ks = s.ks;
   p.rows_per = rows_per_part(s.mt_rows, s.ks);
   p.tmem_cols = s.tmem_cols;
   const uint32_t mp = (uint32_t)((s.mt_rows + 15) / 16 * 16);
-  const CUtensorMap tw = make_tmap_codes(w, K, BW), tx = make_tmap_codes(x, K, mp);
-  const CUtensorMap tlb = lora ? tmap_lb(BW) : tw, ts = lora ? tmap_s(std::min(mp, 128u)) : tx;
+  const CUtensorMap tw = make_tmap_codes(w, K, s.tr), tx = make_tmap_codes(x, K, mp);
+  const CUtensorMap tlb = lora ? tmap_lb(s.tr) : tw, ts = lora ? tmap_s(std::min(mp, 128u)) : tx;
   switch (epi) {
     case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
     case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
