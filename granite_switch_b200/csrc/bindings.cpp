@@ -70,7 +70,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mxfp4_linear", &gsb_mxfp4_linear, "MXFP4 GEMM of bf16 rows, quantised on the way");
   m.def("mxfp4_gemm_swiglu", &gsb_mxfp4_gemm_swiglu, "MXFP4 gate/up GEMM, SwiGLU and MXFP4 quantisation in the epilogue");
   m.def("mxfp4_pair_min_m", &gsb_mxfp4_pair_min_m,
-        "set the smallest M of the CTA-pair MXFP4 GEMM (negative: only reads; returns the old value)");
+        "force the smallest M of the CTA-pair MXFP4 GEMM, for A/B tests (-1: the rule; returns the old value)");
   m.def("rope_kv_fp8", &gsb_rope_kv_fp8, "RoPE on q / k then the quantised fp8 K / V write, one launch");
   m.def("kv_write_fp8", &gsb_kv_write_fp8, "quantised (e4m3, per-row scale) write of a step's K/V into the fp8 cache");
 }

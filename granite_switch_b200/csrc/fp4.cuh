@@ -71,6 +71,34 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   return max(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
+__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
+  const uint32_t p[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack_bf16x2(p[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+
+// fp32 bits of the largest magnitude of eight packed bf16 values (as 16-bit integers, so a
+// NaN is above infinity).
+__device__ __forceinline__ uint32_t max_abs_bits_bf16(const uint4& q) {
+  const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu),
+                              __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+  return max(m << 16, m & 0xffff0000u);
+}
+
+// Eight bf16 values a lane, four lanes a block -> the block's scale byte and the lane's codes.
+__device__ __forceinline__ uint32_t quantise8(const uint4& q, uint32_t& codes) {
+  const uint32_t byte = scale_byte(quad_max(max_abs_bits_bf16(q)));
+  float v[8];
+  unpack8(q, v);
+  codes = pack8(v, inv_scale(byte));
+  if (byte == 255u) codes = 0u;
+  return byte;
+}
+
 // Offset of the 4-byte word with the scales of row `row`, K tile `kt` (128 values).
 __device__ __forceinline__ int64_t sf_word(int64_t row, int64_t kt, int64_t ktiles) {
   const int r = (int)(row & 127);

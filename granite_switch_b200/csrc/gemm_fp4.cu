@@ -40,15 +40,15 @@ namespace gsb {
 namespace f4 {
 
 constexpr int BW = 128;        // weight rows per tile (the MMA's M)
-constexpr int BT = 256;        // tokens per tile (the MMA's N), at most
+constexpr int BT = 128;        // tokens per tile (the MMA's N), at most
 constexpr int BKB = 128;       // bytes of K per stage: 256 elements
 constexpr int THREADS = 192;
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_KS = 8;      // portable cluster size
 constexpr int W_BYTES = BW * BKB;
-constexpr int SFW_BYTES = 1024;  // the stage's two scale atoms
+constexpr int SF_BYTES = 1024;  // a stage's two scale atoms
+constexpr int SF_COLS = 16;     // tensor memory columns of a stage's scales: weights 8, tokens 8
 constexpr int P_STRIDE = BW;
-constexpr int FRAME_PAD = 12 * 1024;  // around the ring of 32-row tiles: the rest of a 128-row frame
 constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int BAR_BYTES = 256;
 
@@ -62,9 +62,9 @@ struct LoraParams {
 struct SplitParams {
   int M, N, kstages, stages, stage_bytes;
   int mt_rows;        // tokens per tile
-  int tr;             // weight rows per tile: 128, or 32
   int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
   int tmem_cols;
+  int reduce_off;     // offset of the reduction buffer: 0 (over the ring) or behind it
   const uint8_t* sfx;
   const uint8_t* sfw;
   float scale;
@@ -79,9 +79,9 @@ struct SplitParams {
   LoraParams lp;
 };
 
-// Tokens per CTA of a cluster in the reduction: a multiple of 32, so that a 32-column
+// Tokens per CTA of a cluster in the reduction: a multiple of 16, so that a 16-column
 // chunk of the accumulator belongs to one CTA.
-__host__ __device__ constexpr int rows_per_part(int rows, int ks) { return ((rows + ks - 1) / ks + 31) / 32 * 32; }
+__host__ __device__ constexpr int rows_per_part(int rows, int ks) { return ((rows + ks - 1) / ks + 15) / 16 * 16; }
 
 // Instruction descriptor, kind::mxf4 with block scaling: e2m1 A and B, K-major, fp32
 // accumulator, UE8M0 scales; sf_id (0 or 2) picks the byte pair of the 32-bit scale words.
@@ -138,6 +138,10 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// The two halves of cluster_sync().
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // mbar_wait of a whole warp that also ends when another warp of the CTA gave up.
 __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
   bool ok = mbar_try_wait(bar, parity);
@@ -161,7 +165,7 @@ __device__ __forceinline__ void st_dsmem_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0+%2], %1;" ::"r"(addr), "f"(v), "n"(OFF));
 }
 template <int... J>
-__device__ __forceinline__ void push_rows32(uint32_t addr, const uint32_t (&r)[32], std::integer_sequence<int, J...>) {
+__device__ __forceinline__ void push_rows16(uint32_t addr, const uint32_t (&r)[16], std::integer_sequence<int, J...>) {
   (st_dsmem_f32<J * P_STRIDE * 4>(addr, __uint_as_float(r[J])), ...);
 }
 
@@ -193,21 +197,13 @@ __device__ __forceinline__ int lora_column(const LoraParams& l, uint64_t mask, i
 
 __device__ __forceinline__ float swiglu_f(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-}  // namespace f4
-}  // namespace gsb
-
-#include "gemv_fp4.cuh"
-
-namespace gsb {
-namespace f4 {
-
 template <int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
     mxfp4_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                        const __grid_constant__ CUtensorMap tm_lb, const __grid_constant__ CUtensorMap tm_s,
                        const SplitParams p, uint32_t* err) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023) + (p.tr < BW ? FRAME_PAD : 0);
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], tfull_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
@@ -215,14 +211,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = p.ks, stages = p.stages;
   const int part = ks > 1 ? (int)cluster_ctarank() : 0;
-  // A tile of 32 rows is one quarter of a 128-row tile: the MMA runs over the whole frame, whose
-  // other rows are whatever lies around the quarter in shared memory, and only its own quarter
-  // of the accumulator's lanes is read. Frame and scales keep their 128-row places.
-  const int tr = p.tr, n0 = (int)(blockIdx.x / ks) * tr, tile = n0 / BW, quarter = (n0 % BW) / 32;
-  const int w_bytes = tr * BKB;
-  const int m0 = blockIdx.y * BT, rows = min(p.M - m0, p.mt_rows);  // several token tiles: mt_rows == BT
-  const int Mp = (rows + 15) / 16 * 16, xt = (Mp + 127) / 128;
-  const int x_bytes = p.mt_rows > 128 ? BT * BKB : (p.mt_rows + 15) / 16 * 16 * BKB;  // stage layout, same in every CTA
+  const int tile = blockIdx.x / ks, n0 = tile * BW;
+  const int m0 = blockIdx.y * p.mt_rows, rows = min(p.M - m0, p.mt_rows);  // several token tiles: 64 or 128 rows each
+  const int Mp = (rows + 15) / 16 * 16, x_bytes = (p.mt_rows + 15) / 16 * 16 * BKB;
   const int mtiles128 = (p.M + 127) / 128;
   const int kb_lo = (int)((int64_t)part * p.kstages / ks), kb_hi = (int)((int64_t)(part + 1) * p.kstages / ks);
   const int n_main = kb_hi - kb_lo;
@@ -252,6 +243,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  // a reduction buffer of its own may be written once its CTA runs
+  if (ks > 1 && p.reduce_off) cluster_arrive();
   griddep_launch();
 
   // The first stages' weights start towards L2 before the wait for the kernel before this
@@ -260,21 +253,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < min(stages, n_main); ++i) tma_prefetch_2d(&tm_w, (kb_lo + i) * BKB, n0);
   griddep_wait();
 
-  uint64_t mask0 = 0ull, mask1 = 0ull;  // adapters of the token tile's two 128-row halves
-  if (p.lora) {
-    mask0 = tile_adapters(p.lp, m0 / 128, mtiles128);
-    if (xt > 1) mask1 = tile_adapters(p.lp, m0 / 128 + 1, mtiles128);
-  }
-  const uint64_t amask = mask0 | mask1;
+  // adapters of the 128-row tile that holds the token tile
+  const uint64_t amask = p.lora ? tile_adapters(p.lp, m0 / 128, mtiles128) : 0ull;
   const int n_lora_all = __popcll(amask) * p.lp.blocks_per_adapter;
   const int n_lora = n_lora_all > part ? (n_lora_all - part + ks - 1) / ks : 0;
   const int total = n_main + n_lora;
-  const int acc_cols = (p.mt_rows + 31) / 32 * 32;  // accumulator, then the ring of scales: 8 + 8 xt columns a stage
+  const int acc_cols = (p.mt_rows + 31) / 32 * 32;  // accumulator, then the ring of scales: SF_COLS columns a stage
 
   if (warp == 0) {
     // ---------------- producer ----------------
     const bool one = elect_one();
-    const uint32_t stage_tx = w_bytes + (p.mt_rows + 15) / 16 * 16 * BKB + SFW_BYTES * (1 + xt);
+    const uint32_t stage_tx = W_BYTES + x_bytes + 2 * SF_BYTES;
     const uint8_t* sfw = p.sfw + ((size_t)tile * p.kstages + kb_lo) * 1024;
     const uint8_t* sfx = p.sfx + ((size_t)(m0 / 128) * p.kstages + kb_lo) * 1024;
     int issued = 0, slot = 0;
@@ -283,30 +272,24 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < total; ++i) {
       if (!ring_wait(&empty_bar[slot], ph, &abort_flag, err)) break;
       uint64_t* bar = &full_bar[slot];
-      uint8_t* sx = sw + w_bytes;
+      uint8_t* sx = sw + W_BYTES;
       if (i < n_main) {
         if (one) {
           uint8_t* sf = sx + x_bytes;
           mbar_arrive_expect_tx(bar, stage_tx);
           tma_load_2d(sw, &tm_w, bar, (kb_lo + i) * BKB, n0);
-          tma_load_2d(sx, &tm_x, bar, (kb_lo + i) * BKB, m0);
           bulk_load(sf, sfw, 1024, bar);
+          tma_load_2d(sx, &tm_x, bar, (kb_lo + i) * BKB, m0);
           bulk_load(sf + 1024, sfx, 1024, bar);
-          if (xt > 1) bulk_load(sf + 2048, sfx + (size_t)p.kstages * 1024, 1024, bar);
         }
         sfw += 1024;
         sfx += 1024;
       } else if (one) {
         int bit;
         const int col = lora_column(p.lp, amask, part + (i - n_main) * ks, bit);
-        const int s_rows = min((p.mt_rows + 15) / 16 * 16, 128);  // rows of the S box
-        mbar_arrive_expect_tx(bar, tr * 64 + xt * s_rows * 64);
+        mbar_arrive_expect_tx(bar, BW * 64 + x_bytes / 2);
         tma_load_2d(sw, &tm_lb, bar, col, n0);
-        // columns of adapters absent from a 128-row tile were never written: such a tile
-        // reads rows past M, which TMA fills with zeros
-        for (int t = 0; t < xt; ++t)
-          tma_load_2d(sx + t * 128 * 64, &tm_s, bar, slice_base(p.lp, n0) + col,
-                      (((t ? mask1 : mask0) >> bit) & 1ull) ? m0 + t * 128 : mtiles128 * 128);
+        tma_load_2d(sx, &tm_s, bar, slice_base(p.lp, n0) + col, m0);
       }
       ++issued;
       sw += p.stage_bytes;
@@ -325,8 +308,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------- MMA issuer ----------------
     const bool one = elect_one();
     const uint32_t idesc_bf = umma_idesc_bf16(BW, Mp), idesc0 = idesc_mxf4(BW, Mp, 0), idesc2 = idesc_mxf4(BW, Mp, 2);
-    const int sf_cols = 8 + 8 * xt;
     const uint32_t base = smem_u32(smem);
+    const int x_col = (m0 & 64) / 32;  // the second 64 rows' scales are the atom's columns 2 and 3
     int slot = 0;
     uint32_t ph = 0, sw = base, tw = tmem_base + acc_cols;
     bool ok = true;
@@ -336,24 +319,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t sx = sw + w_bytes;
+      const uint32_t sx = sw + W_BYTES;
       if (one) {
         if (i < n_main) {
-          // scales: the weights' atoms of both K tiles, then per K tile the tokens' atoms
+          // scales: the weights' atoms of both K tiles, then the tokens'
           const uint32_t sf = sx + x_bytes, tx = tw + 8;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             tmem_cp_sf(tw + 4 * h, sf + 512 * h);
-            tmem_cp_sf(tx + 4 * h * xt, sf + 1024 + 512 * h);
-            if (xt > 1) tmem_cp_sf(tx + 4 * h * xt + 4, sf + 2048 + 512 * h);
+            tmem_cp_sf(tx + 4 * h, sf + 1024 + 512 * h);
           }
-          const uint64_t ad = umma_desc_sw128(sw - quarter * 32 * 128), bd = umma_desc_sw128(sx);
+          const uint64_t ad = umma_desc_sw128(sw), bd = umma_desc_sw128(sx);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_mxf4(tmem_base, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? idesc2 : idesc0, tw + 4 * (kk >> 1),
-                      tx + 4 * xt * (kk >> 1), (i | kk) != 0);
+                      tx + x_col + 4 * (kk >> 1), (i | kk) != 0);
         } else {
-          const uint64_t ad = umma_desc_sw64(sw - quarter * 32 * 64), bd = umma_desc_sw64(sx);
+          const uint64_t ad = umma_desc_sw64(sw), bd = umma_desc_sw64(sx);
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) umma_bf16(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_bf, 1);
         }
@@ -361,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
       sw += p.stage_bytes;
-      tw += sf_cols;
+      tw += SF_COLS;
       if (++slot == stages) {
         slot = 0;
         ph ^= 1;
@@ -381,28 +363,35 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (!ready) abort_flag = 1;
     else tc_fence_after();
   }
-  __syncthreads();
-  if (ks > 1) cluster_sync();  // every main loop is done: the rings are free
+  if (ks > 1) {
+    if (!p.reduce_off) {  // over the ring: every main loop of the cluster has to be done
+      __syncthreads();
+      cluster_arrive();
+    }
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   const int rows_per = p.rows_per;
-  float* R = reinterpret_cast<float*>(smem);
-  if (warp >= 2 && ready && (tr == BW || (warp & 3) == quarter)) {
-    const int q = warp & 3, n = (tr == BW ? q * 32 : 0) + lane;
-    for (int c = 0, owner = 0, oc = 0; c < rows; c += 32) {
+  float* R = reinterpret_cast<float*>(smem + p.reduce_off);
+  if (warp >= 2 && ready) {
+    const int q = warp & 3, n = q * 32 + lane;
+    for (int c = 0, owner = 0, oc = 0; c < rows; c += 16) {
       if (c - oc >= rows_per) {
         ++owner;
         oc += rows_per;
       }
-      uint32_t r[32];
-      tmem_ld32(tmem_base + c + ((uint32_t)(q * 32) << 16), r);
+      uint32_t r[16];
+      tmem_ld16(tmem_base + c + ((uint32_t)(q * 32) << 16), r);
       tmem_wait_ld();
       const int row = part * rows_per + c - oc;
       if (ks > 1) {
-        push_rows32(mapa_shared(smem_u32(R + row * P_STRIDE + n), (uint32_t)owner), r,
-                    std::make_integer_sequence<int, 32>{});
+        push_rows16(mapa_shared(smem_u32(R + row * P_STRIDE + n), (uint32_t)owner), r,
+                    std::make_integer_sequence<int, 16>{});
       } else {
         float* dst = R + row * P_STRIDE + n;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) dst[j * P_STRIDE] = __uint_as_float(r[j]);
+        for (int j = 0; j < 16; ++j) dst[j * P_STRIDE] = __uint_as_float(r[j]);
       }
     }
   }
@@ -410,10 +399,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (ks > 1) cluster_sync();  // every partial row has landed
   if (!abort_flag) {
     const int r0 = part * rows_per, n_rows = max(0, min(rows, r0 + rows_per) - r0);
-    const int groups_log = EPI == kEpiSwiGLU ? 3 : (tr == BW ? 4 : 2);  // 8-column groups per token
-    const int items = n_rows << groups_log;
+    constexpr int GROUPS = (EPI == kEpiSwiGLU) ? 8 : 16;  // 8-column groups per token
+    const int items = n_rows * GROUPS;
     for (int it = threadIdx.x; it < (items + 31) / 32 * 32; it += THREADS) {
-      const int lm = min(it, items - 1) >> groups_log, c = (it & ((1 << groups_log) - 1)) * 8, m = m0 + r0 + lm;
+      const int lm = min(it, items - 1) / GROUPS, c = (it % GROUPS) * 8, m = m0 + r0 + lm;
       float v[8], u[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
@@ -861,7 +850,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 
 // ---------------------------------------------------------------------------- host
 constexpr int kMaxDevices = 64;
-constexpr int GV_MAX_SMEM = 200 * 1024;
 
 static int current_device() {
   int dev = 0;
@@ -908,43 +896,54 @@ static int max_clusters(int ks, int per_sm) {
   return cached[dev][ks][per_sm] = n;
 }
 
-// Smallest M of the pair kernel (gsb_mxfp4_pair_min_m changes it for A/B runs).
-static int g_pair_min_m = 512;
+// Which kernel takes a call. The pair kernel needs about 48 tiles of 256 x 256 to be ahead
+// (measured, us pair / split: 256 x 4096 x 4096 11.5 / 9.7, 512: 11.7 / 11.3, 768: 11.8 / 13; 256 x
+// 25600 x 4096 20.9 / 26.9); one token tile of 128 is always the split kernel's.
+// gsb_mxfp4_pair_min_m forces a smallest M instead, for A/B runs.
+static int g_pair_min_m = -1;
+static bool use_pair(int M, int N) {
+  if (g_pair_min_m >= 0) return M >= g_pair_min_m;
+  return M > BT && (M + 255) / 256 * ((N + 255) / 256) >= 48;
+}
 
 struct SplitPlan {
-  int mt_rows, token_tiles, tr, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes;
+  int mt_rows, token_tiles, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes, reduce_off;
 };
 
-static int env_int(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-
-static SplitPlan split_plan(int M, int N, int64_t K, int epi) {
+// Token tiles of 128 or, where they still run in one wave of two CTAs per SM over a short K, of
+// 64 (256 tokens x 2048 x 2048 8.2 -> 6.5 us; over K = 12800 they cost 20.5 against 15.6 us). Two CTAs
+// per SM hide one another's barriers and latencies, but leave less for each one's ring: for
+// 128-row tiles only when there are more tiles than SMs. K parts: as many as run in one wave,
+// two stages each at least (measured from 1 to 8 at 18 sizes, this takes the fastest).
+static SplitPlan split_plan(int M, int N, int64_t K) {
   SplitPlan s{};
-  s.mt_rows = std::min(M, BT);
-  s.token_tiles = (M + BT - 1) / BT;
   const int kstages = (int)((K + 255) / 256);
-  const int mp = (s.mt_rows + 15) / 16 * 16, xt = (mp + 127) / 128;
-  const int acc = (s.mt_rows + 31) / 32 * 32, sf_cols = 8 + 8 * xt;
-  s.tr = (epi != kEpiSwiGLU && M <= env_int("F4_TR32_M", 64) && (N + 31) / 32 <= env_int("F4_TR32_T", 2 * num_sms())) ? 32 : BW;
-  s.weight_tiles = (N + s.tr - 1) / s.tr;
-  const int tiles = s.token_tiles * s.weight_tiles;
-  s.stage_bytes = s.tr * BKB + (mp > 128 ? BT : mp) * BKB + SFW_BYTES * (1 + xt);
-  const int pad = s.tr < BW ? 2 * FRAME_PAD : 0;
-  for (int per_sm = M <= env_int("F4_TWO_M", 128) ? 2 : 1; per_sm >= 1; --per_sm) {
-    const int room = (per_sm == 2 ? HALF_SMEM : SMEM_LIMIT) - BAR_BYTES - 1024 - pad;
-    s.stages = std::min({MAX_STAGES, room / s.stage_bytes, (512 / per_sm - acc) / sf_cols});
+  s.weight_tiles = (N + BW - 1) / BW;
+  const bool narrow = kstages <= 16 && (M + 63) / 64 * s.weight_tiles <= 2 * num_sms();
+  s.mt_rows = std::min(M, narrow ? 64 : BT);
+  s.token_tiles = (M + s.mt_rows - 1) / s.mt_rows;
+  const int tiles = s.token_tiles * s.weight_tiles, acc = (s.mt_rows + 31) / 32 * 32;
+  s.stage_bytes = W_BYTES + (s.mt_rows + 15) / 16 * 16 * BKB + 2 * SF_BYTES;
+  auto reduce = [&](int ks) { return ks * rows_per_part(s.mt_rows, ks) * P_STRIDE * 4; };
+  for (int per_sm = s.mt_rows <= 64 || tiles > num_sms() ? 2 : 1; per_sm >= 1; --per_sm) {
+    const int room = (per_sm == 2 ? HALF_SMEM : SMEM_LIMIT) - BAR_BYTES - 1024;
+    s.stages = std::min({MAX_STAGES, room / s.stage_bytes, (512 / per_sm - acc) / SF_COLS});
     if (per_sm == 2 && s.stages < 3) continue;
     s.ks = 1;
     for (int ks = 2; ks <= MAX_KS; ++ks)
-      if (kstages / ks >= env_int("F4_MINST", 2) && tiles <= max_clusters(ks, per_sm) &&
-          ks * rows_per_part(s.mt_rows, ks) * P_STRIDE * 4 <= room && ks <= env_int("F4_MAXKS", 8))
-        s.ks = ks;
+      if (kstages / ks >= 2 && tiles <= max_clusters(ks, per_sm) && reduce(ks) <= room) s.ks = ks;
+    // a reduction buffer of its own saves a cluster barrier, if three stages are left
+    const int apart = (room - reduce(s.ks)) / s.stage_bytes;
+    if (s.ks > 1 && apart >= 3) {
+      s.stages = std::min(s.stages, apart);
+      s.reduce_off = s.stages * s.stage_bytes;
+    }
+    s.smem_bytes = (s.reduce_off ? s.reduce_off + reduce(s.ks) : std::max(s.stages * s.stage_bytes, reduce(s.ks))) + 1024;
     break;
   }
-  const int reduce = s.ks * rows_per_part(s.mt_rows, s.ks) * P_STRIDE * 4;
-  const int cols = acc + s.stages * sf_cols;
+  const int cols = acc + s.stages * SF_COLS;
   s.tmem_cols = 32;
   while (s.tmem_cols < cols) s.tmem_cols *= 2;
-  s.smem_bytes = std::max(s.stages * s.stage_bytes, reduce) + pad + 1024;
   return s;
 }
 
@@ -1067,45 +1066,6 @@ static CUtensorMap make_tmap_sf(const Codes& c, int64_t kstages, uint32_t tiles_
   return m;
 }
 
-// Two CTAs per SM where a step of both fits beside their tokens, else one; as many steps in
-// flight as fit and the CTA has. 0 stages: the kernel does not take the call.
-struct GemvPlan {
-  int per_sm, stages, smem;
-};
-static GemvPlan gemv_plan(int MT, int kblocks, int units, int steps) {
-  const int stage = gemv_stage(kblocks), tokens = gemv_tokens(MT, kblocks);
-  for (int per_sm = 2; per_sm >= 1; --per_sm) {
-    const int room = (per_sm == 2 ? 110 * 1024 : GV_MAX_SMEM) - tokens;
-    if (room < stage) continue;
-    const int ctas = per_sm * num_sms(), have = (units + ctas - 1) / ctas * steps;
-    const int stages = std::min({GV_MAX_STAGES, room / stage, have});
-    return {per_sm, stages, stages * stage + tokens};
-  }
-  return {0, 0, 0};
-}
-
-template <int MT, int EPI>
-static void launch_gemv(GemvParams p, const LoraParams& lp, bool dependent, uint32_t* err, cudaStream_t st) {
-  auto kfn = mxfp4_gemv_kernel<MT, EPI>;
-  static bool set[kMaxDevices] = {false};
-  const int dev = current_device();
-  if (!set[dev]) {
-    GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, GV_MAX_SMEM));
-    set[dev] = true;
-  }
-  const int units = EPI == kEpiSwiGLU ? p.N / 64 : (p.N + GV_STEP - 1) / GV_STEP;
-  const GemvPlan g = gemv_plan(MT, p.kblocks, units, EPI == kEpiSwiGLU ? 64 / GV_STEP : 1);
-  p.stages = g.stages;
-  launch(kfn, dim3((unsigned)std::min(units, g.per_sm * num_sms())), GV_THREADS, g.smem, 1, dependent, st, p, lp, err);
-}
-
-template <int EPI>
-static void gemv_by_rows(const GemvParams& p, const LoraParams& lp, bool dependent, uint32_t* err, cudaStream_t st) {
-  if (p.M == 1) launch_gemv<1, EPI>(p, lp, dependent, err, st);
-  else if (p.M == 2) launch_gemv<2, EPI>(p, lp, dependent, err, st);
-  else launch_gemv<4, EPI>(p, lp, dependent, err, st);
-}
-
 static CUtensorMap make_tmap_codes(const Codes& c, int64_t K, uint32_t box_rows) {
   return make_tmap_2d(c.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)c.rows, (uint64_t)K / 2, (uint64_t)c.ld, BKB,
                       box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -1198,41 +1158,6 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());
   bool dependent = pdl_enabled();
 
-  if (M <= GV_MAX_M && gemv_stage((int)(K / 32)) + gemv_tokens(GV_MAX_M, (int)(K / 32)) <= GV_MAX_SMEM) {
-    GemvParams g{};
-    g.M = M;
-    g.N = N;
-    g.kblocks = (int)(K / 32);
-    g.x = reinterpret_cast<const __nv_bfloat16*>(t.bf);
-    g.ldx = t.ldbf;
-    g.x4 = x.q;
-    g.ld4 = x.ld;
-    g.sfx = x.sf;
-    g.w4 = w.q;
-    g.ldw = w.ld;
-    g.sfw = w.sf;
-    g.scale = p.scale;
-    g.out = reinterpret_cast<__nv_bfloat16*>(p.out);
-    g.ldo = p.ldo;
-    g.residual = p.residual;
-    g.ldr = p.ldr;
-    g.a4 = p.a4;
-    g.lda4 = p.lda4;
-    g.sfa_out = p.sfa_out;
-    g.lora = p.lora;
-    if (lora) {
-      g.s = reinterpret_cast<const __nv_bfloat16*>(la.s->data_ptr());
-      g.lds = la.s->stride(0);
-      g.lb = reinterpret_cast<const __nv_bfloat16*>(la.lb->data_ptr());
-      g.ldlb = la.lb->stride(0);
-    }
-    switch (epi) {
-      case kEpiStore: gemv_by_rows<kEpiStore>(g, p.lp, dependent, ep, st); break;
-      case kEpiResAdd: gemv_by_rows<kEpiResAdd>(g, p.lp, dependent, ep, st); break;
-      default: gemv_by_rows<kEpiSwiGLU>(g, p.lp, dependent, ep, st); break;
-    }
-    return;
-  }
   at::Tensor work;  // codes and scales of bf16 rows; the stream orders its reuse
   if (t.bf != nullptr) {
     const int64_t code_bytes = (M * (K / 2) + 1023) / 1024 * 1024;
@@ -1250,7 +1175,7 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
                              rows, CU_TENSOR_MAP_SWIZZLE_64B);
   };
 
-  if (M >= g_pair_min_m) {
+  if (use_pair(M, N)) {
     PairParams pp{};
     pp.M = M;
     pp.N = N;
@@ -1280,20 +1205,20 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
     return;
   }
 
-  const SplitPlan s = split_plan(M, N, K, epi);
+  const SplitPlan s = split_plan(M, N, K);
   GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
+  p.reduce_off = s.reduce_off;
   p.sfx = x.sf;
   p.sfw = w.sf;
   p.stages = s.stages;
   p.stage_bytes = s.stage_bytes;
   p.mt_rows = s.mt_rows;
-  p.tr = s.tr;
   p.ks = s.ks;
   p.rows_per = rows_per_part(s.mt_rows, s.ks);
   p.tmem_cols = s.tmem_cols;
   const uint32_t mp = (uint32_t)((s.mt_rows + 15) / 16 * 16);
-  const CUtensorMap tw = make_tmap_codes(w, K, s.tr), tx = make_tmap_codes(x, K, mp);
-  const CUtensorMap tlb = lora ? tmap_lb(s.tr) : tw, ts = lora ? tmap_s(std::min(mp, 128u)) : tx;
+  const CUtensorMap tw = make_tmap_codes(w, K, BW), tx = make_tmap_codes(x, K, mp);
+  const CUtensorMap tlb = lora ? tmap_lb(BW) : tw, ts = lora ? tmap_s(mp) : tx;
   switch (epi) {
     case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
     case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
@@ -1379,9 +1304,9 @@ std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
   return {a4, sf};
 }
 
-// Sets the smallest M that takes the pair kernel; returns the previous value (negative: only reads).
+// Forces the smallest M that takes the pair kernel (-1: the measured rule); returns the previous value.
 int64_t gsb_mxfp4_pair_min_m(int64_t m) {
   const int64_t old = f4::g_pair_min_m;
-  if (m >= 0) f4::g_pair_min_m = (int)std::min<int64_t>(m, 1 << 30);
+  f4::g_pair_min_m = (int)std::max<int64_t>(-1, std::min<int64_t>(m, 1 << 30));
   return old;
 }

@@ -27,24 +27,6 @@ namespace f4 {
 constexpr int kQuantThreads = 256;
 constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 
-__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
-  const uint32_t p[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = unpack_bf16x2(p[j]);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
-  }
-}
-
-// fp32 bits of the largest magnitude of eight packed bf16 values (as 16-bit integers, so a
-// NaN is above infinity).
-__device__ __forceinline__ uint32_t max_abs_bits_bf16(const uint4& q) {
-  const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu),
-                              __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
-  return max(m << 16, m & 0xffff0000u);
-}
-
 // Warp `blockIdx.x * 8 + ..` takes `kUnits` units of one row; `per_row` warps make a row.
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int K, int k2s, uint32_t per_row,
@@ -70,11 +52,9 @@ __global__ void __launch_bounds__(kQuantThreads)
   for (int u = 0; u < kUnits; ++u) {
     const int k2 = first + u, k = k2 * 256 + lane * 8;
     if (k2 >= k2s) break;  // the whole warp
-    const uint32_t byte = scale_byte(quad_max(max_abs_bits_bf16(q[u])));
-    float v[8];
-    unpack8(q[u], v);
-    const uint32_t codes = pack8(v, inv_scale(byte));
-    if (k < K) *reinterpret_cast<uint32_t*>(xo + k2 * 128) = byte == 255u ? 0u : codes;
+    uint32_t codes;
+    const uint32_t byte = quantise8(q[u], codes);
+    if (k < K) *reinterpret_cast<uint32_t*>(xo + k2 * 128) = codes;
     store_scales256(byte, lane, so + u * 1024);
   }
 }

@@ -214,6 +214,24 @@ def test_gemm_lora_slices(m, bounds):
     _check(F.mxfp4_gemm(*a, *b, s=s, **kw), ref, tol)  # without a mask every adapter is expanded
 
 
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 64, 300])
+@pytest.mark.parametrize("n,k", [(256, 32), (264, 288), (4096, 2080), (1024, 12800)])
+def test_linear_is_quantise_then_gemm(m, n, k):
+    """Bit for bit, whether the rows are quantised in a kernel of their own or on the way; strided rows."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    wide = torch.full((m, k + 64), 3.0, device="cuda", dtype=torch.bfloat16)
+    wide[:, :k] = _rows(m, k, seed=m)
+    x = wide[:, :k]
+    b = F.quantize_rows_mxfp4(_rows(n, k, seed=2, spread=2))
+    s, dirty, lb, mask = _lora_inputs(m, n // 128 * 128 or n, 1, 3, 32, seed=4)
+    want = F.mxfp4_gemm(*F.quantize_rows_mxfp4(x), *b)
+    assert torch.equal(F.mxfp4_linear(x, *b), want)
+    if n % 128 == 0:
+        kw = dict(s=dirty, lb=lb, rank=32, num_adapters=3, tile_mask=mask, residual=want, epi=F.EPI_RESADD, scale=0.5)
+        assert torch.equal(F.mxfp4_linear(x, *b, **kw), F.mxfp4_gemm(*F.quantize_rows_mxfp4(x), *b, **kw))
+
+
 @pytest.mark.parametrize("m,i,h", [(1, 64, 64), (2, 1600, 288), (4, 320, 512), (17, 192, 512), (130, 1600, 256), (300, 512, 1056), (1300, 4096, 512)])
 @pytest.mark.parametrize("lora", [False, True])
 def test_gemm_swiglu(m, i, h, lora):
