@@ -184,16 +184,31 @@ __device__ __forceinline__ int slice_base(const LoraParams& l, int row) {
   return sl * l.num_adapters * l.rank_blocks * 32;
 }
 
-// Column of S (from the slice's first) and of LB of LoRA block j of the adapters in `mask`:
-// adapter by adapter, its rank blocks one after the other. For swiglu each adapter has the
-// gate's blocks, then the up's, whose columns start num_adapters * rank later.
-__device__ __forceinline__ int lora_column(const LoraParams& l, uint64_t mask, int j, int& bit) {
-  const int ai = j / l.blocks_per_adapter, b = j % l.blocks_per_adapter;
-  for (int t = 0; t < ai; ++t) mask &= mask - 1;
-  bit = __ffsll((long long)mask) - 1;
-  return bit * l.rank_blocks * 32 + (b / l.rank_blocks) * l.num_adapters * l.rank_blocks * 32 +
-         (b % l.rank_blocks) * 32;
-}
+// The LoRA blocks (32 columns of S and LB) of the adapters in a mask, one after the other: adapter
+// by adapter its rank blocks; for swiglu each adapter has the gate's blocks, then the up's, whose
+// columns start num_adapters * rank later. Advanced by the whole warp, block by block.
+struct LoraWalk {
+  uint64_t rem;  // adapters left, the current one lowest
+  int bit, block;
+
+  __device__ __forceinline__ void start(uint64_t mask) {
+    rem = mask;
+    bit = __ffsll((long long)mask) - 1;
+    block = 0;
+  }
+  // Column from the slice's first.
+  __device__ __forceinline__ int column(const LoraParams& l) const {
+    const int rank = l.rank_blocks * 32;
+    return bit * rank + (block >= l.rank_blocks ? l.num_adapters * rank - rank : 0) + block * 32;
+  }
+  __device__ __forceinline__ void next(const LoraParams& l) {
+    if (++block == l.blocks_per_adapter) {
+      block = 0;
+      rem &= rem - 1;
+      bit = __ffsll((long long)rem) - 1;
+    }
+  }
+};
 
 __device__ __forceinline__ float swiglu_f(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
@@ -269,6 +284,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     int issued = 0, slot = 0;
     uint32_t ph = 1;
     uint8_t* sw = smem;
+    LoraWalk walk;  // this CTA takes every ks-th block, from block `part`
+    walk.start(amask);
+    for (int j = 0; j < part && n_lora > 0; ++j) walk.next(p.lp);
+    const int s_base = p.lora ? slice_base(p.lp, n0) : 0;
     for (int i = 0; i < total; ++i) {
       if (!ring_wait(&empty_bar[slot], ph, &abort_flag, err)) break;
       uint64_t* bar = &full_bar[slot];
@@ -284,12 +303,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         sfw += 1024;
         sfx += 1024;
-      } else if (one) {
-        int bit;
-        const int col = lora_column(p.lp, amask, part + (i - n_main) * ks, bit);
-        mbar_arrive_expect_tx(bar, BW * 64 + x_bytes / 2);
-        tma_load_2d(sw, &tm_lb, bar, col, n0);
-        tma_load_2d(sx, &tm_s, bar, slice_base(p.lp, n0) + col, m0);
+      } else {
+        if (one) {
+          const int col = walk.column(p.lp);
+          mbar_arrive_expect_tx(bar, BW * 64 + x_bytes / 2);
+          tma_load_2d(sw, &tm_lb, bar, col, n0);
+          tma_load_2d(sx, &tm_s, bar, s_base + col, m0);
+        }
+        for (int j = 0; j < ks; ++j) walk.next(p.lp);
       }
       ++issued;
       sw += p.stage_bytes;
@@ -630,6 +651,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
       }
       const uint64_t both = mask0 | mask1, mine = rank ? mask1 : mask0;
       const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
+      const int base0 = p.lora ? slice_base(p.lp, n0) : 0, base1 = p.lora ? slice_base(p.lp, n0 + 128) : 0;
+      const bool one_slice = base0 == base1;
+      LoraWalk walk;
+      walk.start(both);
       for (int i = 0; i < total; ++i) {
         if (!ring_wait(&empty_bar[slot], ph, &abort_flag, err)) {
           stop = true;
@@ -650,11 +675,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             // As the main loop where the tile lies in one slice of S, else two halves of 128 weight
             // rows with their slice's columns, of which either CTA stages 64 rows of LB. A token tile
             // that lacks the adapter reads zeros.
-            int bit;
-            const int col = lora_column(p.lp, both, i - p.kstages, bit);
-            const int base0 = slice_base(p.lp, n0), base1 = slice_base(p.lp, n0 + 128), one_slice = base0 == base1;
+            const int col = walk.column(p.lp);
             if (leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * ((one_slice ? 1 : 2) * 128 * 64 + 128 * 64));
-            const int y = ((mine >> bit) & 1ull) ? m0 : mtiles128 * 128;
+            const int y = ((mine >> walk.bit) & 1ull) ? m0 : mtiles128 * 128;
             tma_load_2d_pair(sa, &tm_s, fb, base0 + col, y);
             if (!one_slice) tma_load_2d_pair(sa + 128 * 64, &tm_s, fb, base1 + col, y);
             const int first = n0 + (int)rank * (one_slice ? 128 : 64);
@@ -663,6 +686,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
           }
         }
         __syncwarp();
+        if (i >= p.kstages) walk.next(p.lp);
         ++issued;
         if (++slot == C::STAGES) {
           slot = 0;
@@ -688,6 +712,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         if (p.lora)
           total += __popcll(tile_adapters(p.lp, 2 * mt, mtiles128) | tile_adapters(p.lp, 2 * mt + 1, mtiles128)) *
                    p.lp.blocks_per_adapter;
+        const bool one_slice = !p.lora || slice_base(p.lp, nt * C::BN) == slice_base(p.lp, nt * C::BN + 128);
         if (!ring_wait(&tempty_bar, (ltile & 1) ^ 1, &abort_flag, err)) break;
         tc_fence_after();
         for (int i = 0; i < total; ++i) {
@@ -712,8 +737,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                 umma_mxf4_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(256, C::BN, 2 * (kk & 1)),
                                ta + 4 * (kk >> 1), tb + 8 * (kk >> 1), (i | kk) != 0);
             } else {
-              const int n0 = nt * C::BN;
-              const bool one_slice = slice_base(p.lp, n0) == slice_base(p.lp, n0 + 128);
               if (one_slice) {
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
