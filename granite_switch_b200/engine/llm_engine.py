@@ -50,6 +50,9 @@ class EngineConfig:
     max_wait_steps: int | None = DEFAULT_MAX_WAIT_STEPS  # cache_affinity: steps before a cold request
     #                                                    goes first; None = unbounded
     kv_cache_dtype: str = "bfloat16"       # or "fp8_e4m3": e4m3 K/V with a per-(token, KV head) scale
+    # "mxfp4": attention and dense-MLP projections with 4-bit weights and activations (quantised at
+    # load; LoRA, experts, embedding and LM head stay bf16); one GPU
+    weight_dtype: str = "bfloat16"
     # launch step i+1 before reading step i's sampled ids (they reach step i+1's inputs on
     # the device), so scheduling and bookkeeping overlap the GPU
     async_scheduling: bool = True
@@ -414,6 +417,10 @@ class LLM:
             config, path = GraniteSwitchConfig.from_pretrained(model), model
         self.config = config
         tp = ecfg.tensor_parallel_size
+        if ecfg.weight_dtype not in ("bfloat16", "mxfp4"):
+            raise ValueError(f"weight_dtype must be 'bfloat16' or 'mxfp4', got {ecfg.weight_dtype!r}")
+        if ecfg.weight_dtype == "mxfp4" and self.device.type != "cuda":
+            raise ValueError("weight_dtype 'mxfp4' needs a CUDA device (the CPU executor runs the checkpoint's weights)")
         if self.device.type == "cuda":
             from ..models.native import NativeGraniteSwitch, default_num_kv_blocks
             from .executor import NativeExecutor
@@ -427,13 +434,13 @@ class LLM:
                 # keeping only its shard; the loader audits that none went unused
                 ckpt = LazyCheckpoint(path)
                 nm = NativeGraniteSwitch.from_state_dict(config, ckpt, self.device, max_tokens, 1, tp_rank, tp,
-                                                         tp_group, ecfg.max_num_seqs, pipeline)
+                                                         tp_group, ecfg.max_num_seqs, pipeline, ecfg.weight_dtype)
                 ckpt.close()
             else:
                 ri = dict(random_init or {})
                 nm = NativeGraniteSwitch.from_random(config, self.device, max_tokens, 1, tp_rank=tp_rank,
                                                      tp_size=tp, tp_group=tp_group, max_seqs=ecfg.max_num_seqs,
-                                                     pipeline=pipeline, **ri)
+                                                     pipeline=pipeline, weight_dtype=ecfg.weight_dtype, **ri)
             if ecfg.kv_cache_dtype not in ("bfloat16", "fp8_e4m3"):
                 raise ValueError(f"kv_cache_dtype must be 'bfloat16' or 'fp8_e4m3', got {ecfg.kv_cache_dtype!r}")
             nm.kv_fp8 = ecfg.kv_cache_dtype == "fp8_e4m3"

@@ -29,8 +29,12 @@ from ..config import GraniteSwitchConfig
 from ..ops import attention as A
 from ..ops import elementwise as E
 from ..ops import gemm as G
+from ..ops import gemm_fp4 as F4
 from ..routing.scan import expert_table
-from .packing import PackedLinear, PackedMoE, choose_swiglu_tile, pack_linear, pack_moe
+from .packing import PackedLinear, PackedMoE, choose_swiglu_tile, pack_linear, pack_moe, quantise_linear
+
+
+WEIGHT_DTYPES = ("bfloat16", "mxfp4")
 
 
 @dataclass
@@ -79,7 +83,14 @@ class NativeGraniteSwitch:
 
     def __init__(self, config: GraniteSwitchConfig, device: torch.device, max_tokens: int,
                  num_kv_blocks: int, tp_rank: int = 0, tp_size: int = 1, tp_group=None,
-                 max_seqs: int = 512, pipeline=None):
+                 max_seqs: int = 512, pipeline=None, weight_dtype: str = "bfloat16"):
+        if weight_dtype not in WEIGHT_DTYPES:
+            raise ValueError(f"weight_dtype must be one of {WEIGHT_DTYPES}, got {weight_dtype!r}")
+        # MXFP4 projections (attention and dense / shared MLP; LoRA, experts, embedding and LM head
+        # stay bf16); the fused reductions and pipeline stages take bf16 projections only
+        self.mxfp4 = weight_dtype == "mxfp4"
+        if self.mxfp4 and (tp_size > 1 or pipeline is not None):
+            raise ValueError("weight_dtype 'mxfp4' runs on one GPU (no tensor or pipeline parallelism)")
         self.cfg = config
         self.device = device
         self.tp_rank, self.tp_size, self.tp_group = tp_rank, tp_size, tp_group
@@ -133,6 +144,12 @@ class NativeGraniteSwitch:
         self.probe_w = self.probe_b = self.probe_labels = None
 
     # ------------------------------------------------------------------ weights
+    def _swiglu_tile(self) -> int:
+        """gate/up interleave of the packed weight (0: no shared MLP)."""
+        if self.inter <= 0:
+            return 0
+        return F4.SWIGLU_TILE if self.mxfp4 else choose_swiglu_tile(self.inter)
+
     def _finish_weights(self, embed: torch.Tensor, final_norm: torch.Tensor, lm_head: torch.Tensor | None):
         self.embed_w = embed
         self.final_norm = final_norm
@@ -195,12 +212,14 @@ class NativeGraniteSwitch:
 
     @classmethod
     def from_state_dict(cls, config: GraniteSwitchConfig, sd, device, max_tokens: int, num_kv_blocks: int,
-                        tp_rank: int = 0, tp_size: int = 1, tp_group=None, max_seqs: int = 512, pipeline=None):
+                        tp_rank: int = 0, tp_size: int = 1, tp_group=None, max_seqs: int = 512, pipeline=None,
+                        weight_dtype: str = "bfloat16"):
         """Pack a composed checkpoint (``sd``: name -> tensor, or a lazy getter).
 
         With ``pipeline`` only this stage's decoder layers are read.
         """
-        self = cls(config, device, max_tokens, num_kv_blocks, tp_rank, tp_size, tp_group, max_seqs, pipeline)
+        self = cls(config, device, max_tokens, num_kv_blocks, tp_rank, tp_size, tp_group, max_seqs, pipeline,
+                   weight_dtype)
         get = sd.__getitem__ if hasattr(sd, "__getitem__") else sd
         if hasattr(sd, "__contains__"):
             def has(k):
@@ -216,7 +235,7 @@ class NativeGraniteSwitch:
         h, d = config.hidden_size, config.head_dim_eff
         q, kv = config.num_attention_heads * d, config.num_key_value_heads * d
         inter = config.shared_intermediate_size
-        tiles = choose_swiglu_tile(inter // tp_size) if inter > 0 else 0
+        tiles = self._swiglu_tile()
 
         def lin(prefix, slices, parallel, swiglu=0):
             base = prefix + ".base_layer.weight"
@@ -230,8 +249,9 @@ class NativeGraniteSwitch:
                     la, lb = [get(prefix + ".lora_A")], [get(prefix + ".lora_B")]
             else:
                 w, la, lb = get(prefix + ".weight"), None, None
-            return pack_linear(w, la, lb, slices, na, device, swiglu_tile=swiglu, tp_rank=tp_rank,
-                               tp_size=tp_size, parallel=parallel)
+            pl = pack_linear(w, la, lb, slices, na, device, swiglu_tile=swiglu, tp_rank=tp_rank,
+                             tp_size=tp_size, parallel=parallel)
+            return quantise_linear(pl) if self.mxfp4 else pl
 
         for i in range(self.layer_lo, self.layer_hi):
             p = f"model.layers.{i}."
@@ -270,20 +290,22 @@ class NativeGraniteSwitch:
     @classmethod
     def from_random(cls, config: GraniteSwitchConfig, device, max_tokens: int, num_kv_blocks: int,
                     lora_modules=("qkv",), rank: int = 32, seed: int = 0, std: float = 0.02,
-                    tp_rank: int = 0, tp_size: int = 1, tp_group=None, max_seqs: int = 512, pipeline=None):
+                    tp_rank: int = 0, tp_size: int = 1, tp_group=None, max_seqs: int = 512, pipeline=None,
+                    weight_dtype: str = "bfloat16"):
         """Random-init weights of the architecture, generated directly in kernel layout on the GPU.
 
         Every rank draws the full (unsharded) tensors of every layer from the same
         seed and keeps its shard (and, under pipeline parallelism, its stage's
         layers), so TP / PP runs are numerically the same model as one GPU.
         """
-        self = cls(config, device, max_tokens, num_kv_blocks, tp_rank, tp_size, tp_group, max_seqs, pipeline)
+        self = cls(config, device, max_tokens, num_kv_blocks, tp_rank, tp_size, tp_group, max_seqs, pipeline,
+                   weight_dtype)
         g = torch.Generator(device=device).manual_seed(seed)
         na = config.num_adapters
         h, d = config.hidden_size, config.head_dim_eff
         q, kv = config.num_attention_heads * d, config.num_key_value_heads * d
         inter = config.shared_intermediate_size
-        tiles = choose_swiglu_tile(inter // tp_size) if inter > 0 else 0
+        tiles = self._swiglu_tile()
         scale = 2.0  # alpha / r
         n_exp = int(getattr(config, "num_local_experts", 0) or 0)
 
@@ -297,8 +319,9 @@ class NativeGraniteSwitch:
             if lora and na > 0:
                 la = [rnd(na, 1, rank, k, s=0.02) for _ in n_out_slices]
                 lb = [rnd(na, 1, ns, rank, s=0.01 * scale) for ns in n_out_slices]
-            return pack_linear(w, la, lb, n_out_slices, na, device, swiglu_tile=swiglu, tp_rank=tp_rank,
-                               tp_size=tp_size, parallel=parallel)
+            pl = pack_linear(w, la, lb, n_out_slices, na, device, swiglu_tile=swiglu, tp_rank=tp_rank,
+                             tp_size=tp_size, parallel=parallel)
+            return quantise_linear(pl) if self.mxfp4 else pl
 
         for i in range(config.num_decoder_layers):
             lw = LayerWeights(
@@ -375,6 +398,14 @@ class NativeGraniteSwitch:
             self.moe_y = torch.empty(t, self.hidden, dtype=bf, device=dev)
         self.x2 = (torch.empty(t, self.hidden, dtype=bf, device=dev)
                    if moe is not None and self.has_shared_mlp else None)
+        if self.mxfp4:
+            def codes(k):
+                return (torch.empty(t, k // 2, dtype=torch.uint8, device=dev),
+                        torch.empty((t + 127) // 128, (k + 255) // 256 * 2, 512, dtype=torch.uint8, device=dev))
+
+            # quantised inputs of the projections by width, and the SwiGLU output's codes
+            self.in4 = {k: codes(k) for k in {self.hidden, self.num_q * self.head_dim, max(self.inter, F4.BLOCK)}}
+            self.act4 = codes(max(self.inter, F4.BLOCK))
         s_cols = 64
         for lw in self.layers:
             for pl in (lw.qkv, lw.o, lw.gu, lw.down, lw.cross):
@@ -430,14 +461,60 @@ class NativeGraniteSwitch:
         return self.prof.region(name) if self.prof is not None else contextlib.nullcontext()
 
     # ------------------------------------------------------------------ forward pieces
+    @staticmethod
+    def _rows4(codes, m: int):
+        return codes[0][:m], codes[1][: (m + 127) // 128]
+
+    def _norm(self, h: torch.Tensor, w: torch.Tensor, x: torch.Tensor, pl: PackedLinear | None,
+              rows: bool = False):
+        """RMSNorm before projection ``pl``: into ``x`` (bf16), or quantised for an MXFP4 projection,
+        whose codes are returned (``x`` is then written for the LoRA shrink, or on ``rows``)."""
+        if pl is None or pl.w4 is None:
+            E.rmsnorm(h, w, self.cfg.rms_norm_eps, out=x)
+            return None
+        c = self._rows4(self.in4[self.hidden], h.shape[0])
+        return F4.rmsnorm_mxfp4(h, w, self.cfg.rms_norm_eps, *c, out=x if rows or pl.has_lora else None)
+
+    def _proj4(self, pl: PackedLinear, x: torch.Tensor, out, epi, residual, scale, lora: bool, n_rows, xq,
+               keep_act: bool):
+        """An MXFP4 projection: ``xq`` holds the codes of ``x`` if the caller has them. With the SwiGLU
+        epilogue the output's codes are returned, and ``out`` is written on ``keep_act``."""
+        m = x.shape[0]
+        w4, sfw, lb, bounds = pl.w4, pl.sfw, pl.lb, pl.slice_bounds
+        if n_rows is not None:
+            assert n_rows == pl.slice_bounds[1], "n_rows must cover exactly the first slice"
+            w4, sfw, bounds = w4[:n_rows], sfw[: (n_rows + 127) // 128], [0, n_rows]
+            lb = lb[:n_rows] if lb is not None else None
+        kw = {}
+        if pl.has_lora and lora:
+            tm = self.tile_mask[pl.map_id, : (m + 127) // 128]
+            a_all = pl.a_all
+            if n_rows is not None:  # shrink of the first slice only
+                a_all = a_all[: (pl.n_local * pl.rank + 63) // 64 * 64]
+            s = self.s_buf[:m, : a_all.shape[0]]
+            G.lora_shrink(x, a_all, self.row_adapter[pl.map_id, :m], pl.rank, pl.n_local, out=s, tile_mask=tm)
+            kw = dict(s=s, lb=lb, tile_mask=tm, rank=pl.rank, num_adapters=pl.n_local)
+        if xq is None:
+            xq = F4.quantize_rows_mxfp4(x, *self._rows4(self.in4[x.shape[1]], m))
+        if epi == G.EPI_SWIGLU:
+            return F4.mxfp4_gemm_swiglu(*xq, w4, sfw, *self._rows4(self.act4, m), out if keep_act else None, **kw)
+        if kw:
+            kw["slice_bounds"] = bounds
+        epi4 = {G.EPI_STORE: F4.EPI_STORE, G.EPI_RESADD: F4.EPI_RESADD}[epi]
+        return F4.mxfp4_gemm(*xq, w4, sfw, out, epi=epi4, scale=scale, residual=residual, **kw)
+
     def _proj(self, pl: PackedLinear, x: torch.Tensor, out: torch.Tensor, epi=G.EPI_STORE, residual=None,
-              scale=1.0, mc_out: int = 0, lora: bool = True, n_rows: int | None = None):
-        """``out <- epi(x @ W^T (+ switched LoRA))``.
+              scale=1.0, mc_out: int = 0, lora: bool = True, n_rows: int | None = None, xq=None,
+              keep_act: bool = True):
+        """``out <- epi(x @ W^T (+ switched LoRA))``; returns ``out``, or what :meth:`_proj4` does.
 
         ``lora=False`` runs the base weight only (the Shadow-Residual base
         stream); ``n_rows`` restricts the projection to the first output rows
         of ``W``, which must be the first slice (the adapter stream's Q).
         """
+        if pl.w4 is not None:
+            assert mc_out == 0
+            return self._proj4(pl, x, out, epi, residual, scale, lora, n_rows, xq, keep_act)
         m = x.shape[0]
         w, lb, bounds = pl.w, pl.lb, pl.slice_bounds
         if n_rows is not None:
@@ -462,11 +539,11 @@ class NativeGraniteSwitch:
         return out
 
     def _row_parallel(self, pl: PackedLinear, x: torch.Tensor, h: torch.Tensor, mult: float, lora: bool = True,
-                      partial: torch.Tensor | None = None):
+                      partial: torch.Tensor | None = None, xq=None):
         """h <- h + x @ W^T * mult, summed over TP ranks."""
         m = x.shape[0]
         if self.tp_size == 1:
-            self._proj(pl, x, h, epi=G.EPI_RESADD, residual=h, scale=mult, lora=lora)
+            self._proj(pl, x, h, epi=G.EPI_RESADD, residual=h, scale=mult, lora=lora, xq=xq)
             return
         y = (partial if partial is not None else self.h2)[:m]
         if self.tp_rank == 0:
@@ -492,7 +569,7 @@ class NativeGraniteSwitch:
         G.switched_gemm(s, pl.lb, h, epi=G.EPI_RESADD, residual=h, scale=1.0)
 
     def _mlp(self, lw: LayerWeights, x: torch.Tensor, act: torch.Tensor, h: torch.Tensor, mult: float,
-             lora: bool = True, reuse_routing: bool = False, partial: torch.Tensor | None = None) -> None:
+             lora: bool = True, reuse_routing: bool = False, partial: torch.Tensor | None = None, xq=None) -> None:
         """``h <- h + MLP(x) * mult``: shared MLP, expert bank, or their sum (summed over TP ranks).
 
         ``lora=False`` runs base weights only; ``reuse_routing`` sends ``x`` to the
@@ -501,11 +578,18 @@ class NativeGraniteSwitch:
         (reference: src/granite_switch/hf/modeling_granite_switch.py:232-340).
         """
         R = self._region
+
+        def gate_up():
+            """SwiGLU of the gate/up projection: into ``act``, or as codes for an MXFP4 down projection."""
+            aq = self._proj(lw.gu, x, act, epi=G.EPI_SWIGLU, lora=lora, xq=xq,
+                            keep_act=lora and lw.down.has_lora)
+            return aq if lw.down.w4 is not None else None
+
         if lw.moe is None:
             with R("gate_up+swiglu"):
-                self._proj(lw.gu, x, act, epi=G.EPI_SWIGLU, lora=lora)
+                aq = gate_up()
             with R("down"):
-                self._row_parallel(lw.down, act, h, mult, lora=lora, partial=partial)
+                self._row_parallel(lw.down, act, h, mult, lora=lora, partial=partial, xq=aq)
             return
         m = x.shape[0]
         moe = lw.moe
@@ -530,10 +614,10 @@ class NativeGraniteSwitch:
         shared = None
         if lw.gu is not None:
             with R("gate_up+swiglu"):
-                self._proj(lw.gu, x, act, epi=G.EPI_SWIGLU, lora=lora)
+                aq = gate_up()
             with R("down"):
                 shared = self.x2[:m]
-                self._proj(lw.down, act, shared, epi=G.EPI_STORE, lora=lora)
+                self._proj(lw.down, act, shared, epi=G.EPI_STORE, lora=lora, xq=aq)
         with R("moe_combine"):
             if self.tp_size == 1:
                 nat.moe_combine(self.moe_yp, self.moe_slot[: m * k], self.moe_wts[: m * k], k, shared, h, mult, h)
@@ -582,11 +666,12 @@ class NativeGraniteSwitch:
                 with R("rmsnorm"):
                     E.rmsnorm(h, self.layers[0].in_norm, cfg.rms_norm_eps, out=x)
             for li, lw in enumerate(self.layers):
+                xq = None
                 if comm is None:
                     with R("rmsnorm"):
-                        E.rmsnorm(h, lw.in_norm, cfg.rms_norm_eps, out=x)
+                        xq = self._norm(h, lw.in_norm, x, lw.qkv)
                 with R("qkv"):
-                    self._proj(lw.qkv, x, qkv)
+                    self._proj(lw.qkv, x, qkv, xq=xq)
                 with R("rope+kv"):
                     self._rope_and_cache(b, qkv, li)
                 self._attention(b, qkv, li, attn, scale)
@@ -599,7 +684,7 @@ class NativeGraniteSwitch:
                     with R("o"):
                         self._row_parallel(lw.o, attn, h, mult)
                     with R("rmsnorm"):
-                        E.rmsnorm(h, lw.post_norm, cfg.rms_norm_eps, out=x)
+                        xq = self._norm(h, lw.post_norm, x, lw.gu, rows=lw.moe is not None)
                 if comm is not None:
                     with R("gate_up+swiglu"):
                         self._proj(lw.gu, x, act, epi=G.EPI_SWIGLU)
@@ -609,7 +694,7 @@ class NativeGraniteSwitch:
                     with R("finish+rmsnorm"):
                         comm.finish(y, h, nxt, x, cfg.rms_norm_eps)
                 else:
-                    self._mlp(lw, x, act, h, mult)
+                    self._mlp(lw, x, act, h, mult, xq=xq)
                 if probes:
                     self._probe_layer(b, self.layer_lo + li, h)
         if not self.last_stage:

@@ -44,6 +44,8 @@ class PackedLinear:
     map_id: int = -1                 # index into the model's remap table set
     swiglu_tile: int = 0             # > 0: gate/up interleaved per tile of this many rows
     bias: torch.Tensor | None = None
+    w4: torch.Tensor | None = None   # MXFP4 codes [N, K / 2] of the base weight; ``w`` is None then
+    sfw: torch.Tensor | None = None  # their scale atoms (ops.gemm_fp4)
 
     @property
     def has_lora(self) -> bool:
@@ -150,6 +152,28 @@ def pack_linear(base_w: torch.Tensor, lora_a: list[torch.Tensor] | None, lora_b:
     pl.w = w.to(device=device, dtype=dtype).contiguous()
     if bias is not None:
         pl.bias = bias.to(device=device, dtype=dtype)
+    return pl
+
+
+def quantise_linear(pl: PackedLinear) -> PackedLinear:
+    """Replace a packed projection's base weight by its MXFP4 form (the LoRA weights stay bf16).
+    gate/up projections must be interleaved per :data:`ops.gemm_fp4.SWIGLU_TILE` rows."""
+    from ..ops import gemm_fp4 as F
+
+    bad = None
+    if pl.k % F.BLOCK or pl.n % 8:
+        bad = f"needs K a multiple of {F.BLOCK} and N of 8"
+    elif pl.swiglu_tile not in (0, F.SWIGLU_TILE) or (pl.swiglu_tile and pl.n % F.SWIGLU_TILE):
+        bad = f"needs gate/up rows interleaved in whole tiles of {F.SWIGLU_TILE}"
+    elif pl.has_lora and not pl.swiglu_tile and any(b % 128 for b in pl.slice_bounds[:-1]):
+        bad = "with LoRA needs output slices that start at multiples of 128"
+    if bad:
+        raise ValueError(f"an MXFP4 projection {bad} (N={pl.n}, K={pl.k}, slices at {pl.slice_bounds})")
+    quantise = F.quantize_rows_mxfp4 if pl.w.is_cuda else F.quantize_rows_reference
+    pl.w4, pl.sfw = quantise(pl.w)
+    pl.w = None
+    if pl.swiglu_tile and pl.has_lora:
+        pl.lb = F.swiglu_lora_b(pl.lb)
     return pl
 
 

@@ -148,6 +148,8 @@ def main(argv=None):
     ap.add_argument("--tensor-parallel-size", type=int, default=1)
     ap.add_argument("--pipeline-parallel-size", type=int, default=1)
     ap.add_argument("--no-fused-tp-comm", action="store_true", help="reduce with NCCL only")
+    ap.add_argument("--weight-dtype", choices=["bfloat16", "mxfp4"], default="bfloat16",
+                    help="mxfp4: 4-bit weights and activations in the attention and dense-MLP projections")
     ap.add_argument("--kv-cache-dtype", choices=["auto", "bfloat16", "fp8", "fp8_e4m3"], default="auto",
                     help="KV cache storage: bf16 (auto) or e4m3 with a per-(token, KV head) scale")
     ap.add_argument("--no-async-scheduling", action="store_true",
@@ -169,6 +171,7 @@ def main(argv=None):
                         pipeline_parallel_size=pp, fused_tp_comm=not args.no_fused_tp_comm,
                         scheduling_policy=args.scheduling_policy,
                         max_wait_steps=args.max_wait_steps if args.max_wait_steps >= 0 else None,
+                        weight_dtype=args.weight_dtype,
                         kv_cache_dtype="fp8_e4m3" if args.kv_cache_dtype.startswith("fp8") else "bfloat16",
                         async_scheduling=not args.no_async_scheduling)
     sync = None

@@ -89,6 +89,7 @@ def main():
     p.add_argument("--warmup", type=int, default=3)
     p.add_argument("--no-fused-comm", dest="fused", action="store_false")
     p.add_argument("--lora", nargs="*", default=["qkv", "o"], help="projections with adapters")
+    p.add_argument("--weight-dtype", choices=["bfloat16", "mxfp4"], default="bfloat16")
     p.add_argument("--kv-cache-dtype", choices=["bfloat16", "fp8_e4m3"], default="bfloat16")
     p.add_argument("--prefill-split-ctas", type=int, default=None,
                    help="CTAs a split prefill grid aims at (A/B of ops.attention.PREFILL_SPLIT_CTAS)")
@@ -140,7 +141,8 @@ def main():
     ecfg = EngineConfig(max_num_seqs=max(8, len(args.prefill) + args.decode), max_num_batched_tokens=tokens,
                         max_model_len=max([args.prefill_ctx + n for n in args.prefill] + [args.decode_ctx + 1]) + 16,
                         tensor_parallel_size=world,
-                        num_kv_blocks=need_blocks, fused_tp_comm=args.fused, kv_cache_dtype=args.kv_cache_dtype)
+                        num_kv_blocks=need_blocks, fused_tp_comm=args.fused, kv_cache_dtype=args.kv_cache_dtype,
+                        weight_dtype=args.weight_dtype)
     ecfg.programmatic_launch = args.pdl
     ecfg.overlap_attention = args.attn_overlap
     from ..ops import attention as A
@@ -223,7 +225,7 @@ def main():
                               prefill_min_keys=A.PREFILL_MIN_KEYS_PER_SPLIT, small_shrink_max_m=G.SMALL_SHRINK_MAX_M,
                               decode_split_ctas=A.DECODE_SPLIT_CTAS,
                               attn_decode_stages=_native.native().attn_decode_stages(-1),
-                              kv_cache_dtype=args.kv_cache_dtype, fp8_decode_rows=args.fp8_decode_rows,
+                              kv_cache_dtype=args.kv_cache_dtype, weight_dtype=args.weight_dtype, fp8_decode_rows=args.fp8_decode_rows,
                               attn_fp8t_stages=_native.native().attn_fp8t_stages(-1),
                               step_ms=round(plain, 3), step_ms_with_regions=round(step_ms, 3),
                               host_enqueue_ms=round(host_ms, 3), ops=table)), flush=True)

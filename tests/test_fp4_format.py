@@ -105,3 +105,51 @@ def test_cpu_tensors_are_refused():
         F.quantize_rows_mxfp4(x)
     with pytest.raises(RuntimeError, match="CUDA"):
         F.rmsnorm_mxfp4(x, torch.ones(64).bfloat16(), 1e-5)
+
+
+def _packed(n, k, slices, swiglu=0, lora=True):
+    from granite_switch_b200.models.packing import pack_linear
+
+    g = torch.Generator().manual_seed(n + k)
+    la = [torch.randn(2, 1, 8, k, generator=g) for _ in slices] if lora else None
+    lb = [torch.randn(2, 1, s, 8, generator=g) for s in slices] if lora else None
+    return pack_linear(torch.randn(n, k, generator=g), la, lb, slices, 2, "cpu", swiglu_tile=swiglu)
+
+
+def test_quantise_linear():
+    """A packed projection in 4 bits: codes of its weight, LoRA kept in bf16, gate/up expand weights doubled."""
+    from granite_switch_b200.models.packing import quantise_linear
+
+    pl = _packed(384, 96, [256, 128])
+    w, lb = pl.w.clone(), pl.lb.clone()
+    quantise_linear(pl)
+    assert pl.w is None and torch.equal(pl.lb, lb)
+    x4, sf = F.quantize_rows_reference(w)
+    assert torch.equal(pl.w4, x4) and torch.equal(pl.sfw, sf)
+    gu = _packed(256, 64, [128, 128], swiglu=F.SWIGLU_TILE)
+    lb = gu.lb.clone()
+    quantise_linear(gu)
+    assert torch.equal(gu.lb, F.swiglu_lora_b(lb))
+
+
+@pytest.mark.parametrize("kw,what", [(dict(n=64, k=48, slices=[64], lora=False), "multiple of 32"),
+                                     (dict(n=20, k=64, slices=[20], lora=False), "N of 8"),
+                                     (dict(n=128, k=64, slices=[64, 64]), "multiples of 128"),
+                                     (dict(n=256, k=64, slices=[128, 128], swiglu=256), "interleaved")])
+def test_projections_that_are_refused(kw, what):
+    from granite_switch_b200.models.packing import quantise_linear
+
+    with pytest.raises(ValueError, match=what):
+        quantise_linear(_packed(**kw))
+
+
+def test_engine_refuses_what_it_cannot_run():
+    from granite_switch_b200.composer.synthetic import base_config
+    from granite_switch_b200.config import GraniteSwitchConfig
+    from granite_switch_b200.engine import LLM, EngineConfig
+
+    cfg = GraniteSwitchConfig(**base_config("micro"), num_adapters=0)
+    with pytest.raises(ValueError, match="weight_dtype"):
+        LLM(cfg, device="cpu", engine_config=EngineConfig(weight_dtype="fp4"))
+    with pytest.raises(ValueError, match="CUDA"):
+        LLM(cfg, device="cpu", engine_config=EngineConfig(weight_dtype="mxfp4"))
