@@ -49,12 +49,17 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 // Eight values times `inv` -> eight codes, v[0] in the lowest nibble (round to nearest
 // even, above 6 -> 6).
 __device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    r |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_E2M1,
-                                            cudaRoundNearest)
-         << (8 * j);
+  uint32_t r;
+  // a pair's first operand goes to the high nibble
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+        "f"(v[6] * inv), "f"(v[7] * inv));
   return r;
 }
 

@@ -1,13 +1,42 @@
 // Host-side pieces of the MXFP4 ops that the quantisers and the GEMM share (quant_fp4.cu).
 #pragma once
 
+#include "tma_util.h"
+
 #include <ATen/ATen.h>
 #include <cuda_runtime.h>
+
+#include <utility>
 
 namespace gsb {
 namespace f4 {
 
 inline bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// Launches an MXFP4 kernel with `cluster` CTAs a cluster (1: none, or compiled in), always as a
+// programmatic dependent of the kernel before it in the stream: before they wait for that one
+// (griddep_wait), these kernels touch their own shared and tensor memory only and prefetch
+// weights into L2, which reads nothing that could be stale. It saves 1 to 2 us a launch.
+template <typename... KArgs, typename... Args>
+inline void launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, int cluster, cudaStream_t st,
+                   Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  count_launch();
+  GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
 
 // bf16 [M, K] on `dev`, K a multiple of 32, rows 16-byte aligned.
 void check_rows(const char* op, const char* what, const at::Tensor& x, const at::Device& dev);
@@ -15,8 +44,7 @@ void check_rows(const char* op, const char* what, const at::Tensor& x, const at:
 // New code and scale buffers of an [M, K] matrix in place of undefined ones.
 void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf);
 
-// Quantises M > 0 rows on the current device. The kernel lets a programmatic dependent
-// start only once everything before it in the stream is done.
+// Quantises M > 0 rows on the current device.
 void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
                      cudaStream_t st);
 

@@ -1026,39 +1026,9 @@ static void check_out(const char* what, const at::Tensor& t, int64_t M, int64_t 
             "mxfp4_gemm: ", what, " must be bf16 [", M, ", ", N, "] with 16-byte aligned rows");
 }
 
-// Launches with `cluster` CTAs a cluster (1: none; the pair kernel has its size compiled in),
-// as a programmatic dependent of the kernel before when `dependent`.
-template <typename... KArgs, typename... Args>
-static void launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, int cluster, bool dependent,
-                   cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  unsigned n = 0;
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = (unsigned)cluster;
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (dependent) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  count_launch();
-  GSB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-}
-
 template <int EPI>
 static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tlb, const CUtensorMap& ts,
-                         const SplitParams& p, const SplitPlan& s, bool dependent, uint32_t* err, cudaStream_t st) {
+                         const SplitParams& p, const SplitPlan& s, uint32_t* err, cudaStream_t st) {
   auto kfn = mxfp4_split_kernel<EPI>;
   static bool set[kMaxDevices] = {false};
   const int dev = current_device();
@@ -1066,8 +1036,8 @@ static void launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const CUt
     GSB_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - BAR_BYTES));
     set[dev] = true;
   }
-  launch(kfn, dim3((unsigned)(s.weight_tiles * s.ks), (unsigned)s.token_tiles), THREADS, s.smem_bytes, s.ks, dependent,
-         st, tw, tx, tlb, ts, p, err);
+  launch(kfn, dim3((unsigned)(s.weight_tiles * s.ks), (unsigned)s.token_tiles), THREADS, s.smem_bytes, s.ks, st,
+         tw, tx, tlb, ts, p, err);
 }
 
 // Clusters of two of the pair kernel that fit at once (asked once per device and epilogue).
@@ -1097,10 +1067,10 @@ static int pair_clusters() {
 template <int EPI>
 static void launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& tsfx, const CUtensorMap& tsfw,
                         const CUtensorMap& ts, const CUtensorMap& tlb, const CUtensorMap& to, const PairParams& p,
-                        bool dependent, uint32_t* err, cudaStream_t st) {
+                        uint32_t* err, cudaStream_t st) {
   const int tiles = ((p.M + 255) / 256) * ((p.N + PairCfg::BN - 1) / PairCfg::BN);
   const int clusters = std::min(tiles, pair_clusters<EPI>());  // also sets the shared-memory attribute
-  launch(mxfp4_pair_kernel<EPI>, dim3(2 * clusters), PairCfg::THREADS, PairCfg::SMEM_BYTES, 1, dependent, st, tx, tw,
+  launch(mxfp4_pair_kernel<EPI>, dim3(2 * clusters), PairCfg::THREADS, PairCfg::SMEM_BYTES, 1, st, tx, tw,
          tsfx, tsfw, ts, tlb, to, p, err);
 }
 
@@ -1208,7 +1178,6 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   if (M == 0) return;
   auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());
-  bool dependent = pdl_enabled();
 
   at::Tensor work;  // codes and scales of bf16 rows; the stream orders its reuse
   if (t.bf != nullptr) {
@@ -1216,7 +1185,6 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
     work = at::empty({code_bytes + (M + 127) / 128 * k_tiles(K) * 512}, at::TensorOptions().dtype(at::kByte).device(dev));
     x = Codes{work.data_ptr<uint8_t>(), K / 2, work.data_ptr<uint8_t>() + code_bytes, M};
     quantize_launch(t.bf, t.ldbf, M, K, x.q, x.ld, x.sf, st);
-    dependent = true;  // of the quantiser, which lets it start when all before is done
   }
   auto tmap_s = [&](uint32_t rows) {
     return make_tmap_bf16_2d(la.s->data_ptr(), (uint64_t)M, (uint64_t)la.s->size(1), (uint64_t)la.s->stride(0), 32,
@@ -1250,9 +1218,9 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
                                : make_tmap_bf16_2d(p.out, (uint64_t)M, (uint64_t)N, (uint64_t)p.ldo, 64, 32,
                                                    CU_TENSOR_MAP_SWIZZLE_128B);
     switch (epi) {
-      case kEpiStore: launch_pair<kEpiStore>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
-      case kEpiResAdd: launch_pair<kEpiResAdd>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
-      default: launch_pair<kEpiSwiGLU>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, dependent, ep, st); break;
+      case kEpiStore: launch_pair<kEpiStore>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+      case kEpiResAdd: launch_pair<kEpiResAdd>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
+      default: launch_pair<kEpiSwiGLU>(tx, tw, tsfx, tsfw, ts, tlb, to, pp, ep, st); break;
     }
     return;
   }
@@ -1272,9 +1240,9 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   const CUtensorMap tw = make_tmap_codes(w, K, BW), tx = make_tmap_codes(x, K, mp);
   const CUtensorMap tlb = lora ? tmap_lb(BW) : tw, ts = lora ? tmap_s(mp) : tx;
   switch (epi) {
-    case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
-    case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
-    default: launch_split<kEpiSwiGLU>(tw, tx, tlb, ts, p, s, dependent, ep, st); break;
+    case kEpiStore: launch_split<kEpiStore>(tw, tx, tlb, ts, p, s, ep, st); break;
+    case kEpiResAdd: launch_split<kEpiResAdd>(tw, tx, tlb, ts, p, s, ep, st); break;
+    default: launch_split<kEpiSwiGLU>(tw, tx, tlb, ts, p, s, ep, st); break;
   }
 }
 

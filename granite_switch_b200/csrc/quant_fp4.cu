@@ -31,8 +31,8 @@ constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int K, int k2s, uint32_t per_row,
                           uint32_t warps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf) {
+  griddep_launch();
   griddep_wait();
-  griddep_launch();  // after the wait: a dependent may count on all that came before this kernel
   const int lane = threadIdx.x & 31;
   const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   if (warp >= warps) return;
@@ -59,9 +59,9 @@ __global__ void __launch_bounds__(kQuantThreads)
   }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {  // NaN if any is
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
   return r;
 }
 
@@ -75,10 +75,8 @@ __device__ __forceinline__ void norm_store8(const uint4& xq, const uint4& wq, fl
   unpack8(wq, g);
 #pragma unroll
   for (int j = 0; j < 8; ++j) y[j] = f[j] * g[j];
-  float top = fabsf(y[0]);
-#pragma unroll
-  for (int j = 1; j < 8; ++j) top = max_nan(top, fabsf(y[j]));
-  uint32_t byte = scale_byte(quad_max(__float_as_uint(fabsf(top * inv))));
+  const float top = max_abs3(max_abs3(y[0], y[1], y[2]), max_abs3(y[3], y[4], y[5]), max_abs3(y[6], y[7], y[7]));
+  uint32_t byte = scale_byte(quad_max(__float_as_uint(top * inv) & 0x7fffffffu));
   byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
   float s = inv_scale(byte);
   if (byte < 32u) {  // inv * 2^-e may overflow
@@ -108,8 +106,8 @@ __global__ void __launch_bounds__(256)
     rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w, int H,
                          float eps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf,
                          __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  griddep_wait();
   griddep_launch();
+  griddep_wait();
   const int64_t r = blockIdx.x;
   const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
   const uint4* wv = reinterpret_cast<const uint4*>(w);
@@ -158,8 +156,8 @@ __global__ void __launch_bounds__(256)
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_mxfp4_kernel(const uint8_t* __restrict__ x4, int64_t ld4, const uint8_t* __restrict__ sf, int K,
                             int k2s, uint32_t per_row, uint32_t warps, __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  griddep_wait();
   griddep_launch();
+  griddep_wait();
   const int lane = threadIdx.x & 31;
   const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   if (warp >= warps) return;
@@ -234,9 +232,8 @@ void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at:
 void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
                      cudaStream_t st) {
   const StreamGrid g = stream_grid("quantize_mxfp4", M, K);
-  launch_dependent(quantize_mxfp4_kernel, g.grid, dim3(kQuantThreads), 0, st,
-                   reinterpret_cast<const __nv_bfloat16*>(x), ldx, (int)K, (int)(k_tiles(K) / 2), g.per_row, g.warps, x4,
-                   ld4, sf);
+  launch(quantize_mxfp4_kernel, g.grid, kQuantThreads, 0, 1, st, reinterpret_cast<const __nv_bfloat16*>(x), ldx,
+         (int)K, (int)(k_tiles(K) / 2), g.per_row, g.warps, x4, ld4, sf);
 }
 
 }  // namespace f4
@@ -288,8 +285,8 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
   const int vpt = (int)((f4::k_tiles(H) * 16 + 255) / 256);
   auto go = [&](auto kernel) {
-    launch_dependent(kernel, dim3((unsigned)M), dim3(256), 0, st, xp, x.stride(0), wp, (int)H, (float)eps,
-                     x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
+    f4::launch(kernel, dim3((unsigned)M), 256, 0, 1, st, xp, x.stride(0), wp, (int)H, (float)eps,
+               x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
   };
   if (vpt <= 1) go(f4::rmsnorm_mxfp4_kernel<1>);
   else if (vpt <= 2) go(f4::rmsnorm_mxfp4_kernel<2>);
@@ -310,9 +307,9 @@ at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, cons
   f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
   if (M == 0) return out;
   const f4::StreamGrid s = f4::stream_grid("dequantize_mxfp4", M, K);
-  launch_dependent(f4::dequantize_mxfp4_kernel, s.grid, dim3(f4::kQuantThreads), 0,
-                   c10::cuda::getCurrentCUDAStream(x4.device().index()).stream(), x4.data_ptr<uint8_t>(),
-                   x4.stride(0), sf.data_ptr<uint8_t>(), (int)K, (int)(f4::k_tiles(K) / 2), s.per_row, s.warps,
-                   reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), out.stride(0));
+  f4::launch(f4::dequantize_mxfp4_kernel, s.grid, f4::kQuantThreads, 0, 1,
+             c10::cuda::getCurrentCUDAStream(x4.device().index()).stream(), x4.data_ptr<uint8_t>(), x4.stride(0),
+             sf.data_ptr<uint8_t>(), (int)K, (int)(f4::k_tiles(K) / 2), s.per_row, s.warps,
+             reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), out.stride(0));
   return out;
 }

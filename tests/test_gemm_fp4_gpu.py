@@ -347,8 +347,10 @@ def test_streams_and_graphs():
 
 
 def test_programmatic_launch_matches():
-    """Launched as programmatic dependents, with weights quantised just before, results are the same."""
+    """Weights quantised just before, and kernels of either launch kind around: results are the same. (The MXFP4
+    kernels are always programmatic dependents; set_pdl makes the others so too.)"""
     from granite_switch_b200._native import native
+    from granite_switch_b200.ops import elementwise as E
     from granite_switch_b200.ops import gemm_fp4 as F
 
     x, w = _rows(64, 2048, seed=20, spread=1), _rows(2048, 2048, seed=21, spread=1)
@@ -356,7 +358,13 @@ def test_programmatic_launch_matches():
     old = native().set_pdl(True)
     try:
         for _ in range(20):
-            assert torch.equal(F.mxfp4_linear(x, *F.quantize_rows_mxfp4(w)), want)
+            for on in (False, True):
+                native().set_pdl(on)
+                y = E.rmsnorm(x, torch.ones(2048, device="cuda").bfloat16(), 0.0)
+                assert torch.equal(F.mxfp4_linear(x, *F.quantize_rows_mxfp4(w)), want)
+                z = F.mxfp4_linear(y, *F.quantize_rows_mxfp4(w * 2))
+                E.residual_axpy(z, z, 1.0)
+                assert torch.equal(z, 2 * F.mxfp4_linear(y.clone(), *F.quantize_rows_mxfp4(w * 2)))
     finally:
         native().set_pdl(old)
 
