@@ -11,11 +11,14 @@
 //   swiglu   silu(gate) * up quantised to MXFP4 (and, on request, stored as bf16); the
 //            weight rows alternate in runs of 64: gate, up
 //
-// Operand-swapped kernel: the MMA's 128-row side is a tile of weight rows and its N
-// side the step's tokens (up to 256 per CTA), so a weight byte is read once per 256
-// tokens, whatever their number. The K range of a tile is split over the CTAs of a
-// cluster when the tiles alone do not fill the SMs; partial sums meet in distributed
-// shared memory in a fixed order, so results do not depend on timing.
+// Two kernels: the split kernel for few tokens, bound by the stream of weight bytes and by its
+// own latencies, and the pair kernel for many, bound by the tensor core (use_pair below).
+//
+// Split kernel: operands swapped, the MMA's 128-row side a tile of weight rows and its N
+// side up to 128 tokens, so a weight byte is read once per token tile, whatever the tokens'
+// number. The K range of a tile is split over the CTAs of a cluster when the tiles alone do not
+// fill the SMs; partial sums meet in distributed shared memory in a fixed order, so results
+// do not depend on timing.
 //
 // Warp roles (192 threads): warp 0 issues the TMA and bulk loads into a ring of
 // stages (256 K elements each), warp 1 owns the tensor memory and issues the scale
@@ -169,11 +172,11 @@ __device__ __forceinline__ void push_rows16(uint32_t addr, const uint32_t (&r)[1
   (st_dsmem_f32<J * P_STRIDE * 4>(addr, __uint_as_float(r[J])), ...);
 }
 
-// Adapters present among the rows of 128-row tile `t`.
+// Adapters present among the rows of 128-row tile `t` (a mask's bits past the last adapter are ignored).
 __device__ __forceinline__ uint64_t tile_adapters(const LoraParams& l, int t, int tiles) {
   if (t >= tiles) return 0ull;
-  if (l.tile_mask == nullptr) return (l.num_adapters >= 64) ? ~0ull : ((1ull << l.num_adapters) - 1);
-  return l.tile_mask[t];
+  const uint64_t all = (l.num_adapters >= 64) ? ~0ull : ((1ull << l.num_adapters) - 1);
+  return l.tile_mask == nullptr ? all : l.tile_mask[t] & all;
 }
 
 __device__ __forceinline__ int slice_base(const LoraParams& l, int row) {
@@ -1175,6 +1178,7 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
       p.lp.tile_mask = reinterpret_cast<const uint64_t*>(la.tile_mask->data_ptr());
     }
   }
+  GSB_CHECK((x.rows + 255) / 256 * ((w.rows + 255) / 256) < (int64_t(1) << 31), "mxfp4_gemm: output too large");
   if (M == 0) return;
   auto st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   auto* ep = reinterpret_cast<uint32_t*>(err.data_ptr());

@@ -152,13 +152,76 @@ def test_quantize_past_32_bits():
 
 # ------------------------------------------------------------------------------------------- products
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 16, 77, 128, 200, 300, 600])
-@pytest.mark.parametrize("n,k", [(256, 256), (8, 32), (264, 1056), (1024, 4096), (4096, 288)])
+@pytest.mark.parametrize("n,k", [(256, 256), (8, 32), (264, 1056), (1024, 4096), (4096, 288), (12808, 96)])
 def test_gemm_store(m, n, k):
     from granite_switch_b200.ops import gemm_fp4 as F
 
     a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=1)), F.quantize_rows_mxfp4(_rows(n, k, seed=2, spread=3))
     out = F.mxfp4_gemm(*a, *b, scale=0.5)
     _check(out, 0.5 * F.mxfp4_product_reference(*a, *b), 0.5 * _acc_tol(*a, *b))
+
+
+@pytest.fixture
+def pair_always():
+    from granite_switch_b200._native import native
+
+    old = native().mxfp4_pair_min_m(0)
+    yield
+    native().mxfp4_pair_min_m(old)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 8, 32), (1, 264, 4096), (129, 136, 288), (260, 1032, 2080), (384, 384, 256)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_pair_kernel_at_its_edges(pair_always, m, n, k, residual):
+    """The CTA-pair kernel on sizes that the rule gives to the split kernel: partial tiles in every direction."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=31)), F.quantize_rows_mxfp4(_rows(n, k, seed=32, spread=2))
+    ref, tol = F.mxfp4_product_reference(*a, *b), _acc_tol(*a, *b)
+    if residual:
+        h = torch.randn(m, n, device="cuda", generator=_gen(33)).to(torch.bfloat16)
+        ref, tol = h.double() + 0.5 * ref, 0.5 * tol + h.double().abs() * 2.0 ** -23
+        _check(F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.5, residual=h), ref, tol)
+    else:
+        _check(F.mxfp4_gemm(*a, *b), ref, tol)
+
+
+@pytest.mark.parametrize("m", [3, 200, 1400])
+@pytest.mark.parametrize("na,rank", [(64, 32), (3, 96)])
+def test_gemm_lora_limits(m, na, rank):
+    """As many adapters as a mask has bits, a rank of three blocks, mask bits past the last adapter, K over several
+    cluster parts."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    n, k = 1024, 2048
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=34)), F.quantize_rows_mxfp4(_rows(n, k, seed=35, spread=2))
+    s, dirty, lb, mask = _lora_inputs(m, n, 2, na, rank, seed=36)
+    if na < 64:
+        mask = mask | (5 << na)
+    kw = dict(lb=lb, rank=rank, num_adapters=na, slice_bounds=[0, 640, n])
+    ref = F.mxfp4_product_reference(*a, *b, s=s, **kw)
+    tol = _acc_tol(*a, *b, extra=(s.double().abs().sum(1, keepdim=True) * lb.double().abs().max()))
+    _check(F.mxfp4_gemm(*a, *b, s=dirty, tile_mask=mask, **kw), ref, tol)
+
+
+def test_two_streams_at_once():
+    """Calls of every kernel on two streams that overlap give what they give alone."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    b = F.quantize_rows_mxfp4(_rows(4096, 2048, seed=37, spread=1))
+    xs = [_rows(m, 2048, seed=m, spread=1) for m in (7, 100, 700, 2000)]
+    want = [F.mxfp4_linear(x, *b) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] += [F.mxfp4_linear(x, *b) for x in (xs if i else xs[::-1])]
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for j, y in enumerate(outs):
+            assert torch.equal(y, (want if i else want[::-1])[j % 4])
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (222, 1024, 2080), (2048, 2304, 512), (1300, 4096, 1024)])
@@ -192,7 +255,8 @@ def _lora_inputs(m, n, slices, na, rank, seed, absent=2):
     dirty = s.clone()
     for t in range(tiles):
         here = set(ra[t * 128:(t + 1) * 128].tolist()) - {0}
-        mask[t] = sum(1 << (a - 1) for a in here)
+        bits = sum(1 << (a - 1) for a in here)
+        mask[t] = bits - (1 << 64 if bits >> 63 else 0)
         gone = torch.tensor([int(c) not in here for c in col.tolist()], device="cuda")
         dirty[t * 128:(t + 1) * 128, gone] = float("nan")
     lb = (torch.randn(n, na * rank, device="cuda", generator=g) * 0.5).to(torch.bfloat16)
