@@ -30,10 +30,11 @@ __host__ __device__ constexpr int64_t k_tiles(int64_t K) { return (K + 255) / 25
 
 // Scale byte of a block whose largest magnitude has the fp32 bits `amax` (sign clear).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
-  const int f = (int)(amax >> 23);
-  if (f == 255) return 255u;
-  // 7 = 1.75 * 2^2: the exponent less two, one more when the mantissa is above 1.75
-  return (uint32_t)min(252, max(0, f - 2 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0)));
+  // 7 = 1.75 * 2^2: the exponent less two, one more when the mantissa is above 1.75 (the sum
+  // then carries into the exponent)
+  const int f = (int)((amax + 0x1fffffu) >> 23);
+  const uint32_t byte = (uint32_t)(max(2, min(254, f)) - 2);
+  return amax >= 0x7f800000u ? 255u : byte;
 }
 
 // 2^-e of a scale byte, exact for 0..252; 0 for 255 (the codes of such a block are 0).

@@ -24,6 +24,7 @@
 namespace gsb {
 namespace f4 {
 
+constexpr int kSms = 148;
 constexpr int kQuantThreads = 256;
 constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 
@@ -65,91 +66,135 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {  // NaN i
   return r;
 }
 
-// Eight normalised values -> codes, scales and (optionally) their part of the bf16 row. The
-// products x w are exact, and one multiplication by inv (times the block's power of two,
-// exact too) rounds each value; the maximum may be taken before it, since rounding keeps order.
-__device__ __forceinline__ void norm_store8(const uint4& xq, const uint4& wq, float inv, bool inside, int lane,
-                                            uint8_t* codes_out, uint8_t* sf, uint4* out) {
-  float f[8], g[8], y[8];
-  unpack8(xq, f);
-  unpack8(wq, g);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = f[j] * g[j];
-  const float top = max_abs3(max_abs3(y[0], y[1], y[2]), max_abs3(y[3], y[4], y[5]), max_abs3(y[6], y[7], y[7]));
-  uint32_t byte = scale_byte(quad_max(__float_as_uint(top * inv) & 0x7fffffffu));
-  byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
-  float s = inv_scale(byte);
-  if (byte < 32u) {  // inv * 2^-e may overflow
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] *= inv;
-  } else {
-    s *= inv;
-  }
-  const uint32_t codes = pack8(y, s);
-  if (inside) {
-    *reinterpret_cast<uint32_t*>(codes_out) = byte == 255u ? 0u : codes;
-    if (out != nullptr) {
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
-                           __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
-      *out = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-  }
-  store_scales256(byte, lane, sf);
-}
+// Rows in flight per CTA of the norm kernel, and resident CTAs per SM (registers: VPT 16-byte
+// vectors of a row per thread).
+__host__ __device__ constexpr int norm_stages(int vpt) { return vpt <= 4 ? 4 : 2; }
+__host__ __device__ constexpr int norm_ctas(int vpt) { return vpt <= 1 ? 5 : (vpt <= 2 ? 4 : 2); }
 
-// One CTA per row; the sum of squares in the RMSNorm kernel's order.
-template <int VPT>
-__global__ void __launch_bounds__(256)
-    rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w, int H,
-                         float eps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf,
-                         __nv_bfloat16* __restrict__ out, int64_t ldo) {
+// Persistent: a CTA walks rows, each thread copying its own vectors of the next rows into shared
+// memory (cp.async; a thread reads only what it copied, so that needs no barrier) and keeping
+// the weight in registers; one barrier a row, for the sum of squares, which is added in the order
+// of the RMSNorm kernel.
+//
+// A block's maximum is taken of the exact products x w, before the sum is known: rounding keeps
+// order, so it is the normalised block's after one multiplication. inv and the block's power of
+// two then make one factor, and each value is rounded once, by that product's conversion.
+template <int VPT, bool OUT>
+__global__ void __launch_bounds__(256, norm_ctas(VPT))
+    rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int ldx, const __nv_bfloat16* __restrict__ w, int M, int H,
+                         float eps, uint8_t* __restrict__ x4, int ld4, uint8_t* __restrict__ sf,
+                         __nv_bfloat16* __restrict__ out, int ldo) {
+  constexpr int STAGES = norm_stages(VPT);
+  extern __shared__ uint4 ring[];  // [STAGES][VPT][256]
+  __shared__ float4 red[2][2];
   griddep_launch();
   griddep_wait();
-  const int64_t r = blockIdx.x;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
-  const uint4* wv = reinterpret_cast<const uint4*>(w);
-  const int nvec = H / 8, nvec_pad = (int)k_tiles(H) * 16;
-  uint4 buf[VPT];
-  float ss = 0.f;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int nvec = H / 8, units = (int)k_tiles(H) / 2;
+  const uint4* xv = reinterpret_cast<const uint4*>(x) + tid;
+  uint4* slots = ring + tid;
+  uint4 wq[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * 256;
-    buf[i] = v < nvec ? xv[v] : make_uint4(0u, 0u, 0u, 0u);
+    const int v = tid + i * 256;
+    wq[i] = v < nvec ? reinterpret_cast<const uint4*>(w)[v] : make_uint4(0u, 0u, 0u, 0u);
+    if (v >= nvec)  // past the row: zeros for good
+      for (int s = 0; s < STAGES; ++s) slots[(s * VPT + i) * 256] = make_uint4(0u, 0u, 0u, 0u);
   }
+  auto fetch = [&](int r, int s) {
+    if (r < M) {
+      const uint4* src = xv + (int64_t)r * (ldx / 8);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const uint32_t p[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack_bf16x2(p[j]);
-      ss += f.x * f.x + f.y * f.y;
+      for (int i = 0; i < VPT; ++i)
+        if (tid + i * 256 < nvec)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slots + (s * VPT + i) * 256)),
+                       "l"(src + i * 256)
+                       : "memory");
     }
-  }
-  __shared__ float red[8], s_inv;
-  ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    float t = threadIdx.x < 8 ? red[threadIdx.x] : 0.f;
-    t = warp_sum(t);
-    if (threadIdx.x == 0) s_inv = rsqrtf(t / (float)H + eps);
-  }
-  __syncthreads();
-  const float inv = s_inv;
-  const int lane = threadIdx.x & 31;
-  uint8_t* codes = x4 + r * ld4 + threadIdx.x * 4;
-  uint8_t* scales = sf + sf_word(r, 2 * (threadIdx.x >> 5), k_tiles(H));
-  uint4* ov = out ? reinterpret_cast<uint4*>(out + r * ldo) + threadIdx.x : nullptr;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int grid = (int)gridDim.x;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * 256;
-    if (v >= nvec_pad) break;  // the whole warp: nvec_pad is a multiple of 32
-    const bool inside = v < nvec;
-    norm_store8(buf[i], inside ? wv[v] : make_uint4(0u, 0u, 0u, 0u), inv, inside, lane, codes + i * 1024,
-                scales + i * 8 * 1024, ov ? ov + i * 256 : nullptr);
+  for (int s = 0; s < STAGES - 1; ++s) fetch((int)blockIdx.x + s * grid, s);
+  // where this thread's codes and its warp's scale words lie in a row
+  uint8_t* codes0 = x4 + tid * 4;
+  uint8_t* scales0 = sf + (tid >> 5) * 1024;
+  const int atom_row = units * 1024;  // bytes of 128 rows' scales
+  int slot = 0, parity = 0;
+  for (int r = (int)blockIdx.x; r < M; r += grid) {
+    // the slot read last turn is free: this thread's reads of it went into values used since
+    fetch(r + (STAGES - 1) * grid, slot == 0 ? STAGES - 1 : slot - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    const uint4* xs = slots + slot * VPT * 256;
+    constexpr bool KEEP = VPT <= 4;  // the products stay in registers, or are formed again from the ring
+    float y[KEEP ? VPT : 1][8];
+    uint32_t top[VPT];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[8], g[8];
+      unpack8(xs[i * 256], f);
+      unpack8(wq[i], g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss += f[2 * j] * f[2 * j] + f[2 * j + 1] * f[2 * j + 1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= g[j];
+      const float t = max_abs3(max_abs3(f[0], f[1], f[2]), max_abs3(f[3], f[4], f[5]), max_abs3(f[6], f[7], f[7]));
+      if (KEEP) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[KEEP ? i : 0][j] = f[j];
+      }
+      top[i] = quad_max(__float_as_uint(t) & 0x7fffffffu);
+    }
+    ss = warp_sum(ss);
+    if (lane == 0) reinterpret_cast<float*>(red[parity])[tid >> 5] = ss;
+    __syncthreads();
+    const float4 a = red[parity][0], b = red[parity][1];
+    const float sum = ((a.x + b.x) + (a.z + b.z)) + ((a.y + b.y) + (a.w + b.w));
+    const float inv = rsqrtf(sum / (float)H + eps);
+    uint8_t* codes = codes0 + (int64_t)r * ld4;
+    uint8_t* scales = scales0 + (int64_t)(r >> 7) * atom_row + (16 * (r & 31) + 4 * ((r >> 5) & 3));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if ((tid >> 5) + i * 8 >= units) break;  // the whole warp
+      const bool inside = tid + i * 256 < nvec;
+      uint32_t byte = scale_byte(__float_as_uint(__uint_as_float(top[i]) * inv) & 0x7fffffffu);
+      byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
+      float s = inv_scale(byte);
+      float v[8];
+      if (KEEP) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = y[KEEP ? i : 0][j];
+      } else {
+        float g[8];
+        unpack8(xs[i * 256], v);
+        unpack8(wq[i], g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= g[j];
+      }
+      if (byte < 32u) {  // inv * 2^-e may overflow
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+      } else {
+        s *= inv;
+      }
+      const uint32_t c = pack8(v, s);
+      if (inside) *reinterpret_cast<uint32_t*>(codes + i * 1024) = byte == 255u ? 0u : c;
+      store_scales256(byte, lane, scales + i * 8 * 1024);
+      if (OUT && inside) {
+        float f[8], g[8];
+        unpack8(xs[i * 256], f);
+        unpack8(wq[i], g);
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
+                             __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
+        reinterpret_cast<uint4*>(out + (int64_t)r * ldo)[tid + i * 256] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    parity ^= 1;
   }
 }
 
@@ -196,7 +241,7 @@ static void check_codes(const char* op, const at::Tensor& x4, const at::Tensor& 
                         const at::Device& dev) {
   GSB_CHECK(x4.device() == dev && sf.device() == dev, op, ": every tensor must be on one device");
   GSB_CHECK(x4.scalar_type() == at::kByte && x4.dim() == 2 && x4.size(0) == M && x4.size(1) * 2 == K &&
-                x4.stride(1) == 1 && x4.stride(0) % 16 == 0 && aligned16(x4),
+                x4.stride(1) == 1 && x4.stride(0) % 16 == 0 && x4.stride(0) < (int64_t(1) << 31) && aligned16(x4),
             op, ": codes must be uint8 [M, K / 2] with 16-byte aligned rows");
   GSB_CHECK(sf.scalar_type() == at::kByte && sf.is_contiguous() && aligned16(sf) &&
                 sf.numel() == (M + 127) / 128 * k_tiles(K) * 512,
@@ -205,7 +250,7 @@ static void check_codes(const char* op, const at::Tensor& x4, const at::Tensor& 
 
 void check_rows(const char* op, const char* what, const at::Tensor& x, const at::Device& dev) {
   GSB_CHECK(x.is_cuda() && x.device() == dev && x.scalar_type() == at::kBFloat16 && x.dim() == 2 &&
-                (x.size(1) == 1 || x.stride(1) == 1) && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && aligned16(x),
+                (x.size(1) == 1 || x.stride(1) == 1) && (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && std::abs(x.stride(0)) < (int64_t(1) << 31))) && aligned16(x),
             op, ": ", what, " must be bf16 [M, K] on one CUDA device with 16-byte aligned rows");
   GSB_CHECK(x.size(1) >= kBlock && x.size(1) % kBlock == 0 && x.size(1) < (int64_t(1) << 31) &&
                 x.size(0) < (int64_t(1) << 31),
@@ -273,6 +318,7 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   f4::check_codes("rmsnorm_mxfp4", x4, sf, M, H, x.device());
   __nv_bfloat16* op = nullptr;
   int64_t ldo = 0;
+  GSB_CHECK(M < (int64_t(1) << 30), "rmsnorm_mxfp4: too many rows");
   if (out.has_value()) {
     f4::check_rows("rmsnorm_mxfp4", "out", *out, x.device());
     GSB_CHECK(out->size(0) == M && out->size(1) == H, "rmsnorm_mxfp4: out must be [M, H]");
@@ -284,14 +330,19 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   auto* xp = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
   const int vpt = (int)((f4::k_tiles(H) * 16 + 255) / 256);
-  auto go = [&](auto kernel) {
-    f4::launch(kernel, dim3((unsigned)M), 256, 0, 1, st, xp, x.stride(0), wp, (int)H, (float)eps,
-               x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(), op, ldo);
+  auto go = [&](auto kernel, int v) {
+    const int smem = f4::norm_stages(v) * v * 256 * 16;
+    if (smem > 48 * 1024)  // per device and cheap: no cache
+      GSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int64_t ctas = std::min<int64_t>(M, (int64_t)f4::norm_ctas(v) * f4::kSms);
+    f4::launch(kernel, dim3((unsigned)ctas), 256, smem, 1, st, xp, (int)x.stride(0), wp, (int)M, (int)H, (float)eps,
+               x4.data_ptr<uint8_t>(), (int)x4.stride(0), sf.data_ptr<uint8_t>(), op, (int)ldo);
   };
-  if (vpt <= 1) go(f4::rmsnorm_mxfp4_kernel<1>);
-  else if (vpt <= 2) go(f4::rmsnorm_mxfp4_kernel<2>);
-  else if (vpt <= 4) go(f4::rmsnorm_mxfp4_kernel<4>);
-  else go(f4::rmsnorm_mxfp4_kernel<8>);
+  auto pick = [&](auto plain, auto with_out, int v) { op == nullptr ? go(plain, v) : go(with_out, v); };
+  if (vpt <= 1) pick(f4::rmsnorm_mxfp4_kernel<1, false>, f4::rmsnorm_mxfp4_kernel<1, true>, 1);
+  else if (vpt <= 2) pick(f4::rmsnorm_mxfp4_kernel<2, false>, f4::rmsnorm_mxfp4_kernel<2, true>, 2);
+  else if (vpt <= 4) pick(f4::rmsnorm_mxfp4_kernel<4, false>, f4::rmsnorm_mxfp4_kernel<4, true>, 4);
+  else pick(f4::rmsnorm_mxfp4_kernel<8, false>, f4::rmsnorm_mxfp4_kernel<8, true>, 8);
   return {x4, sf};
 }
 
