@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint64_t amask = p.lora ? tile_adapters(p.lp, m0 / 128, mtiles128) : 0ull;
   const int n_lora_all = __popcll(amask) * p.lp.blocks_per_adapter;
   const int n_lora = n_lora_all > part ? (n_lora_all - part + ks - 1) / ks : 0;
-  const int total = n_main + n_lora;
+  const int total = n_main + (n_lora + 1) / 2;  // a stage holds two LoRA blocks
   const int acc_cols = (p.mt_rows + 31) / 32 * 32;  // accumulator, then the ring of scales: SF_COLS columns a stage
 
   if (warp == 0) {
@@ -307,13 +307,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         sfw += 1024;
         sfx += 1024;
       } else {
-        if (one) {
-          const int col = walk.column(p.lp);
-          mbar_arrive_expect_tx(bar, BW * 64 + x_bytes / 2);
-          tma_load_2d(sw, &tm_lb, bar, col, n0);
-          tma_load_2d(sx, &tm_s, bar, s_base + col, m0);
+        const int nb = min(2, n_lora - 2 * (i - n_main));
+        if (one) mbar_arrive_expect_tx(bar, nb * (BW * 64 + x_bytes / 2));
+        for (int b = 0; b < nb; ++b) {
+          if (one) {
+            const int col = walk.column(p.lp);
+            tma_load_2d(sw + b * BW * 64, &tm_lb, bar, col, n0);
+            tma_load_2d(sx + b * (x_bytes / 2), &tm_s, bar, s_base + col, m0);
+          }
+          for (int j = 0; j < ks; ++j) walk.next(p.lp);
         }
-        for (int j = 0; j < ks; ++j) walk.next(p.lp);
       }
       ++issued;
       sw += p.stage_bytes;
@@ -359,9 +362,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma_mxf4(tmem_base, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? idesc2 : idesc0, tw + 4 * (kk >> 1),
                       tx + x_col + 4 * (kk >> 1), (i | kk) != 0);
         } else {
-          const uint64_t ad = umma_desc_sw64(sw), bd = umma_desc_sw64(sx);
+          for (int b = 0; b < min(2, n_lora - 2 * (i - n_main)); ++b) {
+            const uint64_t ad = umma_desc_sw64(sw + b * BW * 64), bd = umma_desc_sw64(sx + b * (x_bytes / 2));
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) umma_bf16(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_bf, 1);
+            for (int kk = 0; kk < 2; ++kk) umma_bf16(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_bf, 1);
+          }
         }
         umma_commit(&empty_bar[slot]);
       }
@@ -653,9 +658,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         mask1 = tile_adapters(p.lp, 2 * mt + 1, mtiles128);
       }
       const uint64_t both = mask0 | mask1, mine = rank ? mask1 : mask0;
-      const int total = p.kstages + __popcll(both) * p.lp.blocks_per_adapter;
       const int base0 = p.lora ? slice_base(p.lp, n0) : 0, base1 = p.lora ? slice_base(p.lp, n0 + 128) : 0;
-      const bool one_slice = base0 == base1;
+      const bool one_slice = base0 == base1;  // then a stage holds two LoRA blocks
+      const int n_lora = __popcll(both) * p.lp.blocks_per_adapter, per = one_slice ? 2 : 1;
+      const int total = p.kstages + (n_lora + per - 1) / per;
       LoraWalk walk;
       walk.start(both);
       for (int i = 0; i < total; ++i) {
@@ -666,30 +672,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         uint8_t* sa = smem + slot * C::STAGE_BYTES;
         uint8_t* sb = sa + C::A_BYTES;
         const uint32_t fb = full_leader + slot * 8;
-        if (one) {
-          if (i < p.kstages) {
+        if (i < p.kstages) {
+          if (one) {
             // tiles past the last row are zeros, scales too
             if (leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * C::STAGE_BYTES);
             tma_load_2d_pair(sa, &tm_x, fb, i * BKB, m0);
             tma_load_2d_pair(sb, &tm_w, fb, i * BKB, n0 + (int)rank * 128);
             tma_load_3d_pair(sa + C::SFA_OFF, &tm_sfx, fb, 0, i, own);
             tma_load_3d_pair(sa + C::SFB_OFF, &tm_sfw, fb, 0, i, 2 * nt);
-          } else {
-            // As the main loop where the tile lies in one slice of S, else two halves of 128 weight
-            // rows with their slice's columns, of which either CTA stages 64 rows of LB. A token tile
-            // that lacks the adapter reads zeros.
-            const int col = walk.column(p.lp);
-            if (leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * ((one_slice ? 1 : 2) * 128 * 64 + 128 * 64));
-            const int y = ((mine >> walk.bit) & 1ull) ? m0 : mtiles128 * 128;
-            tma_load_2d_pair(sa, &tm_s, fb, base0 + col, y);
-            if (!one_slice) tma_load_2d_pair(sa + 128 * 64, &tm_s, fb, base1 + col, y);
-            const int first = n0 + (int)rank * (one_slice ? 128 : 64);
-            tma_load_2d_pair(sb, &tm_lb, fb, col, first);
-            tma_load_2d_pair(sb + 64 * 64, &tm_lb, fb, col, first + (one_slice ? 64 : 128));
+          }
+        } else {
+          // As the main loop where the tile lies in one slice of S, else two halves of 128 weight
+          // rows with their slice's columns, of which either CTA stages 64 rows of LB. A token tile
+          // that lacks the adapter reads zeros.
+          const int nb = min(per, n_lora - per * (i - p.kstages));
+          if (one && leader) mbar_arrive_expect_tx(&full_bar[slot], 2 * ((one_slice ? nb : 2) + nb) * 128 * 64);
+          for (int b = 0; b < nb; ++b) {
+            if (one) {
+              const int col = walk.column(p.lp);
+              const int y = ((mine >> walk.bit) & 1ull) ? m0 : mtiles128 * 128;
+              tma_load_2d_pair(sa + b * 128 * 64, &tm_s, fb, base0 + col, y);
+              if (!one_slice) tma_load_2d_pair(sa + 128 * 64, &tm_s, fb, base1 + col, y);
+              const int first = n0 + (int)rank * (one_slice ? 128 : 64);
+              uint8_t* lb = sb + b * 128 * 64;
+              tma_load_2d_pair(lb, &tm_lb, fb, col, first);
+              tma_load_2d_pair(lb + 64 * 64, &tm_lb, fb, col, first + (one_slice ? 64 : 128));
+            }
+            walk.next(p.lp);
           }
         }
         __syncwarp();
-        if (i >= p.kstages) walk.next(p.lp);
         ++issued;
         if (++slot == C::STAGES) {
           slot = 0;
@@ -711,11 +723,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
       for (int t = cluster_id; t < num_tiles && !stop; t += num_clusters, ++ltile) {
         int mt, nt;
         pair_tile(t, m_tiles, n_tiles, mt, nt);
-        int total = p.kstages;
-        if (p.lora)
-          total += __popcll(tile_adapters(p.lp, 2 * mt, mtiles128) | tile_adapters(p.lp, 2 * mt + 1, mtiles128)) *
-                   p.lp.blocks_per_adapter;
         const bool one_slice = !p.lora || slice_base(p.lp, nt * C::BN) == slice_base(p.lp, nt * C::BN + 128);
+        int n_lora = 0;
+        if (p.lora)
+          n_lora = __popcll(tile_adapters(p.lp, 2 * mt, mtiles128) | tile_adapters(p.lp, 2 * mt + 1, mtiles128)) *
+                   p.lp.blocks_per_adapter;
+        const int per = one_slice ? 2 : 1, total = p.kstages + (n_lora + per - 1) / per;
         if (!ring_wait(&tempty_bar, (ltile & 1) ^ 1, &abort_flag, err)) break;
         tc_fence_after();
         for (int i = 0; i < total; ++i) {
@@ -740,11 +753,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                 umma_mxf4_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc_mxf4(256, C::BN, 2 * (kk & 1)),
                                ta + 4 * (kk >> 1), tb + 8 * (kk >> 1), (i | kk) != 0);
             } else {
-              if (one_slice) {
+              for (int b = 0; one_slice && b < min(2, n_lora - 2 * (i - p.kstages)); ++b) {
+                const uint64_t ad = umma_desc_sw64(sa + b * 128 * 64), bd = umma_desc_sw64(sb + b * 128 * 64);
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
-                  umma_bf16_pair(tmem_base, umma_desc_sw64(sa) + 2 * kk, umma_desc_sw64(sb) + 2 * kk,
-                                 umma_idesc_bf16(256, C::BN), 1);
+                  umma_bf16_pair(tmem_base, ad + 2 * kk, bd + 2 * kk, umma_idesc_bf16(256, C::BN), 1);
               }
               const uint32_t idesc = umma_idesc_bf16(256, 128);
 #pragma unroll

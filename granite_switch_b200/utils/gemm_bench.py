@@ -21,6 +21,12 @@ weight scales, LoRA in bf16; :mod:`ops.gemm_fp8`):
   bf16 expand fused (what an fp8 projection costs),
 * ``fp8_base``   - the fp8 GEMM alone on pre-quantised operands, no adapters.
 
+With ``--mxfp4`` (4-bit base weight and activations, LoRA in bf16; :mod:`ops.gemm_fp4`):
+
+* ``mxfp4_native`` - bf16 LoRA shrink + quantiser + 4-bit GEMM with the bf16 expand
+  fused (what an MXFP4 projection costs),
+* ``mxfp4_base``   - the 4-bit GEMM alone on quantised operands, no adapters.
+
 With ``--reference`` the reference's own switched projection runs beside them
 (``reference``): one cuBLAS GEMM of ``x`` against ``[W; A_1..A_n]`` and the
 reference's Triton expand kernel (``switch_lora_expand`` from the installed
@@ -139,7 +145,8 @@ def reference_case(c, n, k, rank, ref):
                 block_n=block_n)
 
 
-def run_point(m, n, k, rank, na, flush, dev, iters=20, compare_pair=False, fp8=False, ref=None):
+def run_point(m, n, k, rank, na, flush, dev, iters=20, compare_pair=False, fp8=False, ref=None,
+              mxfp4=False):
     c = make_case(m, n, k, rank, na, dev)
     x, w = c["x"], c["w"]
     out = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
@@ -177,6 +184,21 @@ def run_point(m, n, k, rank, na, flush, dev, iters=20, compare_pair=False, fp8=F
             F.fp8_gemm(x8, sfa, w8, sfb, out)
 
         fns += [("fp8_native", fp8_native_fn, None), ("fp8_base", fp8_base_fn, None)]
+    if mxfp4:
+        from ..ops import gemm_fp4 as F4
+
+        x4, sfx = F4.quantize_rows_mxfp4(x)
+        w4, sfw = F4.quantize_rows_mxfp4(w)
+
+        def mxfp4_native_fn():
+            G.lora_shrink(x, c["a_all"], c["ids"], c["rank"], c["na"], out=s, tile_mask=c["mask"])
+            F4.mxfp4_linear(x, w4, sfw, out, s=s, lb=c["lb"], tile_mask=c["mask"], rank=c["rank"],
+                            num_adapters=c["na"])
+
+        def mxfp4_base_fn():
+            F4.mxfp4_gemm(x4, sfx, w4, sfw, out)
+
+        fns += [("mxfp4_native", mxfp4_native_fn, None), ("mxfp4_base", mxfp4_base_fn, None)]
     if ref is not None:
         rc = reference_case(c, n, k, rank, ref)
         x_ext = torch.empty(m, rc["w_ext"].shape[0], dtype=torch.bfloat16, device=dev)
@@ -307,6 +329,7 @@ def main():
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--compare-pair", action="store_true", help="time CTA-pair and single-CTA tiles side by side")
     p.add_argument("--fp8", action="store_true", help="also time the block-scaled fp8 GEMM")
+    p.add_argument("--mxfp4", action="store_true", help="also time the MXFP4 GEMM")
     p.add_argument("--reference", action="store_true",
                    help="also time the reference's switched projection (cuBLAS + its Triton expand)")
     p.add_argument("--shapes", nargs="*", default=None, help="N x K pairs as NxK (default: the three 8B shapes)")
@@ -334,7 +357,8 @@ def main():
         for n, k in shapes:
             for r in ranks:
                 for na in adapters:
-                    res = run_point(m, n, k, r, na, flush, dev, args.iters, args.compare_pair, args.fp8, ref)
+                    res = run_point(m, n, k, r, na, flush, dev, args.iters, args.compare_pair, args.fp8, ref,
+                                    args.mxfp4)
                     print(json.dumps(dict(m=m, n=n, k=k, rank=r, adapters=na, **res)), flush=True)
 
 

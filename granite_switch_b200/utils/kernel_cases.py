@@ -2,7 +2,7 @@
 
 ``python -m granite_switch_b200.utils.kernel_cases <case>`` with case in
 gemm, gemm_pair, gemm_single, cublas, swiglu, attn_prefill64, moe, probe, decode_gemm, decode_shrink, lora_small, fp8_gemm,
-fp8_quant, attn_prefill, attn_decode, attn_decode_fp8, attn_decode_fp8t, rmsnorm, rope, embed, routing, sample (or ``all``). Pair it with ``ncu --clock-control none -k regex:<kernel> -c 1`` (without
+fp8_quant, fp4_gemm, fp4_decode, fp4_quant, fp4_norm, attn_prefill, attn_decode, attn_decode_fp8, attn_decode_fp8t, rmsnorm, rope, embed, routing, sample (or ``all``). Pair it with ``ncu --clock-control none -k regex:<kernel> -c 1`` (without
 ``--clock-control none`` ncu locks the GPU clocks).
 """
 import sys
@@ -60,6 +60,20 @@ if want("fp8_gemm") or want("fp8_quant"):  # block-scaled fp8 GEMM, 4096 x 12800
     if want("fp8_gemm"):
         w8, sfb = F.quantize_weight_fp8((torch.randn(I, H, device=dev) * 0.02).bfloat16())
         out8 = F.fp8_gemm(x8, sfa, w8, sfb)
+if want("fp4_gemm") or want("fp4_decode") or want("fp4_quant") or want("fp4_norm"):
+    # MXFP4: the CTA-pair GEMM at 4096 x 4096 x 4096, the split GEMM of 16 rows over 4096 x 12800, the quantiser
+    # of 8192 x 12800 rows, the norm with quantisation of 8192 x 4096 rows
+    from granite_switch_b200.ops import gemm_fp4 as F4
+    if want("fp4_gemm"):
+        F4.mxfp4_gemm(*F4.quantize_rows_mxfp4(torch.randn(T, H, device=dev).bfloat16()),
+                      *F4.quantize_rows_mxfp4(torch.randn(H, H, device=dev).bfloat16()))
+    if want("fp4_decode"):
+        F4.mxfp4_gemm(*F4.quantize_rows_mxfp4(torch.randn(16, I, device=dev).bfloat16()),
+                      *F4.quantize_rows_mxfp4(torch.randn(H, I, device=dev).bfloat16()))
+    if want("fp4_quant"):
+        F4.quantize_rows_mxfp4(torch.randn(8192, I, device=dev).bfloat16())
+    if want("fp4_norm"):
+        F4.rmsnorm_mxfp4(torch.randn(8192, H, device=dev).bfloat16(), torch.ones(H, device=dev).bfloat16(), 1e-5)
 if want("decode_shrink"):  # LoRA shrink of o_proj in the headline decode step (222 tokens, 12 adapters r32)
     xs = torch.randn(222, H, device=dev).bfloat16()
     a_all = (torch.randn(12 * 32, H, device=dev) * 0.02).bfloat16()
