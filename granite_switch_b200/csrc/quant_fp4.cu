@@ -1,14 +1,15 @@
 // MXFP4 quantisation of bf16 rows, the same fused behind RMSNorm, and the way back
-// (format: fp4.cuh). All three stream their rows once and are bound by memory.
+// (format: fp4.cuh). All three stream their rows once.
 //
 //   quantize_mxfp4: a warp takes 256 neighbours of a row, eight per lane (one 16-byte
-//     load), so a block of 32 is four lanes and its maximum two shuffles; several such
-//     units are in flight per warp.
-//   rmsnorm_mxfp4: one CTA per row, the row in registers (as in elementwise.cu's
-//     RMSNorm). y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then
-//     one rounding, to 4 bits; with `out` the row also leaves as bf16, rounded exactly
-//     as the RMSNorm kernel does, for the LoRA shrink.
-//   dequantize_mxfp4: codes times scale, exact in bf16.
+//     load), so a block of 32 is four lanes and its maximum two shuffles; four such units are
+//     in flight per warp. 8192 x 12800 rows: 45 us, 5.9 TB/s, 0.91 of the measured copy.
+//   rmsnorm_mxfp4: the row in registers between the sum of squares and the conversion.
+//     y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then one rounding, to
+//     4 bits; with `out` the row also leaves as bf16, rounded exactly as the RMSNorm kernel does,
+//     for the LoRA shrink. 8192 x 4096 rows: 24 us, 3.5 TB/s, bound by instruction issue (2.9 of 4
+//     a cycle: unpacking, squares, products, maxima and conversions of every value).
+//   dequantize_mxfp4: codes times scale, exact in bf16. 8192 x 12800 rows: 42 us, 6.4 TB/s.
 #include "common.cuh"
 #include "fp4.cuh"
 #include "fp4_host.h"
