@@ -4,12 +4,19 @@
 #include "tma_util.h"
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <cuda_runtime.h>
 
 #include <utility>
 
 namespace gsb {
 namespace f4 {
+
+// An uninitialised tensor on `dev`, without the dispatcher (these ops' host time is their
+// smallest calls' time).
+inline at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
 
 inline bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 

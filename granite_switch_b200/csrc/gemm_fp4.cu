@@ -1212,7 +1212,7 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   at::Tensor work;  // codes and scales of bf16 rows; the stream orders its reuse
   if (t.bf != nullptr) {
     const int64_t code_bytes = (M * (K / 2) + 1023) / 1024 * 1024;
-    work = at::empty({code_bytes + (M + 127) / 128 * k_tiles(K) * 512}, at::TensorOptions().dtype(at::kByte).device(dev));
+    work = new_tensor({code_bytes + (M + 127) / 128 * k_tiles(K) * 512}, at::kByte, dev);
     x = Codes{work.data_ptr<uint8_t>(), K / 2, work.data_ptr<uint8_t>() + code_bytes, M};
     quantize_launch(t.bf, t.ldbf, M, K, x.q, x.ld, x.sf, st);
   }
@@ -1276,10 +1276,6 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   }
 }
 
-static at::Tensor new_out(int64_t M, int64_t N, const at::Device& dev) {
-  return at::empty({M, N}, at::TensorOptions().dtype(at::kBFloat16).device(dev));
-}
-
 static void check_epi(int64_t epi) {
   GSB_CHECK(epi == kEpiStore || epi == kEpiResAdd, "mxfp4_gemm: epilogue must be store (0) or residual add (1)");
 }
@@ -1302,7 +1298,7 @@ at::Tensor gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at:
   const at::Device dev = x4.device();
   const f4::Codes x = f4::check_operand("x", x4, sfx, K, dev), w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
-  const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(x.rows, w.rows, dev);
+  const at::Tensor out = out_.has_value() ? *out_ : f4::new_tensor({x.rows, w.rows}, at::kBFloat16, dev);
   f4::run_gemm(f4::Tokens{x, nullptr, 0}, w, K, &out, (int)epi, scale, residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
                             slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
@@ -1323,7 +1319,7 @@ at::Tensor gsb_mxfp4_linear(const at::Tensor& x, const at::Tensor& w4, const at:
   const at::Device dev = x.device();
   const f4::Codes w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
-  const at::Tensor out = out_.has_value() ? *out_ : f4::new_out(M, w.rows, dev);
+  const at::Tensor out = out_.has_value() ? *out_ : f4::new_tensor({M, w.rows}, at::kBFloat16, dev);
   f4::run_gemm(f4::Tokens{f4::Codes{nullptr, 0, nullptr, M}, x.data_ptr(), x.stride(0)}, w, K, &out, (int)epi, scale,
                residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,

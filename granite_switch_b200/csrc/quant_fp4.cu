@@ -270,9 +270,8 @@ static StreamGrid stream_grid(const char* op, int64_t M, int64_t K) {
 }
 
 void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf) {
-  const auto opt = at::TensorOptions().dtype(at::kByte).device(dev);
-  if (!x4.defined()) x4 = at::empty({M, K / 2}, opt);
-  if (!sf.defined()) sf = at::empty({(M + 127) / 128, k_tiles(K), 512}, opt);
+  if (!x4.defined()) x4 = new_tensor({M, K / 2}, at::kByte, dev);
+  if (!sf.defined()) sf = new_tensor({(M + 127) / 128, k_tiles(K), 512}, at::kByte, dev);
 }
 
 void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
@@ -353,7 +352,7 @@ at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, cons
   const int64_t M = x4.size(0), K = x4.size(1) * 2;
   c10::cuda::CUDAGuard g(x4.device());
   at::Tensor out = out_.has_value() ? *out_
-                                    : at::empty({M, K}, at::TensorOptions().dtype(at::kBFloat16).device(x4.device()));
+                                    : f4::new_tensor({M, K}, at::kBFloat16, x4.device());
   f4::check_rows("dequantize_mxfp4", "out", out, x4.device());
   GSB_CHECK(out.size(0) == M && out.size(1) == K, "dequantize_mxfp4: out must be [M, K]");
   f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
