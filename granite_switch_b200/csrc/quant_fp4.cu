@@ -242,7 +242,8 @@ static void check_codes(const char* op, const at::Tensor& x4, const at::Tensor& 
                         const at::Device& dev) {
   GSB_CHECK(x4.device() == dev && sf.device() == dev, op, ": every tensor must be on one device");
   GSB_CHECK(x4.scalar_type() == at::kByte && x4.dim() == 2 && x4.size(0) == M && x4.size(1) * 2 == K &&
-                x4.stride(1) == 1 && x4.stride(0) % 16 == 0 && x4.stride(0) < (int64_t(1) << 31) && aligned16(x4),
+                x4.stride(1) == 1 && x4.stride(0) % 16 == 0 && (M <= 1 || x4.stride(0) >= x4.size(1)) &&
+                x4.stride(0) < (int64_t(1) << 31) && aligned16(x4),
             op, ": codes must be uint8 [M, K / 2] with 16-byte aligned rows");
   GSB_CHECK(sf.scalar_type() == at::kByte && sf.is_contiguous() && aligned16(sf) &&
                 sf.numel() == (M + 127) / 128 * k_tiles(K) * 512,
@@ -321,7 +322,8 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   GSB_CHECK(M < (int64_t(1) << 30), "rmsnorm_mxfp4: too many rows");
   if (out.has_value()) {
     f4::check_rows("rmsnorm_mxfp4", "out", *out, x.device());
-    GSB_CHECK(out->size(0) == M && out->size(1) == H, "rmsnorm_mxfp4: out must be [M, H]");
+    GSB_CHECK(out->size(0) == M && out->size(1) == H && (M <= 1 || out->stride(0) >= H),
+              "rmsnorm_mxfp4: out must be [M, H] with rows of their own");
     op = reinterpret_cast<__nv_bfloat16*>(out->data_ptr());
     ldo = out->stride(0);
   }
@@ -354,7 +356,8 @@ at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, cons
   at::Tensor out = out_.has_value() ? *out_
                                     : f4::new_tensor({M, K}, at::kBFloat16, x4.device());
   f4::check_rows("dequantize_mxfp4", "out", out, x4.device());
-  GSB_CHECK(out.size(0) == M && out.size(1) == K, "dequantize_mxfp4: out must be [M, K]");
+  GSB_CHECK(out.size(0) == M && out.size(1) == K && (M <= 1 || out.stride(0) >= K),
+            "dequantize_mxfp4: out must be [M, K] with rows of their own");
   f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
   if (M == 0) return out;
   const f4::StreamGrid s = f4::stream_grid("dequantize_mxfp4", M, K);

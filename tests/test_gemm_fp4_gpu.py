@@ -354,6 +354,23 @@ def test_mlp_block(m):
     assert ((out.double() - x.double() - 0.22 * full).norm() / (0.22 * full).norm()).item() < 2.0 ** -6
 
 
+def test_broadcast_rows_and_in_place_norm():
+    """One row for all as input; the norm's bf16 rows over its own input."""
+    from granite_switch_b200.ops import elementwise as E
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    row = _rows(1, 512, seed=41)
+    w = torch.ones(512, device="cuda").bfloat16()
+    b = F.quantize_rows_mxfp4(_rows(256, 512, seed=42, spread=1))
+    for m in (3, 300):
+        assert torch.equal(F.mxfp4_linear(row.expand(m, 512), *b), F.mxfp4_linear(row.repeat(m, 1), *b))
+        x = torch.randn(m, 512, device="cuda", generator=_gen(43)).to(torch.bfloat16)
+        want, ref = E.rmsnorm(x, w, 1e-5), F.rmsnorm_mxfp4(x, w, 1e-5)
+        x4, sf = F.rmsnorm_mxfp4(x, w, 1e-5, out=x)
+        assert torch.equal(x, want) and torch.equal(x4, ref[0])
+        assert torch.equal(F.scale_bytes_from_atoms(sf, m, 512), F.scale_bytes_from_atoms(ref[1], m, 512))
+
+
 def test_nan_and_empty():
     from granite_switch_b200.ops import gemm_fp4 as F
 
@@ -450,6 +467,9 @@ def test_refusals():
         lambda: F.rmsnorm_mxfp4(x, torch.ones(128, device="cuda").bfloat16(), 1e-5),
         lambda: F.rmsnorm_mxfp4(x, torch.ones(256, device="cuda"), 1e-5),
         lambda: F.dequantize_mxfp4(*a, out=torch.empty(16, 128, dtype=torch.bfloat16, device="cuda")),
+        lambda: F.dequantize_mxfp4(*a, out=out[:1].expand(16, 256)),                # one row for all
+        lambda: F.quantize_rows_mxfp4(x, x4=a[0][:1].expand(16, 128)),
+        lambda: F.mxfp4_gemm(*a, *b, out=out[:1].expand(16, 256)),
         lambda: F.mxfp4_gemm(a[0][:, :64], a[1], *b),                               # K differs
         lambda: F.mxfp4_gemm(*a, b[0], a[1]),                                       # too few scales
         lambda: F.mxfp4_gemm(*a, b[0][:252], b[1]),                                 # N not a multiple of 8
