@@ -431,68 +431,84 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   }
+  const int r0 = part * rows_per, n_rows = max(0, min(rows, r0 + rows_per) - r0);
+  constexpr int GROUPS = (EPI == kEpiSwiGLU) ? 8 : 16;  // 8-column groups per token
+  const int items = n_rows * GROUPS;
+  // a token's eight columns from c, summed over the parts
+  auto sum8 = [&](int lm, int c, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 1
+    for (int q = 0; q < ks; ++q) {
+      const float* src = R + (q * rows_per + lm) * P_STRIDE + c;
+      const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
+      v[0] += a0.x; v[1] += a0.y; v[2] += a0.z; v[3] += a0.w;
+      v[4] += a1.x; v[5] += a1.y; v[6] += a1.z; v[7] += a1.w;
+    }
+  };
+  // The residuals of a thread's first items are loaded before the barrier, four at a time.
+  constexpr int BATCH = 4;
+  uint4 res[BATCH];
+  auto load_residuals = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int it = first + j * THREADS, col = n0 + (it % GROUPS) * 8;
+      res[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (it < items && col < p.N)
+        res[j] = *reinterpret_cast<const uint4*>(p.residual + (int64_t)(m0 + r0 + it / GROUPS) * p.ldr + col);
+    }
+  };
+  if (EPI == kEpiResAdd) load_residuals(threadIdx.x);
   __syncthreads();
   if (ks > 1) cluster_sync();  // every partial row has landed
-  if (!abort_flag) {
-    const int r0 = part * rows_per, n_rows = max(0, min(rows, r0 + rows_per) - r0);
-    constexpr int GROUPS = (EPI == kEpiSwiGLU) ? 8 : 16;  // 8-column groups per token
-    const int items = n_rows * GROUPS;
+  if (abort_flag) {
+    // nothing is written
+  } else if constexpr (EPI == kEpiSwiGLU) {
+    // four neighbouring items are one block of 32 outputs; whole warps run for the shuffles
     for (int it = threadIdx.x; it < (items + 31) / 32 * 32; it += THREADS) {
       const int lm = min(it, items - 1) / GROUPS, c = (it % GROUPS) * 8, m = m0 + r0 + lm;
       float v[8], u[8];
+      sum8(lm, c, v);
+      sum8(lm, c + 64, u);
+      const int col = tile * 64 + c;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
-#pragma unroll 1
-      for (int q = 0; q < ks; ++q) {
-        const float* src = R + (q * rows_per + lm) * P_STRIDE + c;
-        const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
-        v[0] += a0.x; v[1] += a0.y; v[2] += a0.z; v[3] += a0.w;
-        v[4] += a1.x; v[5] += a1.y; v[6] += a1.z; v[7] += a1.w;
-        if (EPI == kEpiSwiGLU) {
-          const float4 b0 = *reinterpret_cast<const float4*>(src + 64), b1 = *reinterpret_cast<const float4*>(src + 68);
-          u[0] += b0.x; u[1] += b0.y; u[2] += b0.z; u[3] += b0.w;
-          u[4] += b1.x; u[5] += b1.y; u[6] += b1.z; u[7] += b1.w;
-        }
-      }
-      if (EPI == kEpiSwiGLU) {
-        // four neighbouring items are one block of 32 outputs
-        const int col = tile * 64 + c;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = swiglu_f(v[j], u[j]);
-        const uint32_t byte = scale_byte(quad_max(max_abs_bits(v)));
-        if (it < items) {
-          if (p.out != nullptr)
-            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)m * p.ldo + col) = make_uint4(
-                pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-          const int64_t kt = k_tiles(p.N / 2);
-          uint8_t* word = p.sfa_out + sf_word(m, col >> 7, kt);
-          if ((c & 31) == 0) word[(col >> 5) & 3] = (uint8_t)byte;
-          // the last tile also clears the scales past the row's end
-          if (col + 8 == p.N / 2)
-            for (int b = p.N / 64; b < kt * 4; ++b) p.sfa_out[sf_word(m, b >> 2, kt) + (b & 3)] = 0;
-          if (byte == 255u) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.f;
-          }
-          *reinterpret_cast<uint32_t*>(p.a4 + (int64_t)m * p.lda4 + col / 2) = pack8(v, inv_scale(byte));
-        }
-      } else {
-        const int col = n0 + c;
-        if (it >= items || col >= p.N) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= p.scale;
-        if (EPI == kEpiResAdd) {
-          const uint4 w = *reinterpret_cast<const uint4*>(p.residual + (int64_t)m * p.ldr + col);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack_bf16x2(ww[j]);
-            v[2 * j] += f.x;
-            v[2 * j + 1] += f.y;
-          }
-        }
+      for (int j = 0; j < 8; ++j) v[j] = swiglu_f(v[j], u[j]);
+      const uint32_t byte = scale_byte(quad_max(max_abs_bits(v)));
+      if (it >= items) continue;
+      if (p.out != nullptr)
         *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)m * p.ldo + col) = make_uint4(
             pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      const int64_t kt = k_tiles(p.N / 2);
+      if ((c & 31) == 0) p.sfa_out[sf_word(m, col >> 7, kt) + ((col >> 5) & 3)] = (uint8_t)byte;
+      // the last tile also clears the scales past the row's end
+      if (col + 8 == p.N / 2)
+        for (int b = p.N / 64; b < kt * 4; ++b) p.sfa_out[sf_word(m, b >> 2, kt) + (b & 3)] = 0;
+      *reinterpret_cast<uint32_t*>(p.a4 + (int64_t)m * p.lda4 + col / 2) =
+          byte == 255u ? 0u : pack8(v, inv_scale(byte));
+    }
+  } else {
+    for (int first = threadIdx.x; first < items; first += BATCH * THREADS) {
+      if (EPI == kEpiResAdd && first != threadIdx.x) load_residuals(first);
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int it = first + j * THREADS, lm = it / GROUPS, c = (it % GROUPS) * 8, col = n0 + c;
+        if (it >= items || col >= p.N) continue;
+        float v[8];
+        sum8(lm, c, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= p.scale;
+        if (EPI == kEpiResAdd) {
+          const uint32_t ww[4] = {res[j].x, res[j].y, res[j].z, res[j].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack_bf16x2(ww[k]);
+            v[2 * k] += f.x;
+            v[2 * k + 1] += f.y;
+          }
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(m0 + r0 + lm) * p.ldo + col) =
+            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
       }
     }
   }
