@@ -48,7 +48,7 @@ inline void launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, i
 // bf16 [M, K] on `dev`, K a multiple of 32, rows 16-byte aligned.
 void check_rows(const char* op, const char* what, const at::Tensor& x, const at::Device& dev);
 
-// New code and scale buffers of an [M, K] matrix in place of undefined ones.
+// New code and scale buffers of an [M, K] matrix in place of undefined ones (two new ones share a storage).
 void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf);
 
 // Quantises M > 0 rows on the current device.

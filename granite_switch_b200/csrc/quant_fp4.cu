@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <tuple>
+#include <utility>
 
 namespace gsb {
 namespace f4 {
@@ -271,8 +272,19 @@ static StreamGrid stream_grid(const char* op, int64_t M, int64_t K) {
 }
 
 void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf) {
+  const int64_t codes = (M * (K / 2) + 127) / 128 * 128, m_tiles = (M + 127) / 128;
+  if (!x4.defined() && !sf.defined()) {
+    // one allocation for both: a second one costs a sixth of a small call
+    x4 = new_tensor({codes + m_tiles * k_tiles(K) * 512}, at::kByte, dev);
+    auto scales = c10::make_intrusive<c10::TensorImpl>(c10::Storage(x4.storage()), x4.key_set(), x4.dtype());
+    scales->set_storage_offset(codes);
+    scales->set_sizes_contiguous({m_tiles, k_tiles(K), 512});
+    sf = at::Tensor(std::move(scales));
+    x4.unsafeGetTensorImpl()->set_sizes_contiguous({M, K / 2});
+    return;
+  }
   if (!x4.defined()) x4 = new_tensor({M, K / 2}, at::kByte, dev);
-  if (!sf.defined()) sf = new_tensor({(M + 127) / 128, k_tiles(K), 512}, at::kByte, dev);
+  if (!sf.defined()) sf = new_tensor({m_tiles, k_tiles(K), 512}, at::kByte, dev);
 }
 
 void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
