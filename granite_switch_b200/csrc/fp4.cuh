@@ -47,9 +47,8 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __uint_as_float(byte == 0u ? 0x400000u : (byte == 255u ? 0x7fc00000u : byte << 23));
 }
 
-// Eight values times `inv` -> eight codes, v[0] in the lowest nibble (round to nearest
-// even, above 6 -> 6).
-__device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
+// Eight values -> eight codes, v[0] in the lowest nibble (round to nearest even, above 6 -> 6).
+__device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
   uint32_t r;
   // a pair's first operand goes to the high nibble
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -59,9 +58,28 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
       "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
       "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(r)
-      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
-        "f"(v[6] * inv), "f"(v[7] * inv));
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
+}
+
+// Eight values times `inv` -> eight codes.
+__device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = v[j] * inv;
+  return pack8(f);
+}
+
+// The same of packed pairs.
+__device__ __forceinline__ uint32_t pack8(const uint64_t (&v)[4], float inv) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t p = f32x2_mul(v[j], f32x2_pack(inv, inv));
+    f[2 * j] = f32x2_lo(p);
+    f[2 * j + 1] = f32x2_hi(p);
+  }
+  return pack8(f);
 }
 
 __device__ __forceinline__ uint32_t max_abs_bits(const float (&v)[8]) {
@@ -85,6 +103,13 @@ __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
     v[2 * j] = f.x;
     v[2 * j + 1] = f.y;
   }
+}
+
+// Eight bf16 values as fp32 pairs.
+__device__ __forceinline__ void unpack_pairs(const uint4& q, uint64_t (&v)[4]) {
+  const uint32_t p[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = f32x2_pack_bits(p[j] << 16, p[j] & 0xffff0000u);
 }
 
 // fp32 bits of the largest magnitude of eight packed bf16 values (as 16-bit integers, so a

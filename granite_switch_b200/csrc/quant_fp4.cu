@@ -7,7 +7,7 @@
 //   rmsnorm_mxfp4: the row in registers between the sum of squares and the conversion.
 //     y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then one rounding, to
 //     4 bits; with `out` the row also leaves as bf16, rounded exactly as the RMSNorm kernel does,
-//     for the LoRA shrink. 8192 x 4096 rows: 24 us, 3.5 TB/s, bound by instruction issue (2.9 of 4
+//     for the LoRA shrink. 8192 x 4096 rows: 21 us, 4.0 TB/s, bound by instruction issue (2.9 of 4
 //     a cycle: unpacking, squares, products, maxima and conversions of every value).
 //   dequantize_mxfp4: codes times scale, exact in bf16. 8192 x 12800 rows: 42 us, 6.4 TB/s.
 #include "common.cuh"
@@ -95,11 +95,15 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
   const int nvec = H / 8, units = (int)k_tiles(H) / 2;
   const uint4* xv = reinterpret_cast<const uint4*>(x) + tid;
   uint4* slots = ring + tid;
-  uint4 wq[VPT];
+  constexpr bool KEEP = VPT <= 4;  // fp32 weights and products stay in registers, or are formed again
+  uint4 wq[KEEP ? 1 : VPT];
+  uint64_t wf[KEEP ? VPT : 1][4];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = tid + i * 256;
-    wq[i] = v < nvec ? reinterpret_cast<const uint4*>(w)[v] : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 q = v < nvec ? reinterpret_cast<const uint4*>(w)[v] : make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (KEEP) unpack_pairs(q, wf[i]);
+    else wq[i] = q;
     if (v >= nvec)  // past the row: zeros for good
       for (int s = 0; s < STAGES; ++s) slots[(s * VPT + i) * 256] = make_uint4(0u, 0u, 0u, 0u);
   }
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
   for (int s = 0; s < STAGES - 1; ++s) fetch((int)blockIdx.x + s * grid, s);
   // where this thread's codes and its warp's scale words lie in a row
   uint8_t* codes0 = x4 + tid * 4;
-  uint8_t* scales0 = sf + (tid >> 5) * 1024;
+  uint8_t* scales0 = sf + (tid >> 5) * 1024 + (lane >> 4) * 512 + ((lane >> 2) & 3);
   const int atom_row = units * 1024;  // bytes of 128 rows' scales
   int slot = 0, parity = 0;
   for (int r = (int)blockIdx.x; r < M; r += grid) {
@@ -128,24 +132,24 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
     fetch(r + (STAGES - 1) * grid, slot == 0 ? STAGES - 1 : slot - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     const uint4* xs = slots + slot * VPT * 256;
-    constexpr bool KEEP = VPT <= 4;  // the products stay in registers, or are formed again from the ring
-    float y[KEEP ? VPT : 1][8];
+    uint64_t y[KEEP ? VPT : 1][4];
     uint32_t top[VPT];
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float f[8], g[8];
-      unpack8(xs[i * 256], f);
-      unpack8(wq[i], g);
+      uint64_t f[4], g[4];
+      unpack_pairs(xs[i * 256], f);
+      if constexpr (!KEEP) unpack_pairs(wq[i], g);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss += f[2 * j] * f[2 * j] + f[2 * j + 1] * f[2 * j + 1];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= g[j];
-      const float t = max_abs3(max_abs3(f[0], f[1], f[2]), max_abs3(f[3], f[4], f[5]), max_abs3(f[6], f[7], f[7]));
-      if (KEEP) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[KEEP ? i : 0][j] = f[j];
+      for (int j = 0; j < 4; ++j) {
+        const float lo = f32x2_lo(f[j]), hi = f32x2_hi(f[j]);
+        ss += lo * lo + hi * hi;
+        f[j] = f32x2_mul(f[j], KEEP ? wf[KEEP ? i : 0][j] : g[j]);
+        if (KEEP) y[KEEP ? i : 0][j] = f[j];
       }
+      const float t = max_abs3(max_abs3(f32x2_lo(f[0]), f32x2_hi(f[0]), f32x2_lo(f[1])),
+                               max_abs3(f32x2_hi(f[1]), f32x2_lo(f[2]), f32x2_hi(f[2])),
+                               max_abs3(f32x2_lo(f[3]), f32x2_hi(f[3]), f32x2_hi(f[3])));
       top[i] = quad_max(__float_as_uint(t) & 0x7fffffffu);
     }
     ss = warp_sum(ss);
@@ -163,35 +167,33 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
       uint32_t byte = scale_byte(__float_as_uint(__uint_as_float(top[i]) * inv) & 0x7fffffffu);
       byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
       float s = inv_scale(byte);
-      float v[8];
-      if (KEEP) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = y[KEEP ? i : 0][j];
-      } else {
-        float g[8];
-        unpack8(xs[i * 256], v);
-        unpack8(wq[i], g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= g[j];
+      uint64_t v[4], g[4];
+      if constexpr (!KEEP) {
+        unpack_pairs(xs[i * 256], v);
+        unpack_pairs(wq[i], g);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = KEEP ? y[KEEP ? i : 0][j] : f32x2_mul(v[j], g[j]);
       if (byte < 32u) {  // inv * 2^-e may overflow
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        for (int j = 0; j < 4; ++j) v[j] = f32x2_mul(v[j], f32x2_pack(inv, inv));
       } else {
         s *= inv;
       }
       const uint32_t c = pack8(v, s);
       if (inside) *reinterpret_cast<uint32_t*>(codes + i * 1024) = byte == 255u ? 0u : c;
-      store_scales256(byte, lane, scales + i * 8 * 1024);
+      // a block's lanes hold its byte alike; the first stores it
+      if ((lane & 3) == 0) scales[i * 8 * 1024] = (uint8_t)byte;
       if (OUT && inside) {
-        float f[8], g[8];
+        float f[8];
         unpack8(xs[i * 256], f);
-        unpack8(wq[i], g);
         uint32_t o[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * g[2 * j],
-                             __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * g[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t gj = KEEP ? wf[KEEP ? i : 0][j] : g[j];
+          o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * f32x2_lo(gj),
+                             __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * f32x2_hi(gj));
+        }
         reinterpret_cast<uint4*>(out + (int64_t)r * ldo)[tid + i * 256] = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
