@@ -7,8 +7,8 @@
 //   rmsnorm_mxfp4: the row in registers between the sum of squares and the conversion.
 //     y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then one rounding, to
 //     4 bits; with `out` the row also leaves as bf16, rounded exactly as the RMSNorm kernel does,
-//     for the LoRA shrink. 8192 x 4096 rows: 21 us, 4.0 TB/s, bound by instruction issue (2.9 of 4
-//     a cycle: unpacking, squares, products, maxima and conversions of every value).
+//     for the LoRA shrink. 8192 x 4096 rows: 19.4 us, 4.4 TB/s, bound by instruction issue (2.75 of
+//     4 a cycle: unpacking, squares, products, maxima and conversions of every value).
 //   dequantize_mxfp4: codes times scale, exact in bf16. 8192 x 12800 rows: 42 us, 6.4 TB/s.
 #include "common.cuh"
 #include "fp4.cuh"
@@ -68,10 +68,12 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {  // NaN i
   return r;
 }
 
-// Rows in flight per CTA of the norm kernel, and resident CTAs per SM (registers: VPT 16-byte
-// vectors of a row per thread).
+// The norm kernel's NT threads hold VPT 16-byte vectors of a row each. Up to 4096 columns 128 threads
+// share a row's fixed instructions among more values than 256 would (8192 x 4096 19.4 against 21.2 us,
+// 8192 x 2048 12.2 against 14.5, 16 x 4096 1.73 against 1.65). Rows in flight per CTA, and resident
+// CTAs per SM (what the registers allow without spills):
 __host__ __device__ constexpr int norm_stages(int vpt) { return vpt <= 4 ? 4 : 2; }
-__host__ __device__ constexpr int norm_ctas(int vpt) { return vpt <= 1 ? 5 : (vpt <= 2 ? 4 : 2); }
+__host__ __device__ constexpr int norm_ctas(int vpt, int nt) { return nt == 256 ? 2 : (vpt <= 2 ? 8 : 5); }
 
 // Persistent: a CTA walks rows, each thread copying its own vectors of the next rows into shared
 // memory (cp.async; a thread reads only what it copied, so that needs no barrier) and keeping
@@ -81,13 +83,14 @@ __host__ __device__ constexpr int norm_ctas(int vpt) { return vpt <= 1 ? 5 : (vp
 // A block's maximum is taken of the exact products x w, before the sum is known: rounding keeps
 // order, so it is the normalised block's after one multiplication. inv and the block's power of
 // two then make one factor, and each value is rounded once, by that product's conversion.
-template <int VPT, bool OUT>
-__global__ void __launch_bounds__(256, norm_ctas(VPT))
+template <int NT, int VPT, bool OUT>
+__global__ void __launch_bounds__(NT, norm_ctas(VPT, NT))
     rmsnorm_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int ldx, const __nv_bfloat16* __restrict__ w, int M, int H,
                          float eps, uint8_t* __restrict__ x4, int ld4, uint8_t* __restrict__ sf,
                          __nv_bfloat16* __restrict__ out, int ldo) {
   constexpr int STAGES = norm_stages(VPT);
-  extern __shared__ uint4 ring[];  // [STAGES][VPT][256]
+  constexpr int GROUPS = 256 / NT;  // threads of the RMSNorm kernel that one thread stands for
+  extern __shared__ uint4 ring[];  // [STAGES][VPT][NT]
   __shared__ float4 red[2][2];
   griddep_launch();
   griddep_wait();
@@ -100,21 +103,21 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
   uint64_t wf[KEEP ? VPT : 1][4];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = tid + i * 256;
+    const int v = tid + i * NT;
     const uint4 q = v < nvec ? reinterpret_cast<const uint4*>(w)[v] : make_uint4(0u, 0u, 0u, 0u);
     if constexpr (KEEP) unpack_pairs(q, wf[i]);
     else wq[i] = q;
     if (v >= nvec)  // past the row: zeros for good
-      for (int s = 0; s < STAGES; ++s) slots[(s * VPT + i) * 256] = make_uint4(0u, 0u, 0u, 0u);
+      for (int s = 0; s < STAGES; ++s) slots[(s * VPT + i) * NT] = make_uint4(0u, 0u, 0u, 0u);
   }
   auto fetch = [&](int r, int s) {
     if (r < M) {
       const uint4* src = xv + (int64_t)r * (ldx / 8);
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
-        if (tid + i * 256 < nvec)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slots + (s * VPT + i) * 256)),
-                       "l"(src + i * 256)
+        if (tid + i * NT < nvec)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slots + (s * VPT + i) * NT)),
+                       "l"(src + i * NT)
                        : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -131,19 +134,19 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
     // the slot read last turn is free: this thread's reads of it went into values used since
     fetch(r + (STAGES - 1) * grid, slot == 0 ? STAGES - 1 : slot - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    const uint4* xs = slots + slot * VPT * 256;
+    const uint4* xs = slots + slot * VPT * NT;
     uint64_t y[KEEP ? VPT : 1][4];
     uint32_t top[VPT];
-    float ss = 0.f;
+    float ss[GROUPS] = {};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       uint64_t f[4], g[4];
-      unpack_pairs(xs[i * 256], f);
+      unpack_pairs(xs[i * NT], f);
       if constexpr (!KEEP) unpack_pairs(wq[i], g);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float lo = f32x2_lo(f[j]), hi = f32x2_hi(f[j]);
-        ss += lo * lo + hi * hi;
+        ss[i % GROUPS] += lo * lo + hi * hi;
         f[j] = f32x2_mul(f[j], KEEP ? wf[KEEP ? i : 0][j] : g[j]);
         if (KEEP) y[KEEP ? i : 0][j] = f[j];
       }
@@ -152,8 +155,11 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
                                max_abs3(f32x2_lo(f[3]), f32x2_hi(f[3]), f32x2_hi(f[3])));
       top[i] = quad_max(__float_as_uint(t) & 0x7fffffffu);
     }
-    ss = warp_sum(ss);
-    if (lane == 0) reinterpret_cast<float*>(red[parity])[tid >> 5] = ss;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) ss[g] = warp_sum(ss[g]);
+    if (lane == 0)
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) reinterpret_cast<float*>(red[parity])[(tid >> 5) + g * (NT / 32)] = ss[g];
     __syncthreads();
     const float4 a = red[parity][0], b = red[parity][1];
     const float sum = ((a.x + b.x) + (a.z + b.z)) + ((a.y + b.y) + (a.w + b.w));
@@ -162,14 +168,14 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
     uint8_t* scales = scales0 + (int64_t)(r >> 7) * atom_row + (16 * (r & 31) + 4 * ((r >> 5) & 3));
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if ((tid >> 5) + i * 8 >= units) break;  // the whole warp
-      const bool inside = tid + i * 256 < nvec;
+      if ((tid >> 5) + i * (NT / 32) >= units) break;  // the whole warp
+      const bool inside = tid + i * NT < nvec;
       uint32_t byte = scale_byte(__float_as_uint(__uint_as_float(top[i]) * inv) & 0x7fffffffu);
       byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
       float s = inv_scale(byte);
       uint64_t v[4], g[4];
       if constexpr (!KEEP) {
-        unpack_pairs(xs[i * 256], v);
+        unpack_pairs(xs[i * NT], v);
         unpack_pairs(wq[i], g);
       }
 #pragma unroll
@@ -181,12 +187,12 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
         s *= inv;
       }
       const uint32_t c = pack8(v, s);
-      if (inside) *reinterpret_cast<uint32_t*>(codes + i * 1024) = byte == 255u ? 0u : c;
+      if (inside) *reinterpret_cast<uint32_t*>(codes + i * NT * 4) = byte == 255u ? 0u : c;
       // a block's lanes hold its byte alike; the first stores it
-      if ((lane & 3) == 0) scales[i * 8 * 1024] = (uint8_t)byte;
+      if ((lane & 3) == 0) scales[i * (NT / 32) * 1024] = (uint8_t)byte;
       if (OUT && inside) {
         float f[8];
-        unpack8(xs[i * 256], f);
+        unpack8(xs[i * NT], f);
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -194,7 +200,7 @@ __global__ void __launch_bounds__(256, norm_ctas(VPT))
           o[j] = pack_bf16x2(__bfloat162float(__float2bfloat16_rn(f[2 * j] * inv)) * f32x2_lo(gj),
                              __bfloat162float(__float2bfloat16_rn(f[2 * j + 1] * inv)) * f32x2_hi(gj));
         }
-        reinterpret_cast<uint4*>(out + (int64_t)r * ldo)[tid + i * 256] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(out + (int64_t)r * ldo)[tid + i * NT] = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     slot = slot + 1 == STAGES ? 0 : slot + 1;
@@ -345,20 +351,20 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   auto st = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   auto* xp = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
-  const int vpt = (int)((f4::k_tiles(H) * 16 + 255) / 256);
-  auto go = [&](auto kernel, int v) {
-    const int smem = f4::norm_stages(v) * v * 256 * 16;
+  const int vectors = (int)f4::k_tiles(H) * 16;  // with those that pad the row to 256 columns
+  auto go = [&](auto kernel, int nt, int v) {
+    const int smem = f4::norm_stages(v) * v * nt * 16;
     if (smem > 48 * 1024)  // per device and cheap: no cache
       GSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const int64_t ctas = std::min<int64_t>(M, (int64_t)f4::norm_ctas(v) * f4::kSms);
-    f4::launch(kernel, dim3((unsigned)ctas), 256, smem, 1, st, xp, (int)x.stride(0), wp, (int)M, (int)H, (float)eps,
+    const int64_t ctas = std::min<int64_t>(M, (int64_t)f4::norm_ctas(v, nt) * f4::kSms);
+    f4::launch(kernel, dim3((unsigned)ctas), nt, smem, 1, st, xp, (int)x.stride(0), wp, (int)M, (int)H, (float)eps,
                x4.data_ptr<uint8_t>(), (int)x4.stride(0), sf.data_ptr<uint8_t>(), op, (int)ldo);
   };
-  auto pick = [&](auto plain, auto with_out, int v) { op == nullptr ? go(plain, v) : go(with_out, v); };
-  if (vpt <= 1) pick(f4::rmsnorm_mxfp4_kernel<1, false>, f4::rmsnorm_mxfp4_kernel<1, true>, 1);
-  else if (vpt <= 2) pick(f4::rmsnorm_mxfp4_kernel<2, false>, f4::rmsnorm_mxfp4_kernel<2, true>, 2);
-  else if (vpt <= 4) pick(f4::rmsnorm_mxfp4_kernel<4, false>, f4::rmsnorm_mxfp4_kernel<4, true>, 4);
-  else pick(f4::rmsnorm_mxfp4_kernel<8, false>, f4::rmsnorm_mxfp4_kernel<8, true>, 8);
+  auto pick = [&](auto plain, auto with_out, int nt, int v) { op == nullptr ? go(plain, nt, v) : go(with_out, nt, v); };
+  if (vectors <= 256) pick(f4::rmsnorm_mxfp4_kernel<128, 2, false>, f4::rmsnorm_mxfp4_kernel<128, 2, true>, 128, 2);
+  else if (vectors <= 512) pick(f4::rmsnorm_mxfp4_kernel<128, 4, false>, f4::rmsnorm_mxfp4_kernel<128, 4, true>, 128, 4);
+  else if (vectors <= 1024) pick(f4::rmsnorm_mxfp4_kernel<256, 4, false>, f4::rmsnorm_mxfp4_kernel<256, 4, true>, 256, 4);
+  else pick(f4::rmsnorm_mxfp4_kernel<256, 8, false>, f4::rmsnorm_mxfp4_kernel<256, 8, true>, 256, 8);
   return {x4, sf};
 }
 
