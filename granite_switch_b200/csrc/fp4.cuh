@@ -28,7 +28,7 @@ constexpr int kBlock = 32;
 
 __host__ __device__ constexpr int64_t k_tiles(int64_t K) { return (K + 255) / 256 * 2; }
 
-// Scale byte of a block whose largest magnitude has the fp32 bits `amax` (sign clear).
+// Scale byte of a block whose largest magnitude has the fp32 bits `amax` (sign clear, or a NaN's).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
   // 7 = 1.75 * 2^2: the exponent less two, one more when the mantissa is above 1.75 (the sum
   // then carries into the exponent)
@@ -37,10 +37,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
   return amax >= 0x7f800000u ? 255u : byte;
 }
 
-// 2^-e of a scale byte, exact for 0..252; 0 for 255 (the codes of such a block are 0).
-__device__ __forceinline__ float inv_scale(uint32_t byte) {
-  return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
-}
+// 2^-e of a scale byte, exact for 0..252. For 255 it means nothing: the caller stores codes of 0.
+__device__ __forceinline__ float inv_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
 // 2^e of a scale byte: 2^-127 is a subnormal, 255 is NaN.
 __device__ __forceinline__ float scale_value(uint32_t byte) {

@@ -873,13 +873,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
               o[g] = make_uint4(pack_bf16x2(v[g][0], v[g][1]), pack_bf16x2(v[g][2], v[g][3]),
                                 pack_bf16x2(v[g][4], v[g][5]), pack_bf16x2(v[g][6], v[g][7]));
           }
-          if (byte == 255u) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j / 8][j % 8] = 0.f;
-          }
           const float inv = inv_scale(byte);
+          const uint32_t keep = byte == 255u ? 0u : ~0u;
           *reinterpret_cast<uint4*>(p.a4 + (int64_t)row * p.lda4 + col / 2 + 16 * b) =
-              make_uint4(pack8(v[0], inv), pack8(v[1], inv), pack8(v[2], inv), pack8(v[3], inv));
+              make_uint4(pack8(v[0], inv) & keep, pack8(v[1], inv) & keep, pack8(v[2], inv) & keep,
+                         pack8(v[3], inv) & keep);
         }
         if (row < p.M) {
           *reinterpret_cast<uint16_t*>(p.sfa_out + sf_word(row, col >> 7, kt) + ((col >> 5) & 3)) = (uint16_t)bytes;

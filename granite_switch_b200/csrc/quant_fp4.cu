@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(NT, norm_ctas(VPT, NT))
     for (int i = 0; i < VPT; ++i) {
       if ((tid >> 5) + i * (NT / 32) >= units) break;  // the whole warp
       const bool inside = tid + i * NT < nvec;
-      uint32_t byte = scale_byte(__float_as_uint(__uint_as_float(top[i]) * inv) & 0x7fffffffu);
+      uint32_t byte = scale_byte(__float_as_uint(__uint_as_float(top[i]) * inv));
       byte = inside ? byte : 0u;  // past the row (whole blocks): inv is NaN in a row that is not finite
       float s = inv_scale(byte);
       uint64_t v[4], g[4];

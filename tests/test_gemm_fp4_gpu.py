@@ -389,6 +389,34 @@ def test_nan_and_empty():
     assert a4.shape == (0, 64)
 
 
+def _check_swiglu_not_finite(m):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(m, 256, seed=51, spread=1)
+    b = F.quantize_rows_mxfp4(_rows(384, 256, seed=52, spread=1))
+    clean = F.mxfp4_gemm_swiglu(*F.quantize_rows_mxfp4(x), *b)
+    x[2, 7] = float("nan")
+    x[m - 1, 200] = float("-inf")
+    act = torch.empty(m, 192, dtype=torch.bfloat16, device="cuda")
+    a4, sf = F.mxfp4_gemm_swiglu(*F.quantize_rows_mxfp4(x), *b, act=act)
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[2] = bad[m - 1] = True
+    got, want = (F.scale_bytes_from_atoms(t, m, 192) for t in (sf, clean[1]))
+    assert (a4[bad] == 0).all() and (got[bad] == 255).all() and act[bad].isnan().all()
+    assert torch.equal(a4[~bad], clean[0][~bad]) and torch.equal(got[~bad], want[~bad]) and act[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_swiglu_rows_that_are_not_finite(m):
+    """A NaN or infinity in a row makes its blocks' scales NaN and their codes 0, and leaves the other rows alone."""
+    _check_swiglu_not_finite(m)
+
+
+@pytest.mark.parametrize("m", [5, 300])
+def test_pair_swiglu_rows_that_are_not_finite(pair_always, m):
+    _check_swiglu_not_finite(m)
+
+
 def test_output_past_32_bits():
     from granite_switch_b200.ops import gemm_fp4 as F
 
