@@ -7,7 +7,7 @@
 //   rmsnorm_mxfp4: the row in registers between the sum of squares and the conversion.
 //     y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then one rounding, to
 //     4 bits; with `out` the row also leaves as bf16, rounded exactly as the RMSNorm kernel does,
-//     for the LoRA shrink. 8192 x 4096 rows: 19.4 us, 4.4 TB/s, bound by instruction issue (2.75 of
+//     for the LoRA shrink. 8192 x 4096 rows: 19.1 us, 4.4 TB/s, bound by instruction issue (2.75 of
 //     4 a cycle: unpacking, squares, products, maxima and conversions of every value).
 //   dequantize_mxfp4: codes times scale, exact in bf16. 8192 x 12800 rows: 42 us, 6.4 TB/s.
 #include "common.cuh"
@@ -70,7 +70,7 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {  // NaN i
 
 // The norm kernel's NT threads hold VPT 16-byte vectors of a row each. Up to 4096 columns 128 threads
 // share a row's fixed instructions among more values than 256 would (8192 x 4096 19.4 against 21.2 us,
-// 8192 x 2048 12.2 against 14.5, 16 x 4096 1.73 against 1.65). Rows in flight per CTA, and resident
+// 8192 x 2048 12.2 against 14.5, 16 x 4096 1.70 against 1.65). Rows in flight per CTA, and resident
 // CTAs per SM (what the registers allow without spills):
 __host__ __device__ constexpr int norm_stages(int vpt) { return vpt <= 4 ? 4 : 2; }
 __host__ __device__ constexpr int norm_ctas(int vpt, int nt) { return nt == 256 ? 2 : (vpt <= 2 ? 8 : 5); }
