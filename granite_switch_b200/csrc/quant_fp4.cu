@@ -2,8 +2,8 @@
 // (format: fp4.cuh). All three stream their rows once.
 //
 //   quantize_mxfp4: a warp takes 256 neighbours of a row, eight per lane (one 16-byte
-//     load), so a block of 32 is four lanes and its maximum two shuffles; four such units are
-//     in flight per warp. 8192 x 12800 rows: 45 us, 5.9 TB/s, 0.91 of the measured copy.
+//     load), so a block of 32 is four lanes and its maximum two shuffles; one, two or four such
+//     units are in flight per warp. 8192 x 12800 rows: 45 us, 5.9 TB/s, 0.91 of the measured copy.
 //   rmsnorm_mxfp4: the row in registers between the sum of squares and the conversion.
 //     y = x w / sqrt(mean(x^2) + eps) in fp32 (the product x w is exact), then one rounding, to
 //     4 bits; with `out` the row also leaves as bf16, rounded exactly as the RMSNorm kernel does,
@@ -28,9 +28,9 @@ namespace f4 {
 
 constexpr int kSms = 148;
 constexpr int kQuantThreads = 256;
-constexpr int kUnits = 4;  // 256-value units of one row in flight per warp
 
-// Warp `blockIdx.x * 8 + ..` takes `kUnits` units of one row; `per_row` warps make a row.
+// Warp `blockIdx.x * 8 + ..` takes UNITS units of one row; `per_row` warps make a row.
+template <int UNITS>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int K, int k2s, uint32_t per_row,
                           uint32_t warps, uint8_t* __restrict__ x4, int64_t ld4, uint8_t* __restrict__ sf) {
@@ -40,11 +40,11 @@ __global__ void __launch_bounds__(kQuantThreads)
   const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   if (warp >= warps) return;
   const uint32_t row = warp / per_row;
-  const int first = (int)(warp - row * per_row) * kUnits;
+  const int first = (int)(warp - row * per_row) * UNITS;
   const __nv_bfloat16* xr = x + row * ldx + lane * 8;
-  uint4 q[kUnits];
+  uint4 q[UNITS];
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
+  for (int u = 0; u < UNITS; ++u) {
     const int k = (first + u) * 256;
     q[u] = make_uint4(0u, 0u, 0u, 0u);
     if (k + lane * 8 < K) q[u] = *reinterpret_cast<const uint4*>(xr + k);
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kQuantThreads)
   uint8_t* xo = x4 + row * ld4 + lane * 4;
   uint8_t* so = sf + sf_word(row, 2 * first, 2 * k2s);
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
+  for (int u = 0; u < UNITS; ++u) {
     const int k2 = first + u, k = k2 * 256 + lane * 8;
     if (k2 >= k2s) break;  // the whole warp
     uint32_t codes;
@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(NT, norm_ctas(VPT, NT))
   }
 }
 
+template <int UNITS>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_mxfp4_kernel(const uint8_t* __restrict__ x4, int64_t ld4, const uint8_t* __restrict__ sf, int K,
                             int k2s, uint32_t per_row, uint32_t warps, __nv_bfloat16* __restrict__ out, int64_t ldo) {
@@ -217,11 +218,11 @@ __global__ void __launch_bounds__(kQuantThreads)
   const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   if (warp >= warps) return;
   const uint32_t row = warp / per_row;
-  const int first = (int)(warp - row * per_row) * kUnits;
+  const int first = (int)(warp - row * per_row) * UNITS;
   const uint8_t* xi = x4 + row * ld4 + lane * 4;
-  uint32_t c[kUnits], b[kUnits];
+  uint32_t c[UNITS], b[UNITS];
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
+  for (int u = 0; u < UNITS; ++u) {
     const int k2 = first + u;
     c[u] = b[u] = 0u;
     if (k2 * 256 + lane * 8 < K) {
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kQuantThreads)
   }
   __nv_bfloat16* oo = out + row * ldo + lane * 8;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
+  for (int u = 0; u < UNITS; ++u) {
     const int k = (first + u) * 256;
     if (k + lane * 8 >= K) continue;
     const float s = scale_value(b[u]);
@@ -268,15 +269,23 @@ void check_rows(const char* op, const char* what, const at::Tensor& x, const at:
             op, ": K must be a positive multiple of 32");
 }
 
-// Warps per row and in all, and the grid, of the streaming kernels.
-struct StreamGrid {
+// How a streaming kernel covers [M, K]: units of 256 values per warp, warps per row and in all, CTAs.
+struct StreamPlan {
+  int units;
   uint32_t per_row, warps;
   dim3 grid;
 };
-static StreamGrid stream_grid(const char* op, int64_t M, int64_t K) {
-  const int64_t per_row = (k_tiles(K) / 2 + kUnits - 1) / kUnits, warps = M * per_row;
+// Many rows are bound by memory, and four units a warp keep enough loads in flight; few are bound by
+// one warp's chain of loads, shuffles and stores, which more and shorter warps take at once. us with
+// 1 / 2 / 4 units, quantising: 16 x 4096 1.24 / 1.40 / 1.66, 1003 x 2080 2.4 / 3.0 / 3.1, 1537 x 2048 3.4 /
+// 3.5 / 3.6, 1024 x 4096 4.0 / 3.5 / 4.3, 2048 x 4096 6.9 / 5.5 / 5.5, 8192 x 4096 22.5 / 17.5 / 15.7.
+static StreamPlan stream_plan(const char* op, int64_t M, int64_t K) {
+  const int64_t row_units = k_tiles(K) / 2, all = M * row_units;
+  const int units = all <= 12800 ? 1 : (all <= 32000 ? 2 : 4);
+  const int64_t per_row = (row_units + units - 1) / units, warps = M * per_row;
   GSB_CHECK(warps < (int64_t(1) << 32) - 64, op, ": too many rows");
-  return {(uint32_t)per_row, (uint32_t)warps, dim3((unsigned)((warps + kQuantThreads / 32 - 1) / (kQuantThreads / 32)))};
+  return {units, (uint32_t)per_row, (uint32_t)warps,
+          dim3((unsigned)((warps + kQuantThreads / 32 - 1) / (kQuantThreads / 32)))};
 }
 
 void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at::Tensor& sf) {
@@ -297,9 +306,12 @@ void make_codes(int64_t M, int64_t K, const at::Device& dev, at::Tensor& x4, at:
 
 void quantize_launch(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* x4, int64_t ld4, uint8_t* sf,
                      cudaStream_t st) {
-  const StreamGrid g = stream_grid("quantize_mxfp4", M, K);
-  launch(quantize_mxfp4_kernel, g.grid, kQuantThreads, 0, 1, st, reinterpret_cast<const __nv_bfloat16*>(x), ldx,
-         (int)K, (int)(k_tiles(K) / 2), g.per_row, g.warps, x4, ld4, sf);
+  const StreamPlan g = stream_plan("quantize_mxfp4", M, K);
+  const auto kernel = g.units == 1   ? quantize_mxfp4_kernel<1>
+                      : g.units == 2 ? quantize_mxfp4_kernel<2>
+                                     : quantize_mxfp4_kernel<4>;
+  launch(kernel, g.grid, kQuantThreads, 0, 1, st, reinterpret_cast<const __nv_bfloat16*>(x), ldx, (int)K,
+         (int)(k_tiles(K) / 2), g.per_row, g.warps, x4, ld4, sf);
 }
 
 }  // namespace f4
@@ -380,8 +392,11 @@ at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, cons
             "dequantize_mxfp4: out must be [M, K] with rows of their own");
   f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
   if (M == 0) return out;
-  const f4::StreamGrid s = f4::stream_grid("dequantize_mxfp4", M, K);
-  f4::launch(f4::dequantize_mxfp4_kernel, s.grid, f4::kQuantThreads, 0, 1,
+  const f4::StreamPlan s = f4::stream_plan("dequantize_mxfp4", M, K);
+  const auto kernel = s.units == 1   ? f4::dequantize_mxfp4_kernel<1>
+                      : s.units == 2 ? f4::dequantize_mxfp4_kernel<2>
+                                     : f4::dequantize_mxfp4_kernel<4>;
+  f4::launch(kernel, s.grid, f4::kQuantThreads, 0, 1,
              c10::cuda::getCurrentCUDAStream(x4.device().index()).stream(), x4.data_ptr<uint8_t>(), x4.stride(0),
              sf.data_ptr<uint8_t>(), (int)K, (int)(f4::k_tiles(K) / 2), s.per_row, s.warps,
              reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), out.stride(0));
