@@ -87,6 +87,22 @@ def test_quantize_matches_reference(m, k):
     assert torch.equal(F.dequantize_mxfp4(x4, sf).double(), F.dequantize_reference(r4, rsf))
 
 
+@pytest.mark.parametrize("m,k", [(700, 8736), (1003, 4640), (1800, 4640), (2000, 4608), (2500, 4128), (4100, 2080)])
+def test_quantize_many_rows(m, k):
+    """Sizes at which a warp takes two or four units of a row, with rows that end inside a warp's units."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(m, k, seed=m + k)
+    x4, sf = F.quantize_rows_mxfp4(x)
+    r4, rsf = F.quantize_rows_reference(x)
+    assert torch.equal(x4, r4)
+    kt = sf.shape[1] * 128
+    assert torch.equal(F.scale_bytes_from_atoms(sf, m, kt), F.scale_bytes_from_atoms(rsf, m, kt))
+    out = torch.full((m + 1, k), 5.0, dtype=torch.bfloat16, device="cuda")
+    F.dequantize_mxfp4(x4, sf, out[:m])
+    assert torch.equal(out[:m].double(), F.dequantize_reference(r4, rsf)) and (out[m:] == 5.0).all()
+
+
 def test_quantize_edges_and_strides():
     """Zeros, subnormals, the largest bf16, borders, infinities and NaN; rows wider than their K; a caller's buffers
     with rows behind the last one left alone."""
