@@ -37,6 +37,7 @@ struct DecodeGemmArgs {
   int64_t ldx;
   const void* w;
   int64_t ldw;
+  bool w_constant;      // w was written long ago: it may be read before the kernels ahead have ended
   void* out;            // bf16 output, or the multicast address (kEpiMultimemRed)
   int64_t ldo;
   int M, N, K;

@@ -72,6 +72,7 @@ struct Params {
   int kblocks;       // K / 64
   int stages;        // ring stages (runtime: stage size follows Mp)
   int stage_bytes;   // ACC * 16 KB of W, then the token rows of the k block
+  int early_w;       // weight tiles may be read before the dependency wait
   float scale;
   void* out;
   int64_t ldo;
@@ -302,11 +303,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto load_x_main = [&](int i, int s) {
     tma_load_2d(smem + s * p.stage_bytes + w_bytes, &tm_x, &full_bar[s], (kb_lo + i) * BK, 0);
   };
-  // Weights are constant: the producer puts the weight tiles of its first ring's worth
-  // of main blocks in flight before it waits for the previous kernel (launched as its
-  // programmatic dependent, this kernel may start while that one still runs). Every
-  // thread waits before it reads the step's activations or adapter masks.
-  const int prefetch = (warp == 0 && lane == 0) ? min(stages, n_main) : 0;
+  // Where the caller says that the weights are constant, the producer puts the weight tiles
+  // of its first ring's worth of main blocks in flight before it waits for the previous
+  // kernel (launched as its programmatic dependent, this kernel may start while that one
+  // still runs). Every thread waits before it reads anything else.
+  const int prefetch = (p.early_w && warp == 0 && lane == 0) ? min(stages, n_main) : 0;
   for (int i = 0; i < prefetch; ++i) load_w_main(i, i);  // fresh ring: no empty-slot wait
   griddep_wait();
   const uint64_t amask = (EPI != kEpiMaskAdapter && p.lora) ? present_adapters(p) : 0ull;
@@ -511,7 +512,7 @@ static int dec_num_sms() {
 
 template <int ACC, int EPI>
 static void launch_decode(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tlb,
-                          const CUtensorMap& ts, const dec::Params& p, int n_tiles, uint32_t* err,
+                          const CUtensorMap& ts, dec::Params p, int n_tiles, uint32_t* err,
                           cudaStream_t stream) {
   auto kfn = dec::decode_gemm_kernel<ACC, EPI>;
   static bool configured = false;  // per instantiation
@@ -539,6 +540,8 @@ static void launch_decode(const CUtensorMap& tw, const CUtensorMap& tx, const CU
     attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
     ++n_attr;
+  } else {
+    p.early_w = 1;  // in plain stream order whatever writes them has ended
   }
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
@@ -660,6 +663,7 @@ bool decode_gemm_try(const DecodeGemmArgs& a, uint32_t* err, cudaStream_t stream
   p.Mp = (a.M + 15) / 16 * 16;
   p.Mp_pad = (p.Mp + 31) / 32 * 32;
   p.kblocks = a.K / 64;
+  p.early_w = a.w_constant;
   p.scale = a.scale;
   p.out = a.out;
   p.ldo = a.ldo;

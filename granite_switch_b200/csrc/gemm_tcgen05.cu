@@ -1052,6 +1052,7 @@ static int splitk_parts(int tiles, int kblocks, int nsms) {
 // x [M, K] bf16, w [N, K] bf16 (both row-major, K contiguous).
 // LoRA (optional): s [M, Ks] bf16 masked shrink output, lb [N, NA*rank] bf16
 // packed expand weights, tile_mask [ceil(M/128)] int64 adapter bitmask.
+// w_constant: no kernel ahead in the stream writes w.
 void gsb_switched_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& out,
                        int64_t epi_kind, int64_t bn, const c10::optional<at::Tensor>& residual,
                        double scale, const c10::optional<at::Tensor>& s,
@@ -1060,7 +1061,7 @@ void gsb_switched_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tenso
                        int64_t num_adapters, std::vector<int64_t> slice_bounds,
                        const c10::optional<at::Tensor>& row_adapter, int64_t mask_rank,
                        int64_t mask_num_adapters, const at::Tensor& err, int64_t mc_out,
-                       const c10::optional<at::Tensor>& tile_expert) {
+                       const c10::optional<at::Tensor>& tile_expert, bool w_constant) {
   using namespace gsb;
   GSB_CHECK(x.is_cuda() && w.is_cuda() && out.is_cuda(), "tensors must be on CUDA");
   GSB_CHECK(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16,
@@ -1190,6 +1191,7 @@ void gsb_switched_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tenso
     d.ldx = x.stride(0);
     d.w = w.data_ptr();
     d.ldw = w.stride(0);
+    d.w_constant = w_constant;
     d.out = epi.out;
     d.ldo = epi.ldo;
     d.M = M;

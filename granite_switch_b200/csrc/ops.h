@@ -15,7 +15,7 @@ void gsb_switched_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tenso
                        int64_t num_adapters, std::vector<int64_t> slice_bounds,
                        const c10::optional<at::Tensor>& row_adapter, int64_t mask_rank,
                        int64_t mask_num_adapters, const at::Tensor& err, int64_t mc_out,
-                       const c10::optional<at::Tensor>& tile_expert);
+                       const c10::optional<at::Tensor>& tile_expert, bool w_constant);
 
 int64_t gsb_gemm_pair_min_m(int64_t m);
 int64_t gsb_gemm_decode_max_m(int64_t v);

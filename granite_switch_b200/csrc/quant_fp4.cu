@@ -212,7 +212,8 @@ template <int UNITS>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_mxfp4_kernel(const uint8_t* __restrict__ x4, int64_t ld4, const uint8_t* __restrict__ sf, int K,
                             int k2s, uint32_t per_row, uint32_t warps, __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  griddep_launch();
+  // No early griddep_launch(): the rows may be the next product's weights, which the decode GEMM
+  // reads before it waits for the kernel ahead of it (and for any kernel that one lets run on).
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const uint32_t warp = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);

@@ -533,9 +533,10 @@ class NativeGraniteSwitch:
             G.switched_gemm(x, w, out, epi=epi, residual=residual, scale=scale, s=s, lb=lb, tile_mask=tm,
                             rank=pl.rank, num_adapters=pl.n_local,
                             slice_bounds=[0, pl.n] if epi == G.EPI_SWIGLU else bounds, bn=bn,
-                            mc_out=mc_out)
+                            mc_out=mc_out, w_constant=True)
         else:
-            G.switched_gemm(x, w, out, epi=epi, residual=residual, scale=scale, bn=bn, mc_out=mc_out)
+            G.switched_gemm(x, w, out, epi=epi, residual=residual, scale=scale, bn=bn, mc_out=mc_out,
+                            w_constant=True)
         return out
 
     def _row_parallel(self, pl: PackedLinear, x: torch.Tensor, h: torch.Tensor, mult: float, lora: bool = True,
@@ -566,7 +567,7 @@ class NativeGraniteSwitch:
         ra = self.row_adapter[pl.map_id, :m]
         s = self.s_buf[:m, : pl.a_all.shape[0]]
         G.lora_shrink(hbase, pl.a_all, ra, pl.rank, pl.n_local, out=s)
-        G.switched_gemm(s, pl.lb, h, epi=G.EPI_RESADD, residual=h, scale=1.0)
+        G.switched_gemm(s, pl.lb, h, epi=G.EPI_RESADD, residual=h, scale=1.0, w_constant=True)
 
     def _mlp(self, lw: LayerWeights, x: torch.Tensor, act: torch.Tensor, h: torch.Tensor, mult: float,
              lora: bool = True, reuse_routing: bool = False, partial: torch.Tensor | None = None, xq=None) -> None:

@@ -64,9 +64,14 @@ def switched_gemm(
     bn: int | None = None,
     mc_out: int = 0,
     tile_expert: torch.Tensor | None = None,
+    w_constant: bool = False,
 ) -> torch.Tensor:
     """``tile_expert`` selects grouped mode: ``w`` is a stack ``[E, N, K]`` and
-    128-row tile ``t`` of ``x`` multiplies expert ``tile_expert[t]`` (-1: skipped)."""
+    128-row tile ``t`` of ``x`` multiplies expert ``tile_expert[t]`` (-1: skipped).
+
+    ``w_constant=True`` says that no kernel still in flight writes ``w`` (a model's weights):
+    under programmatic launch a decode-sized product then streams its first weight tiles
+    before the kernels ahead of it in the stream have ended."""
     m, _ = x.shape
     n = w.shape[-2]
     if out is None:
@@ -84,7 +89,7 @@ def switched_gemm(
     native().switched_gemm(
         x, w, out, epi, bn, residual, float(scale), s, lb, tile_mask, rank, num_adapters,
         list(slice_bounds) if slice_bounds is not None else [0, n], row_adapter, mask_rank,
-        mask_num_adapters, err_buffer(x.device), int(mc_out), tile_expert,
+        mask_num_adapters, err_buffer(x.device), int(mc_out), tile_expert, bool(w_constant),
     )
     return out
 

@@ -535,3 +535,87 @@ def test_refusals():
         with pytest.raises((RuntimeError, ValueError)):
             call()
             pytest.fail(f"call {i} was accepted")
+
+
+@pytest.mark.parametrize("between", [False, True])
+@pytest.mark.parametrize("source", ["dequantise", "product", "norm", "swiglu"])
+def test_outputs_as_weights_of_the_next_product(source, between):
+    """Rows that an MXFP4 kernel has just written are the weights of a decode-sized bf16 product, once directly and
+    once with a quantiser launched in between, under programmatic launch, eagerly and replayed from a graph: the
+    product of the new rows, as in plain stream order. (Three sets of rows go through one buffer.)"""
+    from granite_switch_b200._native import native
+    from granite_switch_b200.ops import gemm as G
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    n = k = 4096
+    x = _rows(16, k, seed=61, spread=1)
+    rows = [_rows(n, k if source in ("dequantise", "norm") else 512, seed=62 + i, spread=1) for i in range(3)]
+    codes = [F.quantize_rows_mxfp4(r) for r in rows]
+    b = F.quantize_rows_mxfp4(_rows(k if source == "product" else 2 * k, 512, seed=66, spread=1))
+    ones = torch.ones(k, device="cuda").bfloat16()
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+    write = dict(dequantise=lambda i: F.dequantize_mxfp4(*codes[i], out=w),
+                 product=lambda i: F.mxfp4_gemm(*codes[i], *b, w),
+                 norm=lambda i: F.rmsnorm_mxfp4(rows[i], ones, 1e-5, out=w),
+                 swiglu=lambda i: F.mxfp4_gemm_swiglu(*codes[i], *b, act=w))[source]
+    assert native().gemm_decode_plan(16, n, k, G.EPI_STORE, 0)[0] > 0  # the kernel that can read weights early
+
+    def chain():
+        outs = []
+        for i in range(3):
+            write(i)
+            if between:
+                F.quantize_rows_mxfp4(x)
+            outs.append(G.switched_gemm(x, w))
+        return outs
+
+    old = native().set_pdl(False)
+    try:
+        want = chain()
+        torch.cuda.synchronize()
+        native().set_pdl(True)
+        eager = [chain() for _ in range(5)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = chain()
+        replayed = []
+        for _ in range(5):
+            for t in captured:
+                t.zero_()
+            graph.replay()
+            replayed.append([t.clone() for t in captured])
+        torch.cuda.synchronize()
+        del graph
+    finally:
+        native().set_pdl(old)
+    for got in eager + replayed:
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("m", [16, 222])
+def test_constant_weights_match(m):
+    """``w_constant`` changes when a decode-sized product starts reading, not its bits."""
+    from granite_switch_b200._native import native
+    from granite_switch_b200.ops import elementwise as E
+    from granite_switch_b200.ops import gemm as G
+
+    h, w = _rows(m, 4096, seed=67, spread=1), _rows(4096, 4096, seed=68, spread=1)
+    gu = _rows(2048, 4096, seed=69, spread=1)
+    ones = torch.ones(4096, device="cuda").bfloat16()
+
+    def chain(constant):
+        x = E.rmsnorm(h, ones, 1e-5)
+        y = G.switched_gemm(x, w, epi=G.EPI_RESADD, residual=h, scale=0.5, w_constant=constant)
+        return y, G.switched_gemm(E.rmsnorm(y, ones, 1e-5), gu, epi=G.EPI_SWIGLU, bn=128, w_constant=constant)
+
+    old = native().set_pdl(False)
+    try:
+        want = chain(False)
+        torch.cuda.synchronize()
+        native().set_pdl(True)
+        got = [chain(c) for c in (False, True) * 5]
+        torch.cuda.synchronize()
+    finally:
+        native().set_pdl(old)
+    for pair in got:
+        assert all(torch.equal(a, c) for a, c in zip(pair, want))
