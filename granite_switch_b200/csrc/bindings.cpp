@@ -11,18 +11,20 @@
 namespace gsb {
 static std::atomic<int64_t> g_kernel_launches{0};
 void count_launch() { g_kernel_launches.fetch_add(1, std::memory_order_relaxed); }
-static std::atomic<bool> g_pdl{false};
-bool pdl_enabled() { return g_pdl.load(std::memory_order_relaxed); }
+static std::atomic<int64_t> g_pdl{-1};
+bool pdl_enabled() { return g_pdl.load(std::memory_order_relaxed) == 1; }
+bool pdl_allowed() { return g_pdl.load(std::memory_order_relaxed) != 0; }
 }  // namespace gsb
 
-static bool gsb_set_pdl(bool on) { return gsb::g_pdl.exchange(on); }
+static int64_t gsb_set_pdl(int64_t mode) { return gsb::g_pdl.exchange(mode > 0 ? 1 : (mode < 0 ? -1 : 0)); }
 
 static int64_t gsb_kernel_launches() { return gsb::g_kernel_launches.load(std::memory_order_relaxed); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kernel_launches", &gsb_kernel_launches, "kernels launched by this extension since it was loaded");
   m.def("set_pdl", &gsb_set_pdl,
-        "launch the GEMMs as programmatic dependents of the kernel before them (returns the old setting)");
+        "programmatic dependent launch: 1 every kernel that supports it, 0 none, -1 (as loaded) the MXFP4 kernels only "
+        "(returns the old setting)");
   m.doc() = "granite_switch_b200 sm_100a kernels";
   m.def("switched_gemm", &gsb_switched_gemm, "tcgen05 GEMM with fused switched-LoRA expand");
   m.def("gemm_pair_min_m", &gsb_gemm_pair_min_m, "set the smallest M of the CTA-pair GEMM (returns the old value)");

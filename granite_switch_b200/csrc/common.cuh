@@ -460,6 +460,8 @@ void count_launch();
 // Whether kernels that support it are launched as programmatic dependents of the
 // kernel before them (griddep_wait / griddep_launch); set_pdl() in bindings.cpp.
 bool pdl_enabled();
+// The same for kernels that are launched so unless it was turned off.
+bool pdl_allowed();
 
 // Merge of split-KV attention partials (attention.cu) for the rows of the given
 // work tiles: ws_o [nsplit][T][Hq][D] normalised fp32, ws_lse [nsplit][T][Hq] log2.

@@ -20,8 +20,8 @@ inline at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const a
 
 inline bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
-// Launches an MXFP4 kernel with `cluster` CTAs a cluster (1: none, or compiled in), always as a
-// programmatic dependent of the kernel before it in the stream: before they wait for that one
+// Launches an MXFP4 kernel with `cluster` CTAs a cluster (1: none, or compiled in), unless set_pdl(0) turned
+// that off as a programmatic dependent of the kernel before it in the stream: before they wait for that one
 // (griddep_wait), these kernels touch their own shared and tensor memory only and prefetch
 // weights into L2, which reads nothing that could be stale. It saves 1 to 2 us a launch.
 template <typename... KArgs, typename... Args>
@@ -34,7 +34,7 @@ inline void launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, i
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)cluster;
   attr[1].val.clusterDim.y = 1;

@@ -41,6 +41,7 @@ inline std::string gsb_str(const Ts&... vs) {
   } while (0)
 
 bool pdl_enabled();
+bool pdl_allowed();
 void count_launch();
 
 // Launches `kernel` as a programmatic dependent of the kernel before it in `st` when

@@ -59,7 +59,8 @@ class EngineConfig:
     # pipeline parallelism: run each step as two micro-batches so consecutive stages overlap
     pipeline_microbatches: bool = True
     # launch the decode-sized GEMMs as programmatic dependents of the kernel before them:
-    # they set up and start streaming weights while that kernel finishes (process-wide)
+    # they set up and start streaming weights while that kernel finishes (process-wide;
+    # False turns it off for the MXFP4 kernels too, which start so by default)
     programmatic_launch: bool = True
     # a step with decode rows and prefill chunks runs the prefill attention on a second
     # stream beside the decode attention

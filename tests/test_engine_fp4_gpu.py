@@ -199,3 +199,23 @@ def test_parallel_models_are_refused():
         NativeGraniteSwitch(None, torch.device("cuda", 0), 64, 8, tp_size=2, weight_dtype="mxfp4")
     with pytest.raises(ValueError, match="weight_dtype"):
         NativeGraniteSwitch(None, torch.device("cuda", 0), 64, 8, weight_dtype="int4")
+
+
+@pytest.mark.parametrize("on", [False, True])
+def test_programmatic_launch_switch_reaches_the_kernels(on):
+    """An engine with 4-bit projections sets the launch kind of every kernel, the MXFP4 ones included."""
+    from granite_switch_b200._native import native
+    from granite_switch_b200.composer.synthetic import base_config
+    from granite_switch_b200.config import GraniteSwitchConfig
+    from granite_switch_b200.engine import LLM, EngineConfig, SamplingParams
+
+    old = native().set_pdl(-1)
+    try:
+        llm = LLM(GraniteSwitchConfig(**base_config("tiny")), device="cuda:0",
+                  engine_config=EngineConfig(max_num_seqs=2, max_num_batched_tokens=64, num_kv_blocks=32,
+                                             max_model_len=128, weight_dtype="mxfp4", programmatic_launch=on),
+                  random_init={})
+        assert len(llm.generate([[5, 6, 7]], SamplingParams(max_tokens=2))[0].output_ids) == 2
+        assert native().set_pdl(1) == int(on)
+    finally:
+        native().set_pdl(old)

@@ -619,3 +619,45 @@ def test_constant_weights_match(m):
         native().set_pdl(old)
     for pair in got:
         assert all(torch.equal(a, c) for a, c in zip(pair, want))
+
+
+def _programmatic_edges(graph):
+    """(programmatic dependencies, all dependencies) of a captured graph."""
+    import ctypes
+
+    rt = ctypes.CDLL("libcudart.so.12")
+    raw, n = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert rt.cudaGraphGetEdges_v2(raw, None, None, None, ctypes.byref(n)) == 0
+    src, dst = (ctypes.c_void_p * n.value)(), (ctypes.c_void_p * n.value)()
+    data = (ctypes.c_uint8 * (8 * n.value))()  # per edge: from port, to port, type, five reserved bytes
+    assert rt.cudaGraphGetEdges_v2(raw, src, dst, data, ctypes.byref(n)) == 0
+    return sum(data[8 * i + 2] == 1 for i in range(n.value)), n.value
+
+
+def test_programmatic_launch_can_be_turned_off():
+    """The MXFP4 kernels start as programmatic dependents as the extension is loaded and with set_pdl(1), and in
+    plain stream order with set_pdl(0); their results are the same."""
+    from granite_switch_b200._native import native
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    x = _rows(64, 1024, seed=71, spread=1)
+    w = torch.ones(1024, device="cuda").bfloat16()
+    b = F.quantize_rows_mxfp4(_rows(1024, 1024, seed=72, spread=1))
+    outs = []
+    for mode in (-1, 0, 1):
+        old = native().set_pdl(mode)
+        try:
+            graph = torch.cuda.CUDAGraph(keep_graph=True)
+            with torch.cuda.graph(graph):
+                y = F.dequantize_mxfp4(*F.quantize_rows_mxfp4(F.mxfp4_linear(x, *b)))
+                y = F.mxfp4_gemm(*F.rmsnorm_mxfp4(y, w, 1e-5), *b)
+        finally:
+            assert native().set_pdl(old) == mode
+        few, every = _programmatic_edges(graph)
+        assert every >= 5 and few == (0 if mode == 0 else every)
+        graph.instantiate()
+        graph.replay()
+        outs.append(y.clone())
+        torch.cuda.synchronize()
+        del graph
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
