@@ -466,14 +466,15 @@ class NativeGraniteSwitch:
         return codes[0][:m], codes[1][: (m + 127) // 128]
 
     def _norm(self, h: torch.Tensor, w: torch.Tensor, x: torch.Tensor, pl: PackedLinear | None,
-              rows: bool = False):
+              rows: bool = False, lora: bool = True):
         """RMSNorm before projection ``pl``: into ``x`` (bf16), or quantised for an MXFP4 projection,
-        whose codes are returned (``x`` is then written for the LoRA shrink, or on ``rows``)."""
+        whose codes are returned (``x`` is then written for the LoRA shrink, unless the projection
+        runs with ``lora=False``, or on ``rows``)."""
         if pl is None or pl.w4 is None:
             E.rmsnorm(h, w, self.cfg.rms_norm_eps, out=x)
             return None
         c = self._rows4(self.in4[self.hidden], h.shape[0])
-        return F4.rmsnorm_mxfp4(h, w, self.cfg.rms_norm_eps, *c, out=x if rows or pl.has_lora else None)
+        return F4.rmsnorm_mxfp4(h, w, self.cfg.rms_norm_eps, *c, out=x if rows or (lora and pl.has_lora) else None)
 
     def _proj4(self, pl: PackedLinear, x: torch.Tensor, out, epi, residual, scale, lora: bool, n_rows, xq,
                keep_act: bool):
@@ -762,7 +763,6 @@ class NativeGraniteSwitch:
         Logits are read from the adapter stream. Under tensor parallelism both
         streams are reduced over NCCL; the cross stream is replicated.
         """
-        cfg = self.cfg
         R = self._region
         t = b.num_tokens
         hb = self.hbase[:t]
@@ -770,14 +770,13 @@ class NativeGraniteSwitch:
             hb.copy_(h)  # both streams start from the embedding
         qa = self.qa[:t]
         q_n = self.num_q * self.head_dim
-        eps = cfg.rms_norm_eps
         hb2 = self.hbase2[:t] if self.hbase2 is not None else None
         for li, lw in enumerate(self.layers):
             # base stream: q, k, v without LoRA; k/v go to the cache
             with R("rmsnorm"):
-                E.rmsnorm(hb, lw.in_norm, eps, out=x)
+                xq = self._norm(hb, lw.in_norm, x, lw.qkv, lora=False)
             with R("qkv"):
-                self._proj(lw.qkv, x, qkv, lora=False)
+                self._proj(lw.qkv, x, qkv, lora=False, xq=xq)
             with R("rope+kv"):
                 self._rope_and_cache(b, qkv, li)
             self._attention(b, qkv, li, attn, scale)
@@ -785,9 +784,9 @@ class NativeGraniteSwitch:
                 self._row_parallel(lw.o, attn, hb, mult, lora=False, partial=hb2)
             # adapter stream: switched Q only, same base K/V
             with R("rmsnorm"):
-                E.rmsnorm(h, lw.in_norm, eps, out=x)
+                xq = self._norm(h, lw.in_norm, x, lw.qkv)
             with R("qkv"):
-                self._proj(lw.qkv, x, qa, n_rows=q_n)
+                self._proj(lw.qkv, x, qa, n_rows=q_n, xq=xq)
             with R("rope+kv"):
                 E.rope_kv(qa, b.positions, self.cos_sin, self.num_q, 0, self.head_dim)
             self._attention(b, qa, li, attn, scale)
@@ -795,12 +794,13 @@ class NativeGraniteSwitch:
                 self._row_parallel(lw.o, attn, h, mult)
             # MLPs: base stream first (its output feeds the cross stream; with
             # experts, its routing is the adapter stream's too)
+            experts = lw.moe is not None
             with R("rmsnorm"):
-                E.rmsnorm(hb, lw.post_norm, eps, out=x)
-            self._mlp(lw, x, act, hb, mult, lora=False, partial=hb2)
+                xq = self._norm(hb, lw.post_norm, x, lw.gu, rows=experts, lora=False)
+            self._mlp(lw, x, act, hb, mult, lora=False, partial=hb2, xq=xq)
             with R("rmsnorm"):
-                E.rmsnorm(h, lw.post_norm, eps, out=x)
-            self._mlp(lw, x, act, h, mult, reuse_routing=True)
+                xq = self._norm(h, lw.post_norm, x, lw.gu, rows=experts)
+            self._mlp(lw, x, act, h, mult, reuse_routing=True, xq=xq)
             with R("cross_stream"):
                 self._cross_stream(lw.cross, hb, h)
             if b.probe_groups:

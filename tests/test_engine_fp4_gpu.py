@@ -219,3 +219,29 @@ def test_programmatic_launch_switch_reaches_the_kernels(on):
         assert native().set_pdl(1) == int(on)
     finally:
         native().set_pdl(old)
+
+
+def test_norms_are_rounded_once(family_dir, monkeypatch):
+    """Every layer norm goes from fp32 to 4 bits in one kernel, in both streams of Shadow Residual: the bf16 RMSNorm
+    runs for the final norm alone, and only the inputs of the o projections meet a quantiser of their own."""
+    from granite_switch_b200.models import native
+
+    cfg, model = _model(family_dir, "mxfp4")
+    calls = dict(rmsnorm=0, rmsnorm_mxfp4=0, quantize_rows_mxfp4=0)
+
+    def counted(module, name):
+        fn = getattr(module, name)
+
+        def call(*a, **kw):
+            calls[name] += 1
+            return fn(*a, **kw)
+
+        monkeypatch.setattr(module, name, call)
+
+    counted(native.E, "rmsnorm")
+    counted(native.F4, "rmsnorm_mxfp4")
+    counted(native.F4, "quantize_rows_mxfp4")
+    steps, streams = 2, 2 if model.layers[0].cross is not None else 1
+    _logits(cfg, model, [], steps=steps)
+    n = steps * len(model.layers) * streams
+    assert calls == dict(rmsnorm=steps, rmsnorm_mxfp4=2 * n, quantize_rows_mxfp4=n)
