@@ -73,6 +73,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mxfp4_gemm_swiglu", &gsb_mxfp4_gemm_swiglu, "MXFP4 gate/up GEMM, SwiGLU and MXFP4 quantisation in the epilogue");
   m.def("mxfp4_pair_min_m", &gsb_mxfp4_pair_min_m,
         "force the smallest M of the CTA-pair MXFP4 GEMM, for A/B tests (-1: the rule; returns the old value)");
+  m.def("mxfp4_gemm_plan", &gsb_mxfp4_gemm_plan,
+        "plan of an (M, N, K) MXFP4 product: [1 for the CTA-pair kernel, tokens per tile, K parts, stages]");
+  m.def("mxfp4_split_give_up", &gsb_mxfp4_split_give_up,
+        "make one K part of the split MXFP4 GEMM report a wait that ran out, for tests (-1: none; returns the old value)");
   m.def("rope_kv_fp8", &gsb_rope_kv_fp8, "RoPE on q / k then the quantised fp8 K / V write, one launch");
   m.def("kv_write_fp8", &gsb_kv_write_fp8, "quantised (e4m3, per-row scale) write of a step's K/V into the fp8 cache");
 }

@@ -23,7 +23,8 @@
 // Warp roles (192 threads): warp 0 issues the TMA and bulk loads into a ring of
 // stages (256 K elements each), warp 1 owns the tensor memory and issues the scale
 // copies and MMAs, warps 2..5 drain the accumulator; all warps run the epilogue.
-// Every wait is bounded; a CTA that gives up still arrives at the cluster barriers.
+// Every wait is bounded; a CTA that gives up still arrives at the cluster barriers, and tells its
+// cluster, which then stores nothing of that tile: its sums would lack that CTA's part.
 //
 // What bounds it (B200, CUDA-graph replays over rotating weights): its own chain of latencies
 // more than the bytes. 1 x 4096 x 4096 takes 5.2 us (the codes' and scales' bytes 1.4 us at the
@@ -78,6 +79,7 @@ struct SplitParams {
   int ks, rows_per;   // K parts per tile (cluster size), tokens per part in the reduction
   int tmem_cols;
   int reduce_off;     // offset of the reduction buffer: 0 (over the ring) or behind it
+  int give_up;        // K part that reports a wait that ran out, at once (tests), or -1
   const uint8_t* sfx;
   const uint8_t* sfw;
   float scale;
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], tfull_bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int abort_flag;
+  __shared__ volatile int abort_flag, peer_abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = p.ks, stages = p.stages;
@@ -252,7 +254,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(&tfull_bar, 1);
-    abort_flag = 0;
+    abort_flag = part == p.give_up;
+    peer_abort = 0;
+    if (part == p.give_up) raise_error(err, kErrGemmWait);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -462,10 +466,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   };
   if (EPI == kEpiResAdd) load_residuals(threadIdx.x);
-  __syncthreads();
-  if (ks > 1) cluster_sync();  // every partial row has landed
-  if (abort_flag) {
-    // nothing is written
+  __syncthreads();  // abort_flag is final
+  if (ks > 1) {
+    if (abort_flag && threadIdx.x < ks)
+      asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(
+                       mapa_shared(smem_u32(const_cast<int*>(&peer_abort)), threadIdx.x))
+                   : "memory");
+    cluster_sync();  // every partial row has landed
+  }
+  if (abort_flag || peer_abort) {
+    // nothing of the tile is written, by any CTA of the cluster
   } else if constexpr (EPI == kEpiSwiGLU) {
     // four neighbouring items are one block of 32 outputs; whole warps run for the shuffles
     for (int it = threadIdx.x; it < (items + 31) / 32 * 32; it += THREADS) {
@@ -1004,6 +1014,9 @@ static bool use_pair(int M, int N) {
   return M > BT && (M + 255) / 256 * ((N + 255) / 256) >= 48;
 }
 
+// K part that gives up in the split kernel's calls (tests), or -1.
+static int g_split_give_up = -1;
+
 struct SplitPlan {
   int mt_rows, token_tiles, weight_tiles, ks, stages, stage_bytes, tmem_cols, smem_bytes, reduce_off;
 };
@@ -1275,6 +1288,7 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   const SplitPlan s = split_plan(M, N, K);
   GSB_CHECK(s.token_tiles <= 65535, "mxfp4_gemm: too many rows");
   p.reduce_off = s.reduce_off;
+  p.give_up = g_split_give_up;
   p.sfx = x.sf;
   p.sfw = w.sf;
   p.stages = s.stages;
@@ -1371,5 +1385,23 @@ std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
 int64_t gsb_mxfp4_pair_min_m(int64_t m) {
   const int64_t old = f4::g_pair_min_m;
   f4::g_pair_min_m = (int)std::max<int64_t>(-1, std::min<int64_t>(m, 1 << 30));
+  return old;
+}
+
+// The plan of an M x N x K product: {1 for the pair kernel, tokens per tile, K parts per tile, stages}.
+std::vector<int64_t> gsb_mxfp4_gemm_plan(int64_t M, int64_t N, int64_t K) {
+  using namespace gsb::f4;
+  GSB_CHECK(M >= 1 && M < (int64_t(1) << 24) && N >= 1 && N < (int64_t(1) << 24) && K >= 1 && K < (int64_t(1) << 31),
+            "mxfp4_gemm_plan: sizes out of range");
+  if (use_pair((int)M, (int)N)) return {1, 256, 1, PairCfg::STAGES};
+  const SplitPlan s = split_plan((int)M, (int)N, K);
+  return {0, s.mt_rows, s.ks, s.stages};
+}
+
+// Makes one K part of every split-kernel cluster behave as if a wait had run out (-1: none); returns the previous
+// value.
+int64_t gsb_mxfp4_split_give_up(int64_t part) {
+  const int64_t old = gsb::f4::g_split_give_up;
+  gsb::f4::g_split_give_up = (int)std::max<int64_t>(-1, std::min<int64_t>(part, gsb::f4::MAX_KS));
   return old;
 }

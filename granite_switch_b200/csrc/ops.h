@@ -117,3 +117,5 @@ std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
     const c10::optional<at::Tensor>& s, const c10::optional<at::Tensor>& lb, const c10::optional<at::Tensor>& tile_mask,
     int64_t rank, int64_t num_adapters, const at::Tensor& err);
 int64_t gsb_mxfp4_pair_min_m(int64_t m);
+std::vector<int64_t> gsb_mxfp4_gemm_plan(int64_t M, int64_t N, int64_t K);
+int64_t gsb_mxfp4_split_give_up(int64_t part);

@@ -661,3 +661,36 @@ def test_programmatic_launch_can_be_turned_off():
         torch.cuda.synchronize()
         del graph
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 4096, 4096), (16, 512, 2048), (128, 2048, 12800)])
+@pytest.mark.parametrize("part", [0, 1])
+def test_a_part_that_gives_up_writes_nothing(m, n, k, part):
+    """When one K part of a tile's cluster reports a wait that ran out, no CTA of the cluster stores sums that lack
+    it: the output, a residual's in place, SwiGLU's codes and scales stay as they were. The error word says so, and
+    the next call is right."""
+    from granite_switch_b200 import _native
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    nat, dev = _native.native(), torch.device("cuda", torch.cuda.current_device())
+    pair, _, ks, _ = nat.mxfp4_gemm_plan(m, n, k)
+    assert not pair and ks > part  # every tile has that part
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=73)), F.quantize_rows_mxfp4(_rows(n, k, seed=74, spread=2))
+    h = torch.randn(m, n, device="cuda", generator=_gen(75)).to(torch.bfloat16)
+    want = F.mxfp4_gemm(*a, *b, epi=F.EPI_RESADD, scale=0.5, residual=h)
+    keep = h.clone()
+    a4 = torch.full((m, n // 4), 0xAB, dtype=torch.uint8, device="cuda")
+    sf = torch.full(((m + 127) // 128, (n // 2 + 255) // 256 * 2, 512), 0xCD, dtype=torch.uint8, device="cuda")
+    act = torch.full((m, n // 2), 5.0, dtype=torch.bfloat16, device="cuda")
+    assert _native.read_errors(dev) == 0
+    old = nat.mxfp4_split_give_up(part)
+    try:
+        F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.5, residual=h)
+        assert _native.read_errors(dev) == _native.ERR_GEMM_WAIT
+        F.mxfp4_gemm_swiglu(*a, *b, a4, sf, act)
+        assert _native.read_errors(dev) == _native.ERR_GEMM_WAIT
+    finally:
+        nat.mxfp4_split_give_up(old)
+    assert torch.equal(h, keep) and (a4 == 0xAB).all() and (sf == 0xCD).all() and (act == 5.0).all()
+    F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.5, residual=h)
+    assert torch.equal(h, want) and _native.read_errors(dev) == 0
