@@ -1174,8 +1174,9 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
                      const at::Tensor& err, const at::Device& dev) {
   Codes& x = t.c;
   GSB_CHECK(K >= kBlock && K % kBlock == 0 && K < (int64_t(1) << 31), "mxfp4_gemm: K must be a positive multiple of 32");
-  GSB_CHECK(x.rows < (int64_t(1) << 24) && w.rows > 0 && w.rows < (int64_t(1) << 24) && w.rows % 8 == 0,
-            "mxfp4_gemm: N must be a positive multiple of 8");
+  GSB_CHECK(w.rows > 0 && w.rows % 8 == 0, "mxfp4_gemm: N must be a positive multiple of 8");
+  GSB_CHECK(x.rows < (int64_t(1) << 24) && w.rows < (int64_t(1) << 24),
+            "mxfp4_gemm: at most 2^24 - 1 rows of x and of the weight");
   GSB_CHECK(err.device() == dev, "mxfp4_gemm: error word on another device");
   const int M = (int)x.rows, N = (int)w.rows;
   SplitParams p{};

@@ -694,3 +694,17 @@ def test_a_part_that_gives_up_writes_nothing(m, n, k, part):
     assert torch.equal(h, keep) and (a4 == 0xAB).all() and (sf == 0xCD).all() and (act == 5.0).all()
     F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.5, residual=h)
     assert torch.equal(h, want) and _native.read_errors(dev) == 0
+
+
+def test_too_many_rows_are_named():
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    few = F.quantize_rows_mxfp4(_rows(8, 32, seed=76))
+    many = (torch.zeros(1 << 24, 16, dtype=torch.uint8, device="cuda"),
+            torch.zeros(1 << 17, 2, 512, dtype=torch.uint8, device="cuda"))
+    out = torch.empty(8, 8, dtype=torch.bfloat16, device="cuda")
+    for a, b in ((many, few), (few, many)):
+        with pytest.raises(RuntimeError, match="2\\^24 - 1 rows"):
+            F.mxfp4_gemm(*a, *b, out)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        F.mxfp4_gemm(*few, few[0][:7], few[1], out)
