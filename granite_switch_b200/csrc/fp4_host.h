@@ -20,6 +20,38 @@ inline at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const a
 
 inline bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
+// Bytes that a matrix (or a contiguous tensor, as one row) takes: rows of `width` bytes, `stride` apart.
+struct Span {
+  uintptr_t at;
+  int64_t rows, width, stride;
+};
+inline Span span(const at::Tensor& t) {
+  const int64_t item = (int64_t)t.element_size();
+  const bool matrix = t.dim() == 2 && t.size(0) > 1 && t.stride(0) != 0;
+  const int64_t width = (t.dim() == 2 ? t.size(1) : t.numel()) * item;
+  return {reinterpret_cast<uintptr_t>(t.data_ptr()), t.numel() == 0 ? 0 : (matrix ? t.size(0) : 1), width,
+          matrix ? t.stride(0) * item : 0};
+}
+// Whether two spans share a byte; columns of one buffer do not. (Rows at different strides whose ranges meet: yes.)
+inline bool overlap(const Span& a, const Span& b) {
+  if (a.rows == 0 || b.rows == 0) return false;
+  if (a.at + (a.rows - 1) * a.stride + a.width <= b.at || b.at + (b.rows - 1) * b.stride + b.width <= a.at) return false;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride;
+  if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return true;
+  const int64_t d = ((int64_t)(b.at - a.at) % stride + stride) % stride;
+  return d < a.width || d + b.width > stride;
+}
+// Refuses an output that shares bytes with another operand: its CTAs would read what others have written.
+inline void check_apart(const char* op, const char* what, const at::Tensor& out, const char* other, const at::Tensor& t) {
+  GSB_CHECK(!overlap(span(out), span(t)), op, ": ", what, " must not overlap ", other);
+}
+// The same, but the output may be the operand itself.
+inline void check_same_or_apart(const char* op, const char* what, const at::Tensor& out, const char* other,
+                                const at::Tensor& t) {
+  if (out.data_ptr() == t.data_ptr() && (out.size(0) <= 1 || out.stride(0) == t.stride(0))) return;
+  check_apart(op, what, out, other, t);
+}
+
 // Launches an MXFP4 kernel with `cluster` CTAs a cluster (1: none, or compiled in), unless set_pdl(0) turned
 // that off as a programmatic dependent of the kernel before it in the stream: before they wait for that one
 // (griddep_wait), these kernels touch their own shared and tensor memory only and prefetch

@@ -1152,6 +1152,18 @@ static CUtensorMap make_tmap_codes(const Codes& c, int64_t K, uint32_t box_rows)
                       box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Refuses an output of a product that shares bytes with what the product reads.
+static void check_output_apart(const char* what, const at::Tensor& out, const at::Tensor* x4, const at::Tensor* sfx,
+                               const at::Tensor& w4, const at::Tensor& sfw, const c10::optional<at::Tensor>& s,
+                               const c10::optional<at::Tensor>& lb) {
+  if (x4 != nullptr) check_apart("mxfp4_gemm", what, out, "x", *x4);
+  if (sfx != nullptr) check_apart("mxfp4_gemm", what, out, "x's scales", *sfx);
+  check_apart("mxfp4_gemm", what, out, "the weight", w4);
+  check_apart("mxfp4_gemm", what, out, "the weight's scales", sfw);
+  if (s.has_value()) check_apart("mxfp4_gemm", what, out, "s", *s);
+  if (lb.has_value()) check_apart("mxfp4_gemm", what, out, "lb", *lb);
+}
+
 struct LoraArgs {
   const c10::optional<at::Tensor>& s;
   const c10::optional<at::Tensor>& lb;
@@ -1197,6 +1209,7 @@ static void run_gemm(Tokens t, const Codes& w, int64_t K, const at::Tensor* out,
   if (epi == kEpiResAdd) {
     GSB_CHECK(residual.has_value(), "mxfp4_gemm: the residual epilogue needs a residual");
     check_out("residual", *residual, M, N, dev);
+    check_same_or_apart("mxfp4_gemm", "out", *out, "the residual, unless it is the residual", *residual);
     p.residual = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
     p.ldr = residual->stride(0);
   }
@@ -1331,6 +1344,7 @@ at::Tensor gsb_mxfp4_gemm(const at::Tensor& x4, const at::Tensor& sfx, const at:
   const f4::Codes x = f4::check_operand("x", x4, sfx, K, dev), w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
   const at::Tensor out = out_.has_value() ? *out_ : f4::new_tensor({x.rows, w.rows}, at::kBFloat16, dev);
+  if (out_.has_value()) f4::check_output_apart("out", out, &x4, &sfx, w4, sfw, s, lb);
   f4::run_gemm(f4::Tokens{x, nullptr, 0}, w, K, &out, (int)epi, scale, residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
                             slice_bounds.has_value() ? *slice_bounds : std::vector<int64_t>{0, w.rows}},
@@ -1352,6 +1366,8 @@ at::Tensor gsb_mxfp4_linear(const at::Tensor& x, const at::Tensor& w4, const at:
   const f4::Codes w = f4::check_operand("w", w4, sfw, K, dev);
   c10::cuda::CUDAGuard g(dev);
   const at::Tensor out = out_.has_value() ? *out_ : f4::new_tensor({M, w.rows}, at::kBFloat16, dev);
+  // out may be x, which is quantised before the product starts
+  if (out_.has_value()) f4::check_output_apart("out", out, nullptr, nullptr, w4, sfw, s, lb);
   f4::run_gemm(f4::Tokens{f4::Codes{nullptr, 0, nullptr, M}, x.data_ptr(), x.stride(0)}, w, K, &out, (int)epi, scale,
                residual, nullptr,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters,
@@ -1377,6 +1393,14 @@ std::tuple<at::Tensor, at::Tensor> gsb_mxfp4_gemm_swiglu(
   f4::make_codes(x.rows, I, dev, a4, sf);
   const f4::Codes o = f4::check_operand("output", a4, sf, I, dev);
   GSB_CHECK(o.rows == x.rows, "mxfp4_gemm_swiglu: output codes must be [M, I / 2]");
+  f4::check_output_apart("output codes", a4, &x4, &sfx, w4, sfw, s, lb);
+  f4::check_output_apart("output scales", sf, &x4, &sfx, w4, sfw, s, lb);
+  f4::check_apart("mxfp4_gemm_swiglu", "output scales", sf, "the output codes", a4);
+  if (act.has_value()) {
+    f4::check_output_apart("act", *act, &x4, &sfx, w4, sfw, s, lb);
+    f4::check_apart("mxfp4_gemm_swiglu", "act", *act, "the output codes", a4);
+    f4::check_apart("mxfp4_gemm_swiglu", "act", *act, "the output scales", sf);
+  }
   f4::run_gemm(f4::Tokens{x, nullptr, 0}, w, K, act.has_value() ? &*act : nullptr, kEpiSwiGLU, 1.0, c10::nullopt, &o,
                f4::LoraArgs{s, lb, tile_mask, rank, num_adapters, {}}, err, dev);
   return {a4, sf};

@@ -14,7 +14,9 @@ nibble) and scale atoms ``[ceil(M / 128), 2 ceil(K / 256), 512]``: byte
 ``32 j`` of the atom's 128; bytes of blocks past K are 0. Activations and weights have the
 same format, so :func:`quantize_rows_mxfp4` serves both.
 
-Products are summed in fp32 by the tensor core and rounded once, in the epilogue.
+Products are summed in fp32 by the tensor core and rounded once, in the epilogue. An output
+that shares memory with an operand is refused, but for the few that may be an operand itself
+(the residual, the norm's ``x``, the linear's ``x``).
 """
 from __future__ import annotations
 

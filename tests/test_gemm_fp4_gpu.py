@@ -708,3 +708,75 @@ def test_too_many_rows_are_named():
             F.mxfp4_gemm(*a, *b, out)
     with pytest.raises(RuntimeError, match="multiple of 8"):
         F.mxfp4_gemm(*few, few[0][:7], few[1], out)
+
+
+def test_overlapping_outputs_are_refused():
+    """An output that shares memory with what the call reads (or with another output) is refused, unless it is the
+    residual, the norm's rows or the linear's rows themselves; columns and rows of one buffer beside them are not."""
+    from granite_switch_b200.ops import elementwise as E
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, k = 200, 256
+    bytes_ = torch.zeros(1 << 21, dtype=torch.uint8, device="cuda")
+
+    def at(offset, shape, dtype=torch.uint8):
+        n = shape[0] * shape[1] * torch.empty(0, dtype=dtype).element_size()
+        return bytes_[offset:offset + n].view(dtype).view(shape)
+
+    def atoms(offset, rows, cols):
+        tiles, kt = (rows + 127) // 128, (cols + 255) // 256 * 2
+        return bytes_[offset:offset + tiles * kt * 512].view(tiles, kt, 512)
+
+    x = at(0, (m, k), torch.bfloat16)  # 102,400 bytes
+    x.copy_(_rows(m, k, seed=81, spread=1))
+    w = torch.ones(k, device="cuda").bfloat16()
+    a, b = F.quantize_rows_mxfp4(x), F.quantize_rows_mxfp4(_rows(k, k, seed=82, spread=1))
+    here = at(200704, (m, k // 2)), atoms(262144, m, k)  # codes and scales in the buffer
+    here[0].copy_(a[0])
+    here[1].copy_(a[1])
+    h = at(400384, (m + 8, k), torch.bfloat16)
+    s, lb = at(600064, (m, 32), torch.bfloat16), at(700416, (k, 32), torch.bfloat16)
+    lora = dict(s=s, lb=lb, rank=32, num_adapters=1)
+    bad = [
+        lambda: F.quantize_rows_mxfp4(x, x4=at(1024, (m, k // 2))),
+        lambda: F.quantize_rows_mxfp4(x, sf=atoms(102384, m, k)),
+        lambda: F.quantize_rows_mxfp4(x, x4=at(200704, (m, k // 2)), sf=atoms(200704, m, k)),
+        lambda: F.dequantize_mxfp4(*here, out=at(200704 - 4096, (m, k), torch.bfloat16)),
+        lambda: F.dequantize_mxfp4(*here, out=at(262144 - 4096, (m, k), torch.bfloat16)),
+        lambda: F.rmsnorm_mxfp4(x, w, 1e-5, out=at(512, (m, k), torch.bfloat16)),          # a row further down
+        lambda: F.rmsnorm_mxfp4(x, w, 1e-5, x4=at(0, (m, k // 2))),
+        lambda: F.rmsnorm_mxfp4(x, w, 1e-5, *here, out=at(200704, (m, k), torch.bfloat16)),
+        lambda: F.rmsnorm_mxfp4(x, at(400384, (1, k), torch.bfloat16)[0], 1e-5, out=h[:m]),
+        lambda: F.mxfp4_gemm(*here, *b, at(200704, (m, k), torch.bfloat16)),
+        lambda: F.mxfp4_gemm(*a, *b, h[:m], epi=F.EPI_RESADD, residual=h[8:]),
+        lambda: F.mxfp4_gemm(*a, *b, at(600064, (m, k), torch.bfloat16), **lora),
+        lambda: F.mxfp4_gemm(*a, *b, at(700416, (m, k), torch.bfloat16), **lora),
+        lambda: F.mxfp4_gemm(*a, here[0], here[1], at(200704, (m, m), torch.bfloat16)),      # the weight
+        lambda: F.mxfp4_linear(x, *here, at(262144, (m, m), torch.bfloat16)),                # its scales
+        lambda: F.mxfp4_gemm_swiglu(*here, *b, a4=at(200704, (m, k // 4))),
+        lambda: F.mxfp4_gemm_swiglu(*here, *b, sf=atoms(262144, m, k // 2)),
+        lambda: F.mxfp4_gemm_swiglu(*here, *b, act=at(200704, (m, k // 2), torch.bfloat16)),
+        lambda: F.mxfp4_gemm_swiglu(*a, *b, a4=at(400384, (m, k // 4)), act=at(400384, (m, k // 2), torch.bfloat16)),
+    ]
+    keep = bytes_.clone()
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    assert torch.equal(bytes_, keep)
+    # columns of one buffer, rows behind one another, and the operand itself
+    want = F.mxfp4_gemm(*a, *b)
+    wide = torch.empty(m, 3 * k, dtype=torch.bfloat16, device="cuda")
+    wide[:, :k] = x
+    F.mxfp4_linear(wide[:, :k], *b, wide[:, k:2 * k])
+    F.mxfp4_gemm(*a, *b, wide[:, 2 * k:], epi=F.EPI_RESADD, residual=wide[:, k:2 * k], scale=0.0)
+    assert torch.equal(wide[:, :k], x) and torch.equal(wide[:, k:2 * k], want) and torch.equal(wide[:, 2 * k:], want)
+    F.mxfp4_linear(wide[:, :k], *b, wide[:, :k])
+    assert torch.equal(wide[:, :k], want)
+    y = torch.cat((x, x))
+    F.rmsnorm_mxfp4(y[:m], w, 1e-5, out=y[m:])
+    assert torch.equal(y[m:], E.rmsnorm(x, w, 1e-5)) and torch.equal(y[:m], x)
+    one = torch.empty(3 * k, dtype=torch.bfloat16, device="cuda").view(1, -1)
+    one[:, k:2 * k] = x[:1]
+    F.rmsnorm_mxfp4(one[:, k:2 * k], w, 1e-5, out=one[:, 2 * k:])
+    assert torch.equal(one[:, 2 * k:], E.rmsnorm(x[:1], w, 1e-5))
