@@ -780,3 +780,123 @@ def test_overlapping_outputs_are_refused():
     one[:, k:2 * k] = x[:1]
     F.rmsnorm_mxfp4(one[:, k:2 * k], w, 1e-5, out=one[:, 2 * k:])
     assert torch.equal(one[:, 2 * k:], E.rmsnorm(x[:1], w, 1e-5))
+
+
+# ------------------------------------------------------------- the CTA-pair kernel at sizes of the split kernel's
+def _is_pair(m, n, k):
+    from granite_switch_b200._native import native
+
+    return native().mxfp4_gemm_plan(m, n, k)[0] == 1
+
+
+@pytest.mark.parametrize("m", [3, 200, 1400])
+@pytest.mark.parametrize("na,rank", [(64, 32), (3, 96)])
+def test_pair_lora_limits(pair_always, m, na, rank):
+    assert _is_pair(m, 1024, 2048)
+    test_gemm_lora_limits(m, na, rank)
+
+
+@pytest.mark.parametrize("m", [1, 3, 5, 130, 300, 1100])
+@pytest.mark.parametrize("bounds", [[0, 640], [0, 1024, 1280, 1536], [0, 384, 512, 2176], [0, 128, 256, 384, 640]])
+def test_pair_lora_slices(pair_always, m, bounds):
+    """Bounds at odd multiples of 128 cut a 256-row weight tile in two slices of S."""
+    assert _is_pair(m, bounds[-1], 512)
+    test_gemm_lora_slices(m, bounds)
+
+
+def _check_lora_residual(m, bounds, na, rank, k=1056):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    n = bounds[-1]
+    a, b = F.quantize_rows_mxfp4(_rows(m, k, seed=91)), F.quantize_rows_mxfp4(_rows(n, k, seed=92, spread=2))
+    s, dirty, lb, mask = _lora_inputs(m, n, len(bounds) - 1, na, rank, seed=93)
+    kw = dict(lb=lb, rank=rank, num_adapters=na, slice_bounds=bounds)
+    h = torch.randn(m, n, device="cuda", generator=_gen(94)).to(torch.bfloat16)
+    ref = h.double() + 0.5 * F.mxfp4_product_reference(*a, *b, s=s, **kw)
+    tol = _acc_tol(*a, *b, extra=(s.double().abs().sum(1, keepdim=True) * lb.double().abs().max()))
+    tol = 0.5 * tol + h.double().abs() * 2.0 ** -23
+    _check(F.mxfp4_gemm(*a, *b, h, epi=F.EPI_RESADD, scale=0.5, residual=h, s=dirty, tile_mask=mask, **kw), ref, tol)
+
+
+@pytest.mark.parametrize("m", [2, 129, 700])
+@pytest.mark.parametrize("bounds,na,rank", [([0, 384, 1160], 2, 32), ([0, 896], 5, 96), ([0, 128, 264], 3, 64)])
+def test_lora_with_residual(m, bounds, na, rank):
+    _check_lora_residual(m, bounds, na, rank)
+
+
+@pytest.mark.parametrize("m", [2, 129, 700])
+@pytest.mark.parametrize("bounds,na,rank", [([0, 384, 1160], 2, 32), ([0, 896], 5, 96), ([0, 128, 264], 3, 64)])
+def test_pair_lora_with_residual(pair_always, m, bounds, na, rank):
+    assert _is_pair(m, bounds[-1], 1056)
+    _check_lora_residual(m, bounds, na, rank)
+
+
+def test_lora_products_of_the_rule_reach_the_pair_kernel():
+    """A size that the rule itself gives to the pair kernel, with three slices, one of them cutting a tile."""
+    assert _is_pair(2100, 1664, 1056)
+    _check_lora_residual(2100, [0, 1152, 1408, 1664], 4, 32)
+
+
+@pytest.mark.parametrize("m,i,h", [(1, 64, 64), (17, 192, 512), (4, 320, 512), (130, 1088, 256), (300, 512, 1056),
+                                   (257, 192, 2080)])
+@pytest.mark.parametrize("lora", [False, True])
+def test_pair_swiglu(pair_always, m, i, h, lora):
+    assert _is_pair(m, 2 * i, h)
+    test_gemm_swiglu(m, i, h, lora)
+
+
+@pytest.mark.parametrize("m", [2, 190, 1025])
+def test_pair_mlp_block(pair_always, m):
+    test_mlp_block(m)
+
+
+def _check_swiglu_padding(m, i):
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    a = F.quantize_rows_mxfp4(_rows(m, 256, seed=95, spread=1))
+    b = F.quantize_rows_mxfp4(_rows(2 * i, 256, seed=96, spread=1))
+    a4 = torch.full((m + 3, i // 2), 0xAB, dtype=torch.uint8, device="cuda")
+    sf = torch.full(((m + 127) // 128, (i + 255) // 256 * 2, 512), 0xFF, dtype=torch.uint8, device="cuda")
+    F.mxfp4_gemm_swiglu(*a, *b, a4[:m], sf)
+    byte = F.scale_bytes_from_atoms(sf, m, sf.shape[1] * 128)
+    assert not byte[:, i // 32:].any() and (byte[:, :i // 32] < 255).all()
+    rest = F.scale_bytes_from_atoms(sf, sf.shape[0] * 128, sf.shape[1] * 128)[m:]
+    assert (rest == 0xFF).all() and (a4[m:] == 0xAB).all()  # rows behind the last one stay as they were
+
+
+@pytest.mark.parametrize("m", [1, 100, 300])
+@pytest.mark.parametrize("i", [64, 192, 320, 1088])
+def test_swiglu_clears_the_scales_past_its_rows(m, i):
+    _check_swiglu_padding(m, i)
+
+
+@pytest.mark.parametrize("m", [1, 100, 300])
+@pytest.mark.parametrize("i", [64, 192, 320, 1088])
+def test_pair_swiglu_clears_the_scales_past_its_rows(pair_always, m, i):
+    assert _is_pair(m, 2 * i, 256)
+    _check_swiglu_padding(m, i)
+
+
+@pytest.mark.parametrize("m,h", [(1000, 4128), (1003, 6144), (1000, 8192), (1001, 8224), (999, 12800), (900, 16384),
+                                 (1500, 4224), (1500, 8256)])
+@pytest.mark.parametrize("with_out", [False, True])
+def test_rmsnorm_quantised_wide_rows(m, h, with_out):
+    """Widths of every instantiation above 4096 columns, with more rows than CTAs: rings and sums are used again."""
+    test_rmsnorm_quantised(m, h, with_out)
+
+
+@pytest.mark.parametrize("h", [2048, 4096, 8192, 12800])
+def test_rmsnorm_scales_of_old_buffers(h):
+    """A caller's buffers: scales past the row's end are cleared, rows behind the last one stay as they were."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    m, h = 700, h - 96
+    x = _rows(m, h, seed=97, spread=1)
+    w = torch.ones(h, device="cuda").bfloat16()
+    x4 = torch.full((m + 2, h // 2), 0xAB, dtype=torch.uint8, device="cuda")
+    sf = torch.full(((m + 127) // 128, (h + 255) // 256 * 2, 512), 0xFF, dtype=torch.uint8, device="cuda")
+    F.rmsnorm_mxfp4(x, w, 1e-5, x4[:m], sf)
+    f4, fsf = F.rmsnorm_mxfp4(x, w, 1e-5)
+    byte = F.scale_bytes_from_atoms(sf, sf.shape[0] * 128, sf.shape[1] * 128)
+    assert torch.equal(x4[:m], f4) and (x4[m:] == 0xAB).all() and (byte[m:] == 0xFF).all()
+    assert torch.equal(byte[:m, :h // 32], F.scale_bytes_from_atoms(fsf, m, h)) and not byte[:m, h // 32:].any()
