@@ -329,9 +329,11 @@ std::tuple<at::Tensor, at::Tensor> gsb_quantize_mxfp4(const at::Tensor& x, const
   at::Tensor x4 = x4_.value_or(at::Tensor()), sf = sf_.value_or(at::Tensor());
   f4::make_codes(M, K, x.device(), x4, sf);
   f4::check_codes("quantize_mxfp4", x4, sf, M, K, x.device());
-  f4::check_apart("quantize_mxfp4", "codes", x4, "x", x);
-  f4::check_apart("quantize_mxfp4", "scales", sf, "x", x);
-  f4::check_apart("quantize_mxfp4", "scales", sf, "the codes", x4);
+  if (x4_.has_value() || sf_.has_value()) {
+    f4::check_apart("quantize_mxfp4", "codes", x4, "x", x);
+    f4::check_apart("quantize_mxfp4", "scales", sf, "x", x);
+    f4::check_apart("quantize_mxfp4", "scales", sf, "the codes", x4);
+  }
   if (M > 0)
     f4::quantize_launch(x.data_ptr(), x.stride(0), M, K, x4.data_ptr<uint8_t>(), x4.stride(0), sf.data_ptr<uint8_t>(),
                         c10::cuda::getCurrentCUDAStream(x.device().index()).stream());
@@ -353,11 +355,13 @@ std::tuple<at::Tensor, at::Tensor> gsb_rmsnorm_mxfp4(const at::Tensor& x, const 
   at::Tensor x4 = x4_.value_or(at::Tensor()), sf = sf_.value_or(at::Tensor());
   f4::make_codes(M, H, x.device(), x4, sf);
   f4::check_codes("rmsnorm_mxfp4", x4, sf, M, H, x.device());
-  for (const at::Tensor* o : {&x4, &sf}) {
-    f4::check_apart("rmsnorm_mxfp4", "codes and scales", *o, "x", x);
-    f4::check_apart("rmsnorm_mxfp4", "codes and scales", *o, "the weight", w);
+  if (x4_.has_value() || sf_.has_value()) {
+    for (const at::Tensor* o : {&x4, &sf}) {
+      f4::check_apart("rmsnorm_mxfp4", "codes and scales", *o, "x", x);
+      f4::check_apart("rmsnorm_mxfp4", "codes and scales", *o, "the weight", w);
+    }
+    f4::check_apart("rmsnorm_mxfp4", "scales", sf, "the codes", x4);
   }
-  f4::check_apart("rmsnorm_mxfp4", "scales", sf, "the codes", x4);
   __nv_bfloat16* op = nullptr;
   int64_t ldo = 0;
   GSB_CHECK(M < (int64_t(1) << 30), "rmsnorm_mxfp4: too many rows");
@@ -404,8 +408,10 @@ at::Tensor gsb_dequantize_mxfp4(const at::Tensor& x4, const at::Tensor& sf, cons
   GSB_CHECK(out.size(0) == M && out.size(1) == K && (M <= 1 || out.stride(0) >= K),
             "dequantize_mxfp4: out must be [M, K] with rows of their own");
   f4::check_codes("dequantize_mxfp4", x4, sf, M, K, x4.device());
-  f4::check_apart("dequantize_mxfp4", "out", out, "the codes", x4);
-  f4::check_apart("dequantize_mxfp4", "out", out, "the scales", sf);
+  if (out_.has_value()) {
+    f4::check_apart("dequantize_mxfp4", "out", out, "the codes", x4);
+    f4::check_apart("dequantize_mxfp4", "out", out, "the scales", sf);
+  }
   if (M == 0) return out;
   const f4::StreamPlan s = f4::stream_plan("dequantize_mxfp4", M, K);
   const auto kernel = s.units == 1   ? f4::dequantize_mxfp4_kernel<1>
