@@ -900,3 +900,59 @@ def test_rmsnorm_scales_of_old_buffers(h):
     byte = F.scale_bytes_from_atoms(sf, sf.shape[0] * 128, sf.shape[1] * 128)
     assert torch.equal(x4[:m], f4) and (x4[m:] == 0xAB).all() and (byte[m:] == 0xFF).all()
     assert torch.equal(byte[:m, :h // 32], F.scale_bytes_from_atoms(fsf, m, h)) and not byte[:m, h // 32:].any()
+
+
+def _check_strided_operands(m):
+    """Codes, shrink output and expand weights that are columns of wider buffers, weights that are rows of a larger one,
+    an output among other columns: as of contiguous copies, bit for bit, and nothing beside the output written."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    n, k, na, rank = 384, 1056, 3, 32
+    a = F.quantize_rows_mxfp4(_rows(m, k, seed=101, spread=1))
+    big = F.quantize_rows_mxfp4(_rows(n + 128, k, seed=102, spread=1))
+    b = big[0][128:], big[1][1:]
+    s, dirty, lb, mask = _lora_inputs(m, n, 2, na, rank, seed=103)
+    kw = dict(tile_mask=mask, rank=rank, num_adapters=na, slice_bounds=[0, 128, n])
+
+    def inside(t, fill):
+        wide = torch.full((t.shape[0] + 2, t.shape[1] + 64), fill, dtype=t.dtype, device="cuda")
+        wide[1:-1, 32:-32] = t
+        return wide[1:-1, 32:-32]
+
+    want = F.mxfp4_gemm(*a, b[0].clone(), b[1].clone(), s=dirty, lb=lb, **kw)
+    out = torch.full((m + 2, n + 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = F.mxfp4_gemm(inside(a[0], 0xAB), a[1], inside(b[0], 0xCD), b[1], out[1:-1, 32:-32],
+                       s=inside(dirty, float("nan")), lb=inside(lb, float("nan")), **kw)
+    assert torch.equal(got, want)
+    out[1:-1, 32:-32] = 5.0
+    assert (out == 5.0).all()
+
+
+@pytest.mark.parametrize("m", [1, 7, 200, 700])
+def test_strided_operands(m):
+    _check_strided_operands(m)
+
+
+@pytest.mark.parametrize("m", [1, 7, 200, 700])
+def test_pair_strided_operands(pair_always, m):
+    _check_strided_operands(m)
+
+
+def test_graphs_replayed_in_turn():
+    """Two captured graphs and eager calls between them, each with a workspace of its own."""
+    from granite_switch_b200.ops import gemm_fp4 as F
+
+    b = F.quantize_rows_mxfp4(_rows(1024, 2080, seed=104, spread=1))
+    xs = [_rows(m, 2080, seed=105 + m, spread=1) for m in (9, 600)]
+    want = [F.mxfp4_linear(x, *b) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(F.mxfp4_linear(F.dequantize_mxfp4(*F.quantize_rows_mxfp4(x)), *b))
+    back = [F.mxfp4_linear(F.dequantize_mxfp4(*F.quantize_rows_mxfp4(x)), *b) for x in xs]
+    for _ in range(4):
+        for i in (0, 1):
+            graphs[i].replay()
+            assert torch.equal(F.mxfp4_linear(xs[1 - i], *b), want[1 - i])
+            assert torch.equal(outs[i], back[i])
