@@ -1006,7 +1006,8 @@ static int max_clusters(int ks, int per_sm) {
 
 // Which kernel takes a call. The pair kernel needs about 48 tiles of 256 x 256 to be ahead
 // (measured, us pair / split: 256 x 4096 x 4096 11.5 / 9.7, 512: 11.7 / 11.3, 768: 11.8 / 13; 256 x
-// 25600 x 4096 20.9 / 26.9); one token tile of 128 is always the split kernel's.
+// 25600 x 4096 20.9 / 26.9; K, at which these were taken, is not looked at); one token tile of 128 is
+// always the split kernel's.
 // gsb_mxfp4_pair_min_m forces a smallest M instead, for A/B runs.
 static int g_pair_min_m = -1;
 static bool use_pair(int M, int N) {

@@ -11,8 +11,11 @@ NaN. K is a multiple of 32.
 An ``[M, K]`` matrix is held as codes ``[M, K / 2]`` (two a byte, the lower K in the low
 nibble) and scale atoms ``[ceil(M / 128), 2 ceil(K / 256), 512]``: byte
 ``16 (r % 32) + 4 (r // 32) + j`` of an atom is row ``r``'s scale for the 32 values at
-``32 j`` of the atom's 128; bytes of blocks past K are 0. Activations and weights have the
-same format, so :func:`quantize_rows_mxfp4` serves both.
+``32 j`` of the atom's 128; bytes of blocks past K are 0, bytes of rows past M in the last atom
+are not written (compare scales through :func:`scale_bytes_from_atoms`). Activations and weights
+have the same format, so :func:`quantize_rows_mxfp4` serves both. Where a call allocates both,
+codes and scales are views of one storage: keeping or saving either keeps both (``clone`` parts
+them).
 
 Products are summed in fp32 by the tensor core and rounded once, in the epilogue. An output
 that shares memory with an operand is refused, but for the few that may be an operand itself
@@ -163,4 +166,4 @@ def swiglu_reference(acc: torch.Tensor) -> torch.Tensor:
 
 __all__ = ["quantize_rows_mxfp4", "dequantize_mxfp4", "rmsnorm_mxfp4", "mxfp4_gemm", "mxfp4_linear",
            "mxfp4_gemm_swiglu", "swiglu_lora_b", "quantize_rows_reference", "dequantize_reference",
-           "mxfp4_product_reference", "swiglu_reference", "EPI_STORE", "EPI_RESADD", "SWIGLU_TILE"]
+           "scale_bytes_from_atoms", "mxfp4_product_reference", "swiglu_reference", "EPI_STORE", "EPI_RESADD", "SWIGLU_TILE"]
